@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
 
@@ -27,6 +27,23 @@ def dtype_id(dt: torch.dtype) -> int:
         return _DTYPES[dt]
     except KeyError:
         raise TypeError(f"fast_memory_b200 supports float32, bfloat16 and float16 tensors, got {dt}") from None
+
+
+class LocalAttnArgs(ctypes.Structure):
+    """``fm_local_attn_args``"""
+    _fields_ = ([(n, c_void_p) for n in ("q", "k", "v")] +
+                [(f"{t}_stride_{x}", c_int64) for t in "qkv" for x in ("head", "row")] +
+                [("n_q_rows", c_int64), ("n_k_rows", c_int64)] +
+                [(n, c_int32) for n in ("dtype", "d", "n_q_heads", "n_kv_heads", "n_docs", "window", "causal")] +
+                [("sm_scale", c_float), ("softcap", c_float)] +
+                [(n, c_void_p) for n in ("cu_q", "cu_k", "prefix", "slopes", "page_table", "lengths", "seqs")] +
+                [("page_table_width", c_int64), ("n_pages", c_int64), ("page_size", c_int32), ("n_seqs", c_int32)])
+
+
+class PageCacheArgs(ctypes.Structure):
+    """``fm_page_cache``"""
+    _fields_ = ([(n, c_void_p) for n in ("k_pages", "v_pages", "page_table", "lengths", "refcounts", "status")] +
+                [("n_pages", c_int64), ("width", c_int64)] + [(n, c_int32) for n in ("dtype", "d", "n_heads", "page_size", "n_seqs")])
 
 
 _SIGNATURES = {
@@ -74,6 +91,19 @@ _SIGNATURES = {
                           c_size_t, c_void_p]),
     "fm_unit_rows": (c_int, [c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p]),
     "fm_table_scores": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "fm_local_attn_workspace_bytes": (c_size_t, [POINTER(LocalAttnArgs)]),
+    "fm_local_attn_fwd": (c_int, [POINTER(LocalAttnArgs), c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "fm_local_attn_bwd_workspace_bytes": (c_size_t, [POINTER(LocalAttnArgs)]),
+    "fm_local_attn_bwd": (c_int, [POINTER(LocalAttnArgs), c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_size_t, c_void_p]),
+    "fm_page_cache_workspace_bytes": (c_size_t, [POINTER(PageCacheArgs), c_int64]),
+    "fm_cache_append": (c_int, [POINTER(PageCacheArgs), c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
+                                c_int64, c_void_p, c_size_t, c_void_p]),
+    "fm_cache_fork": (c_int, [POINTER(PageCacheArgs), c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "fm_cache_free": (c_int, [POINTER(PageCacheArgs), c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "fm_cache_compact": (c_int, [POINTER(PageCacheArgs), c_void_p, c_size_t, c_void_p]),
+    "fm_cache_copy_pages": (c_int, [POINTER(PageCacheArgs), c_void_p, c_void_p, c_int64, c_void_p]),
+    "fm_cache_gather": (c_int, [POINTER(PageCacheArgs), c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "fm_gather_mean": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
 }
 

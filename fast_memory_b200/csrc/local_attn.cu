@@ -1,0 +1,207 @@
+// Local attention, entry points and the one-row-a-warp kernels (local_attn.cuh has the mathematics).
+//
+// The row kernels hold a query (or a key) in registers and walk the runs of visible rows, one dot product and one shuffle
+// reduction a pair: no tiles, no masks, fp32 throughout.  They serve what the tiled kernels do not.
+#include "local_attn.cuh"
+
+#include <type_traits>
+
+namespace fm {
+
+namespace {
+
+constexpr int kRowThreads = 256;
+
+template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) local_rows_fwd_kernel(LocalParams p)
+{
+    const int64_t w = (int64_t(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
+    if (w >= int64_t(p.Hq) * p.S) return;
+    const int head = int(w / p.S), r = int(w % p.S);
+    const Doc doc = local_doc(p, p.cu_q ? local_find(p.cu_q, p.n_docs, r) : p.table ? r : 0);
+    local_row_forward<T, D>(p, doc, head, r - doc.q0);
+}
+
+// delta[row] = dO . O - d_lse
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowThreads) local_delta_kernel(LocalParams p, BwdParams g, const T *o, const float *d_lse, float *delta)
+{
+    const int64_t w = (int64_t(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
+    if (w >= int64_t(p.Hq) * p.S) return;
+    RowRegs<T, D> a, b;
+    a.load(o + w * D);
+    b.load(static_cast<const T *>(g.dout) + (w / p.S) * g.do_sh + (w % p.S) * g.do_st);
+    const float x = a.dot(b);
+    if ((threadIdx.x & 31) == 0) delta[w] = x - (d_lse ? d_lse[w] : 0.f);
+}
+
+template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) local_rows_dq_kernel(LocalParams p, BwdParams g)
+{
+    const int64_t w = (int64_t(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
+    if (w >= int64_t(p.Hq) * p.S) return;
+    const int head = int(w / p.S), r = int(w % p.S);
+    const Doc doc = local_doc(p, p.cu_q ? local_find(p.cu_q, p.n_docs, r) : 0);
+    local_row_dq<T, D>(p, g, doc, head, r - doc.q0);
+}
+
+template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) local_rows_dkv_kernel(LocalParams p, BwdParams g)
+{
+    const int64_t w = (int64_t(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
+    if (w >= int64_t(p.H) * p.N) return;
+    const int h = int(w / p.N), r = int(w % p.N);
+    const Doc doc = local_doc<true>(p, p.cu_k ? local_find(p.cu_k, p.n_docs, r) : 0);
+    local_row_dkv<T, D>(p, g, doc, h, r - doc.k0);
+}
+
+inline unsigned row_grid(int64_t rows) { return unsigned(ceil_div(rows * 32, kRowThreads)); }
+
+// f(T{}, std::integral_constant<int, D>{}) for the call's element type and head dim
+template <typename T, typename F> int with_dim(int d, F &&f)
+{
+    switch (d) {
+    case 16: return f(T{}, std::integral_constant<int, 16>{});
+    case 32: return f(T{}, std::integral_constant<int, 32>{});
+    case 64: return f(T{}, std::integral_constant<int, 64>{});
+    case 128: return f(T{}, std::integral_constant<int, 128>{});
+    default: return f(T{}, std::integral_constant<int, 256>{});
+    }
+}
+template <typename F> int with_type(int dtype, int d, F &&f)
+{
+    if (dtype == FM_F32) return with_dim<float>(d, f);
+    if (dtype == FM_BF16) return with_dim<__nv_bfloat16>(d, f);
+    return with_dim<__half>(d, f);
+}
+
+}  // namespace
+
+int local_rows_fwd(const LocalParams &p, int dtype, cudaStream_t st)
+{
+    return with_type(dtype, p.d, [&](auto t, auto dim) -> int {
+        using T = decltype(t);
+        local_rows_fwd_kernel<T, decltype(dim)::value><<<row_grid(int64_t(p.Hq) * p.S), kRowThreads, 0, st>>>(p);
+        FM_LAUNCHED("local_rows_fwd_kernel");
+        return FM_OK;
+    });
+}
+
+int local_rows_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st)
+{
+    return with_type(dtype, p.d, [&](auto t, auto dim) -> int {
+        using T = decltype(t);
+        constexpr int D = decltype(dim)::value;
+        if (p.S > 0) {
+            local_rows_dq_kernel<T, D><<<row_grid(int64_t(p.Hq) * p.S), kRowThreads, 0, st>>>(p, g);
+            FM_LAUNCHED("local_rows_dq_kernel");
+        }
+        if (p.N > 0) {
+            local_rows_dkv_kernel<T, D><<<row_grid(int64_t(p.H) * p.N), kRowThreads, 0, st>>>(p, g);
+            FM_LAUNCHED("local_rows_dkv_kernel");
+        }
+        return FM_OK;
+    });
+}
+
+static int local_params(const fm_local_attn_args *a, LocalParams &p)
+{
+    FM_REQUIRE(a, "local attention: null arguments");
+    FM_REQUIRE(a->dtype == FM_F32 || a->dtype == FM_BF16 || a->dtype == FM_F16, "local attention: unknown element type %d", a->dtype);
+    FM_REQUIRE(a->n_q_rows >= 0 && a->n_q_rows < (int64_t(1) << 30) && a->n_k_rows >= 0 && a->n_k_rows < (int64_t(1) << 30),
+               "local attention: bad row counts %lld, %lld", (long long)a->n_q_rows, (long long)a->n_k_rows);
+    FM_REQUIRE(a->n_kv_heads > 0 && a->n_q_heads > 0 && a->n_q_heads % a->n_kv_heads == 0,
+               "local attention: %d query heads do not share %d KV heads evenly", a->n_q_heads, a->n_kv_heads);
+    FM_REQUIRE(a->n_docs > 0 && a->window >= 0, "local attention: bad document count %d or window %d", a->n_docs, a->window);
+    FM_REQUIRE(a->softcap >= 0.f, "local attention: the cap must not be negative");
+    FM_REQUIRE(int64_t(a->n_q_heads) * a->n_q_rows < (int64_t(1) << 31) && int64_t(a->n_kv_heads) * a->n_k_rows < (int64_t(1) << 31),
+               "local attention: more than 2^31 rows over all heads");
+    if (a->d != 16 && a->d != 32 && a->d != 64 && a->d != 128 && a->d != 256) {
+        set_error("local attention: head dim %d (16, 32, 64, 128 and 256 are built)", a->d);
+        return FM_ERR_UNSUPPORTED;
+    }
+    p = LocalParams{};
+    p.q = a->q; p.k = a->k; p.v = a->v;
+    p.q_sh = a->q_stride_head; p.q_st = a->q_stride_row;
+    p.k_sh = a->k_stride_head; p.k_st = a->k_stride_row;
+    p.v_sh = a->v_stride_head; p.v_st = a->v_stride_row;
+    p.Hq = a->n_q_heads; p.H = a->n_kv_heads; p.G = p.Hq / p.H; p.d = a->d;
+    p.S = int(a->n_q_rows); p.N = int(a->n_k_rows);
+    p.n_docs = a->n_docs;
+    p.cu_q = a->cu_q; p.cu_k = a->cu_k; p.prefix = a->prefix;
+    p.slopes = a->slopes; p.scale = a->sm_scale; p.cap = a->softcap;
+    p.window = a->window; p.causal = a->causal != 0;
+    if (a->page_table) {
+        FM_REQUIRE(a->lengths && a->n_seqs > 0 && a->n_pages > 0 && a->n_pages < (int64_t(1) << 31), "paged attention: lengths, n_seqs and n_pages are needed");
+        int shift = 0;
+        while ((1 << shift) < a->page_size) ++shift;
+        if (a->page_size < 16 || a->page_size > 256 || (1 << shift) != a->page_size) {
+            set_error("paged attention: page size %d (a power of two from 16 to 256)", a->page_size);
+            return FM_ERR_UNSUPPORTED;
+        }
+        FM_REQUIRE(a->page_table_width >= 0 && a->page_table_width < (int64_t(1) << 30 >> shift), "paged attention: page table too wide");
+        FM_REQUIRE(a->cu_q || a->n_q_rows == a->n_docs, "paged attention: one query a sequence without cu_q");
+        p.table = a->page_table; p.lengths = a->lengths; p.seqs = a->seqs;
+        p.table_ld = int(a->page_table_width); p.page_shift = shift; p.n_pages = int(a->n_pages); p.n_seqs = a->n_seqs;
+    } else {
+        FM_REQUIRE(a->n_docs == 1 || (a->cu_q && a->cu_k), "local attention: several documents need cu_q and cu_k");
+    }
+    return FM_OK;
+}
+
+}  // namespace fm
+
+extern "C" {
+
+size_t fm_local_attn_workspace_bytes(const fm_local_attn_args *a) { (void)a; return 256; }
+
+int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *workspace, size_t workspace_bytes, fm_stream_t stream)
+{
+    using namespace fm;
+    LocalParams p;
+    if (int rc = local_params(a, p)) return rc;
+    if (p.S == 0) return FM_OK;
+    FM_REQUIRE(p.q && o && lse && (p.table || p.N == 0 || (p.k && p.v)), "fm_local_attn_fwd: null pointer");
+    (void)workspace; (void)workspace_bytes;
+    p.o = o;
+    p.lse = lse;
+    return local_rows_fwd(p, a->dtype, static_cast<cudaStream_t>(stream));
+}
+
+size_t fm_local_attn_bwd_workspace_bytes(const fm_local_attn_args *a)
+{
+    if (!a || a->n_q_rows < 0 || a->n_q_heads < 0) return 0;
+    return fm::align_up(size_t(a->n_q_heads) * size_t(a->n_q_rows) * sizeof(float), 256) + 256;
+}
+
+int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *lse, const void *d_o, int64_t do_stride_head,
+                      int64_t do_stride_row, const float *d_lse, void *dq, void *dk, void *dv, void *workspace, size_t workspace_bytes,
+                      fm_stream_t stream)
+{
+    using namespace fm;
+    LocalParams p;
+    if (int rc = local_params(a, p)) return rc;
+    if (p.table) {
+        set_error("fm_local_attn_bwd: a paged cache has no backward pass");
+        return FM_ERR_UNSUPPORTED;
+    }
+    if (p.S == 0 && p.N == 0) return FM_OK;
+    FM_REQUIRE(p.S == 0 || (p.q && o && lse && d_o && dq), "fm_local_attn_bwd: null pointer");
+    FM_REQUIRE(p.N == 0 || (p.k && p.v && dk && dv), "fm_local_attn_bwd: null pointer");
+    if (workspace_bytes < fm_local_attn_bwd_workspace_bytes(a) || !workspace) {
+        set_error("fm_local_attn_bwd: workspace of %zu bytes, %zu are needed", workspace_bytes, fm_local_attn_bwd_workspace_bytes(a));
+        return FM_ERR_WORKSPACE;
+    }
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    float *delta = static_cast<float *>(workspace);
+    BwdParams g{d_o, do_stride_head, do_stride_row, lse, delta, dq, dk, dv};
+    if (p.S > 0) {
+        const int rc = with_type(a->dtype, p.d, [&](auto t, auto dim) -> int {
+            using T = decltype(t);
+            local_delta_kernel<T, decltype(dim)::value><<<row_grid(int64_t(p.Hq) * p.S), kRowThreads, 0, st>>>(p, g, static_cast<const T *>(o), d_lse, delta);
+            FM_LAUNCHED("local_delta_kernel");
+            return FM_OK;
+        });
+        if (rc) return rc;
+    }
+    return local_rows_bwd(p, g, a->dtype, st);
+}
+
+}  // extern "C"

@@ -160,6 +160,91 @@ int fm_hashed_attn_bwd(const void *q, const void *k, const void *v, int dtype, i
                        const void *o, const float *lse, const void *d_o, float *dq, float *dk, float *dv, fm_stream_t stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Local attention: the near context that a memory's result is merged with (the `attention_forward` that mem:302 calls
+ * and the reference does not ship), over packed documents or over the pages of a cache.
+ *   p = n_k - n_q + i            position of query i of a document with n_q queries and n_k keys
+ *   s = sm_scale q.k;  if softcap > 0: s = softcap tanh(s / softcap);  if slopes: s -= slopes[head] |p - j|
+ *   key j is visible iff  j < prefix[doc]  or  p - window < j <= p  (causal) / |p - j| < window  (not causal)
+ *   lse = log sum e^s (fp32, natural log), o = sum e^(s - lse) v;  a query that sees nothing: o = 0, lse = -inf
+ * q / k / v have strides in ELEMENTS for head and row (the last dim is contiguous, rows start on 16-byte boundaries);
+ * o [n_q_heads, n_q_rows, d] in `dtype` and lse [n_q_heads, n_q_rows] are contiguous.  cu_q and cu_k
+ * start at 0; query rows behind the last document get o = 0, lse = -inf.  n_q_heads is a multiple of n_kv_heads: heads
+ * [h G, (h+1) G) share KV head h.
+ * Paged (page_table != NULL): k / v are pools [n_pages, n_kv_heads, page_size, d] (strides ignored), document t is sequence
+ * seqs[t] (NULL: t) whose keys lie in pages page_table[seq, 0 ..]; lengths[seq] counts them, the new tokens - the
+ * queries - included; cu_q == NULL: one query a sequence.  page_size is a power of two from 16 to 256.
+ * d: 16, 32, 64, 128, 256.  All arrays are DEVICE arrays; numbers in them that point outside are forced inside.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+    const void *q, *k, *v;
+    int64_t q_stride_head, q_stride_row, k_stride_head, k_stride_row, v_stride_head, v_stride_row;
+    int64_t n_q_rows, n_k_rows;
+    int32_t dtype, d, n_q_heads, n_kv_heads;
+    int32_t n_docs, window, causal;       /* window 0: no bound                                       */
+    float sm_scale, softcap;              /* softcap 0: no cap                                        */
+    const int32_t *cu_q, *cu_k;           /* [n_docs + 1]; NULL: one document                         */
+    const int32_t *prefix;                /* [n_docs] or NULL                                         */
+    const float *slopes;                  /* [n_q_heads] or NULL                                      */
+    const int32_t *page_table, *lengths, *seqs;
+    int64_t page_table_width, n_pages;
+    int32_t page_size, n_seqs;            /* n_seqs: rows of page_table                               */
+} fm_local_attn_args;
+size_t fm_local_attn_workspace_bytes(const fm_local_attn_args *args);
+int fm_local_attn_fwd(const fm_local_attn_args *args, void *o, float *lse, void *workspace, size_t workspace_bytes, fm_stream_t stream);
+
+/* Gradients of fm_local_attn_fwd (documents, not pages): o [n_q_heads, n_q_rows, d] contiguous and lse are the result the
+ * caller ended up with - of this attention alone or merged with a memory's (mem:332, 354-378) -, d_o its gradient (strides
+ * as q's), d_lse [n_q_heads, n_q_rows] fp32 or NULL.  dq / dk / dv: contiguous, in `dtype`, written whole: rows behind the last
+ * document are zero.  dk and dv sum over the heads of a group.  No atomics: the same call gives the same bits. */
+size_t fm_local_attn_bwd_workspace_bytes(const fm_local_attn_args *args);
+int fm_local_attn_bwd(const fm_local_attn_args *args, const void *o, const float *lse, const void *d_o, int64_t do_stride_head,
+                      int64_t do_stride_row, const float *d_lse, void *dq, void *dk, void *dv, void *workspace,
+                      size_t workspace_bytes, fm_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Pages of a cache of keys and values (no counterpart in the reference, which keeps one packed array a layer):
+ * k_pages / v_pages [n_pages, n_heads, page_size, d]; page_table [n_seqs, width] int32, -1 behind a sequence's last page;
+ * lengths [n_seqs]; refcounts [n_pages], 0 = free; status: one int32 that collects the bits below.  DEVICE arrays.
+ * What a call decides (which pages, whether they suffice) is decided on the device: nothing is read back, calls can be
+ * captured.  The r-th page a call asks for is the r-th lowest free one.  A page that is not full has one owner.
+ * A call that fails a check sets its bit in status and changes NOTHING.
+ * Calls on one cache go on one stream, one after the other, each with a workspace that no other call uses meanwhile.
+ * page_size: a power of two from 16 to 256; rows of d elements are a multiple of 16 bytes.
+ * ------------------------------------------------------------------------------------------- */
+#define FM_CACHE_BAD_SEQ 1   /* a sequence out of range or named twice, or prefix sums that do not rise */
+#define FM_CACHE_NO_PAGES 2  /* too few free pages                                                     */
+#define FM_CACHE_TOO_LONG 4  /* a sequence would outgrow its row of the page table                     */
+#define FM_CACHE_NOT_EMPTY 8 /* a fork into a sequence that holds tokens                               */
+typedef struct {
+    void *k_pages, *v_pages;
+    int32_t *page_table, *lengths, *refcounts, *status;
+    int64_t n_pages, width;
+    int32_t dtype, d, n_heads, page_size, n_seqs;
+} fm_page_cache;
+/* for calls over n sequences (compact: 0) */
+size_t fm_page_cache_workspace_bytes(const fm_page_cache *cache, int64_t n);
+/* Sequence seqs[i] grows by rows cu_new[i] .. cu_new[i+1] (NULL: row i) of k_new / v_new [n_heads, n_tokens, d], strides in
+ * elements, rows on 16-byte boundaries.  Rows behind cu_new[n] are not read. */
+int fm_cache_append(const fm_page_cache *cache, const int32_t *seqs, int64_t n, const int32_t *cu_new, const void *k_new, const void *v_new,
+                    int64_t n_tokens, int64_t k_stride_head, int64_t k_stride_row, int64_t v_stride_head, int64_t v_stride_row,
+                    void *workspace, size_t workspace_bytes, fm_stream_t stream);
+/* Empty sequence children[i] becomes a copy of parents[i] as it was before the call: full pages are shared, the rows of a
+ * partial last page copied.  A parent may have several children. */
+int fm_cache_fork(const fm_page_cache *cache, const int32_t *parents, const int32_t *children, int64_t n, void *workspace,
+                  size_t workspace_bytes, fm_stream_t stream);
+/* Empties the sequences; pages without an owner become free. */
+int fm_cache_free(const fm_page_cache *cache, const int32_t *seqs, int64_t n, void *workspace, size_t workspace_bytes, fm_stream_t stream);
+/* With L pages in use, the i-th used page from L on moves to the i-th free page below L; tables and refcounts follow. */
+int fm_cache_compact(const fm_page_cache *cache, void *workspace, size_t workspace_bytes, fm_stream_t stream);
+/* Contents of pages src[i] -> dst[i], K and V (pairs with a page that does not exist are passed over).  The pages of dst
+ * differ from each other and from those of src. */
+int fm_cache_copy_pages(const fm_page_cache *cache, const int32_t *src, const int32_t *dst, int64_t n, fm_stream_t stream);
+/* Rows starts[i] (NULL: 0) .. of sequence seqs[i] as rows cu[i] .. cu[i+1] of k_out / v_out [n_heads, n_tokens, d]; rows the
+ * sequence does not have, and rows that no sequence claims, are zero. */
+int fm_cache_gather(const fm_page_cache *cache, const int32_t *seqs, const int32_t *cu, const int32_t *starts, int64_t n,
+                    int64_t n_tokens, void *k_out, void *v_out, fm_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Shard filter of a globally indexed table: for every (head, bucket) row of k_hashes [C, H, Z] (int64
  * GLOBAL key indices) keep the entries in [lo, hi), rebased to the shard (index - lo), slot order kept,
  * packed (head, bucket, slot) into flat_out (room for C*H*Z entries); counts_out [H, C] int64.

@@ -1,0 +1,377 @@
+"""Local attention and its gradients against their definition in 64 bits (tests/local_reference.py has the bounds)."""
+import pytest
+import torch
+
+import fast_memory_b200 as fm
+from tests.local_reference import Case, assert_within
+
+pytestmark = pytest.mark.gpu
+BF, HF, F = torch.bfloat16, torch.float16, torch.float32
+
+CASES = {
+    "one token": dict(nq=(1,)),
+    "one query, many keys": dict(nq=(1,), nk=(1000,), d=128),
+    "tile edges": dict(nq=(127, 128, 129, 1), d=128, hq=4, h=2),
+    "two tiles and a bit": dict(nq=(257,), nk=(385,), d=128, dtype=HF),
+    "not causal": dict(nq=(140, 60), nk=(200, 300), causal=False),
+    "not causal, window": dict(nq=(300,), nk=(333,), causal=False, window=50, d=128),
+    "window": dict(nq=(500,), window=37),
+    "window of one": dict(nq=(130,), window=1, d=128),
+    "window, many tiles": dict(nq=(1100,), window=300, d=128, hq=3, h=3),
+    "more queries than keys": dict(nq=(200, 90), nk=(70, 0)),            # the first queries see nothing
+    "more queries than keys, not causal": dict(nq=(200, 3), nk=(70, 0), causal=False, window=90),
+    "empty documents": dict(nq=(0, 50, 0, 3, 0), nk=(0, 60, 5, 3, 0)),
+    "tail": dict(nq=(33, 90), tail=45, d=128),
+    "prefix": dict(nq=(150, 200, 20), prefix=(40, 0, 999), window=16, d=128),
+    "prefix beyond the window": dict(nq=(400,), nk=(700,), prefix=(130,), window=100, d=128, softcap=20.0),
+    "capped": dict(nq=(260,), softcap=5.0, d=128, scale=0.3),
+    "distance": dict(nq=(300,), slopes=True, hq=4, h=1, d=128),
+    "distance, capped, not causal": dict(nq=(90, 150), slopes=True, softcap=15.0, causal=False, hq=6, h=2),
+    "group of seven": dict(nq=(50, 141), hq=7, h=1, d=128),
+    "group of three, two heads": dict(nq=(70, 1, 200), nk=(170, 30, 200), hq=6, h=2, dtype=HF),
+    "token major": dict(nq=(200, 111), token_major=True, hq=4, h=2, d=128),
+    "fp32": dict(nq=(70, 200), dtype=F, d=64, hq=2, h=1, slopes=True),
+    "fp32, d 128": dict(nq=(131,), nk=(300,), dtype=F, d=128, window=100, softcap=10.0, prefix=(7,)),
+    "fp32 token major": dict(nq=(65, 1), dtype=F, token_major=True, hq=4, h=2),
+    "d 16": dict(nq=(100,), d=16),
+    "d 32": dict(nq=(100, 30), d=32, dtype=HF),
+    "d 256": dict(nq=(90,), nk=(140,), d=256),
+    "many documents": dict(nq=tuple((i * 7) % 11 for i in range(70)), nk=tuple((i * 5) % 13 for i in range(70)), hq=2, h=2, d=128),
+    "large logits": dict(nq=(300,), d=128, scale=1.0),
+}
+
+
+def _run(c, **kw):
+    return fm.local_attention(c.q, c.k, c.v, c.scale, **(kw or c.kwargs()))
+
+
+@pytest.mark.parametrize("name", CASES)
+def test_forward(name):
+    c = Case(**CASES[name])
+    o, lse = _run(c)
+    assert o.dtype == c.dtype and lse.dtype == torch.float32 and o.shape == c.q.shape and lse.shape == c.q.shape[:2]
+    ro, rl, to, tl = c.forward()
+    assert_within(lse, rl, tl, "lse")
+    assert_within(o, ro, to, "o")
+    blind = torch.isinf(rl)
+    assert (o[blind] == 0).all()
+    if len(c.nq) == 1 and c.q.shape[1] == c.nq[0]:
+        o2, lse2 = _run(c, **c.kwargs(plain=True))
+        assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("with_lse", [False, True])
+@pytest.mark.parametrize("name", CASES)
+def test_backward(name, with_lse):
+    c = Case(**CASES[name], seed=3)
+    o, lse = _run(c)
+    d_lse = c.d_lse if with_lse else None
+    grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, d_lse=d_lse, **c.kwargs())
+    for got, (want, bound), what in zip(grads, c.backward(o, lse, d_lse), ("dq", "dk", "dv")):
+        assert got.dtype == c.dtype
+        assert_within(got, want, bound, what)
+    again = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, d_lse=d_lse, **c.kwargs())
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64), (F, 64)])
+def test_random_calls(dtype, d):
+    import random
+    rng = random.Random(17)
+    for n in range(12):
+        h, g = rng.choice([(1, 1), (2, 2), (1, 5), (3, 1)])
+        docs = rng.randint(1, 5)
+        nq = [rng.choice([0, 1, 17, 63, 64, 130, 300]) for _ in range(docs)]
+        c = Case(dtype=dtype, d=d, hq=h * g, h=h, nq=nq, nk=[x + rng.choice([0, 0, 5, 128, 333]) for x in nq], causal=rng.random() < 0.7,
+                 window=rng.choice([0, 0, 3, 64, 129, 200]), softcap=rng.choice([0.0, 12.0]), slopes=rng.random() < 0.4,
+                 prefix=[rng.randint(0, 150) for _ in range(docs)] if rng.random() < 0.4 else None, token_major=rng.random() < 0.3,
+                 tail=rng.choice([0, 9]), seed=n)
+        o, lse = _run(c)
+        ro, rl, to, tl = c.forward()
+        assert_within(lse, rl, tl, f"lse of call {n}")
+        assert_within(o, ro, to, f"o of call {n}")
+        grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+        for got, (want, bound), what in zip(grads, c.backward(o, lse), ("dq", "dk", "dv")):
+            assert_within(got, want, bound, f"{what} of call {n}")
+
+
+def _assert_rows(got, want, bound, rows, name):
+    assert_within(got[:, rows], want[:, rows], bound[:, rows], name)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F, 64)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf"), torch.finfo(torch.float16).min])
+def test_hidden_values_take_no_part(dtype, d, bad):
+    """Keys, values, queries and output gradients that a row does not see may hold anything."""
+    c = Case(dtype=dtype, d=d, hq=2, h=1, nq=(100, 60, 200), window=70, tail=20, seed=8)
+    clean = [t.clone() for t in (c.q, c.k, c.v, c.d_out)]
+    o0, lse0 = _run(c)
+    ro, rl, to, tl = c.forward()
+    g0 = c.backward(o0, lse0)
+    # document 1, the tail, and the last position of document 2 (which only its own query sees)
+    for t in (c.q, c.k, c.v, c.d_out):
+        t[:, 100:160] = bad
+        t[:, 360:] = bad
+    c.k[:, 359] = bad
+    c.v[:, 359] = bad
+    o, lse = _run(c)
+    rows = torch.ones(380, dtype=torch.bool, device="cuda")
+    rows[100:160] = rows[359:] = False
+    _assert_rows(o, ro, to, rows, "o")
+    _assert_rows(lse, rl, tl, rows, "lse")
+    assert (o[:, 360:] == 0).all() and torch.isinf(lse[:, 360:]).all()
+    if bad != bad:
+        assert torch.isnan(o[:, 359]).all() and torch.isnan(o[:, 101:160]).all()
+    o1, lse1 = o0.clone(), lse0.clone()                    # what the caller has: the clean rows, and what became of the others
+    o1[:, 100:160], lse1[:, 100:160] = o[:, 100:160], lse[:, 100:160]
+    c.k[:, 359], c.v[:, 359] = clean[1][:, 359], clean[2][:, 359]
+    grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o1, lse1, c.d_out, **c.kwargs())
+    rows[359] = True
+    for got, (want, bound), name in zip(grads, g0, ("dq", "dk", "dv")):
+        _assert_rows(got, want, bound, rows, name)
+        assert (got[:, 360:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64)])
+def test_one_bad_value_reaches_the_rows_that_see_it(dtype, d):
+    c = Case(dtype=dtype, d=d, nq=(300,), seed=2)
+    o0, lse0 = _run(c)
+    ro, rl, to, tl = c.forward()
+    g0 = c.backward(o0, lse0)
+    c.v[0, 150, 7] = float("nan")
+    o, lse = _run(c)
+    at = torch.arange(300, device="cuda")
+    assert_within(lse, rl, tl, "lse")
+    _assert_rows(o, ro, to, at < 150, "o")
+    assert torch.isnan(o[:, 150:, 7]).all()
+    assert torch.isfinite(o[:, :, :7]).all() and torch.isfinite(o[:, :, 8:]).all()
+    c = Case(dtype=dtype, d=d, nq=(300,), seed=2)
+    c.d_out[1, 40, 3] = float("nan")                       # keys up to 40 get it, dv in column 3 only
+    dq, dk, dv = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o0, lse0, c.d_out, **c.kwargs())
+    assert torch.isnan(dv[:, :41, 3]).all() and torch.isfinite(dv[:, :41, 4:]).all()
+    _assert_rows(dk, *g0[1], at > 40, "dk")
+    _assert_rows(dv, *g0[2], at > 40, "dv")
+    assert torch.isnan(dk[:, :41]).all() and torch.isnan(dq[1, 40]).all() and torch.isfinite(dq[0]).all()
+
+
+def test_gradient_against_differences():
+    """The directional derivative of a loss over o and lse, by central differences of the fp32 operator: h = 2^-7 leaves an
+    error of h^2 / 6 of the third derivative and 2^-24 |loss| / h of rounding, together well under 1e-2 of the derivative."""
+    c = Case(dtype=F, d=32, hq=4, h=2, nq=(40, 60), nk=(50, 75), window=30, softcap=8.0, slopes=True, prefix=(5, 0), seed=4)
+    kw = c.kwargs()
+    g = torch.Generator().manual_seed(9)
+    dirs = [torch.randn(t.shape, generator=g).cuda() / t.numel() ** 0.5 for t in (c.q, c.k, c.v)]
+
+    def loss(q, k, v):
+        o, lse = fm.local_attention(q, k, v, c.scale, **kw)
+        return (o.double() * c.d_out.double()).sum() + (lse.double() * c.d_lse.double()).sum()
+
+    leaves = [t.clone().requires_grad_() for t in (c.q, c.k, c.v)]
+    loss(*leaves).backward()
+    for i, x in enumerate(dirs):
+        h = 2.0 ** -7
+        moved = [[t + s * h * (x if j == i else 0) for j, t in enumerate((c.q, c.k, c.v))] for s in (1, -1)]
+        diff = float(loss(*moved[0]) - loss(*moved[1])) / (2 * h)
+        want = float((leaves[i].grad.double() * x.double()).sum())
+        assert abs(diff - want) <= 1e-2 * abs(want) + 2.0 ** -24 * 1000 / h * 4, (i, diff, want)
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F, 64)])
+def test_autograd_is_the_explicit_backward(dtype, d):
+    c = Case(dtype=dtype, d=d, hq=4, h=2, nq=(90, 80), seed=6)
+    leaves = [t.detach().clone().requires_grad_() for t in (c.q, c.k, c.v)]
+    o, lse = fm.local_attention(*leaves, c.scale, **c.kwargs())
+    ((o * c.d_out).sum() + (lse * c.d_lse).sum()).backward()
+    o2, lse2 = _run(c)
+    assert torch.equal(o, o2) and torch.equal(lse, lse2)
+    want = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o2, lse2, c.d_out, d_lse=c.d_lse, **c.kwargs())
+    assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+    # a loss that reads one result only; an expanded output gradient
+    leaves = [t.detach().clone().requires_grad_() for t in (c.q, c.k, c.v)]
+    o, lse = fm.local_attention(*leaves, c.scale, **c.kwargs())
+    o.sum().backward()
+    want = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o2, lse2, torch.ones_like(o2), **c.kwargs())
+    assert all(torch.equal(t.grad, w) for t, w in zip(leaves, want))
+    leaves = [t.detach().clone().requires_grad_() for t in (c.q, c.k, c.v)]
+    _, lse = fm.local_attention(*leaves, c.scale, **c.kwargs())
+    lse.sum().backward()
+    assert torch.equal(leaves[2].grad, torch.zeros_like(leaves[2]))
+
+
+def test_registered_operators():
+    c = Case(d=64, nq=(40, 30), hq=2, h=1)
+    kw = c.kwargs()
+    cu = kw["cu_seqlens_q"]
+    args = (c.q.clone().requires_grad_(), c.k, c.v, c.scale, True, 0, 0.0, None, cu, cu, None)
+    torch.library.opcheck(torch.ops.fast_memory_b200.local_attention.default, args,
+                          test_utils=("test_schema", "test_autograd_registration", "test_faketensor"))
+    o, lse = _run(c)
+    torch.library.opcheck(torch.ops.fast_memory_b200.local_attention_backward.default,
+                          (c.q, c.k, c.v, o, lse, c.d_out, None, c.scale, True, 0, 0.0, None, cu, cu, None),
+                          test_utils=("test_schema", "test_faketensor"))
+    compiled = torch.compile(lambda q, k, v: fm.local_attention(q, k, v, c.scale, **kw), backend="aot_eager")(c.q, c.k, c.v)
+    assert torch.equal(compiled[0], o) and torch.equal(compiled[1], lse)
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_strides_alignment_and_views(dtype):
+    """Any layout gives what its contiguous copy gives."""
+    c = Case(dtype=dtype, d=64, hq=4, h=2, nq=(150,), seed=5)
+    o0, lse0 = _run(c)
+    g0 = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o0, lse0, c.d_out, **c.kwargs())
+
+    def offset(t):                                         # rows that start off the 16-byte grid
+        buf = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape)
+        return buf.copy_(t)
+
+    def columns(t):                                        # the last dim is not contiguous
+        return t.transpose(1, 2).contiguous().transpose(1, 2)
+
+    def sliced(t):                                         # part of a wider projection, [tokens, heads, 2 d]
+        wide = torch.full((t.shape[1], t.shape[0], 2 * t.shape[2]), float("nan"), dtype=t.dtype, device="cuda")
+        wide[..., :t.shape[2]] = t.transpose(0, 1)
+        return wide[..., :t.shape[2]].transpose(0, 1)
+
+    for f in (offset, columns, sliced):
+        q, k, v, g = (f(t) for t in (c.q, c.k, c.v, c.d_out))
+        o, lse = fm.local_attention(q, k, v, c.scale, **c.kwargs())
+        assert torch.equal(o, o0) and torch.equal(lse, lse0)
+        for got, want in zip(fm.local_attention_backward(q, k, v, c.scale, o, lse, g, **c.kwargs()), g0):
+            assert torch.equal(got, want)
+    one = c.v[:1, :, :].expand(2, -1, -1)                  # shared by broadcasting
+    o, _ = fm.local_attention(c.q, c.k, one, c.scale, **c.kwargs())
+    o1, _ = fm.local_attention(c.q, c.k, one.contiguous(), c.scale, **c.kwargs())
+    assert torch.equal(o, o1)
+
+
+def test_gradient_of_a_broadcast_input():
+    c = Case(d=64, hq=2, h=2, nq=(100,), seed=5)
+    v = c.v[:1].clone().requires_grad_()
+    o, lse = fm.local_attention(c.q, c.k, v.expand(2, -1, -1), c.scale)
+    (o * c.d_out).sum().backward()
+    _, _, dv = fm.local_attention_backward(c.q, c.k, v.detach().expand(2, -1, -1), c.scale, o.detach(), lse.detach(), c.d_out)
+    assert torch.equal(v.grad, dv.sum(0, keepdim=True))
+
+
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (F, 64)])
+def test_captured_and_replayed(dtype, d):
+    """Two graphs, replayed on two streams at once with new inputs and new documents, and an eager call beside them."""
+    cases = [Case(dtype=dtype, d=d, hq=4, h=2, nq=(300, 100), window=90, seed=i) for i in range(2)]
+    graphs, outs, kws = [], [], []
+    for c in cases:
+        kw = c.kwargs()
+        o, lse = fm.local_attention(c.q, c.k, c.v, c.scale, **kw)                    # first call outside the capture
+        fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **kw)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o, lse = fm.local_attention(c.q, c.k, c.v, c.scale, **kw)
+            grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **kw)
+        graphs.append(g)
+        outs.append((o, lse, *grads))
+        kws.append(kw)
+    fresh = [Case(dtype=dtype, d=d, hq=4, h=2, nq=(170, 230), window=90, seed=10 + i) for i in range(2)]
+    for c, f, kw in zip(cases, fresh, kws):
+        for name in ("q", "k", "v", "d_out"):
+            getattr(c, name).copy_(getattr(f, name))
+        kw["cu_seqlens_q"].copy_(f.kwargs()["cu_seqlens_q"])
+        kw["cu_seqlens_k"].copy_(f.kwargs()["cu_seqlens_k"])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = fm.local_attention(fresh[0].q, fresh[0].k, fresh[0].v, fresh[0].scale, **fresh[0].kwargs())
+    torch.cuda.synchronize()
+    for f, got in zip(fresh, outs):
+        o, lse = _run(f)
+        want = (o, lse, *fm.local_attention_backward(f.q, f.k, f.v, f.scale, o, lse, f.d_out, **f.kwargs()))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(eager[0], outs[0][0])
+
+
+def test_merged_with_a_memory():
+    """Local attention over new keys and a memory of old ones, merged, is attention over both; the gradients of the merged
+    result come from the two backward passes with the merged (out, lse)."""
+    H, G, N, S, d, C = 2, 2, 512, 160, 64, 4
+    g = torch.Generator().manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=g).bfloat16().cuda()
+    k_old, v_old, k, v, q, d_out = rnd(H, N, d), rnd(H, N, d), rnd(H, S, d), rnd(H, S, d), rnd(H * G, S, d), rnd(H * G, S, d)
+    sm = d ** -0.5
+    mem = fm.Memory.build(k_old, v_old, A=rnd(H, C, d), bucket_size=N)                 # every bucket holds every key
+    o_l, lse_l = fm.local_attention(q, k, v, sm, window=50)
+    o_m, lse_m = mem.query(q, sm)
+    out, lse = fm.merge(o_l, lse_l, o_m, lse_m)
+    dq_l, dk, dv = fm.local_attention_backward(q, k, v, sm, out.bfloat16(), lse, d_out, window=50)
+    dq_m, dk_old, dv_old = mem.query_backward(q, sm, out.bfloat16(), lse, d_out)
+    # dense in 64 bits
+    x = [t.double().requires_grad_() for t in (q, k, v, k_old, v_old)]
+    keys, vals = torch.cat([x[3], x[1]], 1).repeat_interleave(G, 0), torch.cat([x[4], x[2]], 1).repeat_interleave(G, 0)
+    i, j = torch.arange(S, device="cuda")[:, None], torch.arange(S, device="cuda")[None, :]
+    mask = torch.cat([torch.ones(S, N, dtype=torch.bool, device="cuda"), (j <= i) & (j > i - 50)], 1)
+    s = (x[0] @ keys.transpose(1, 2) * sm).masked_fill(~mask, float("-inf"))
+    ref = torch.softmax(s, -1) @ vals
+    (ref * d_out.double()).sum().backward()
+    # bf16 results of size <= 1 over weights that sum to one: two roundings of each part, 2^-8 each, of |o| <= max|v|
+    u = 2.0 ** -8
+    ref = ref.detach()
+    assert (out.double() - ref).abs().max() <= 3 * u * float(vals.detach().abs().max()) / 4
+    assert (lse.double() - torch.logsumexp(s, -1)).abs().max() <= 1e-3
+    for got, want in ((dq_l.double() + dq_m.double(), x[0].grad), (dk.double(), x[1].grad), (dv.double(), x[2].grad),
+                      (dk_old.double(), x[3].grad), (dv_old.double(), x[4].grad)):
+        # every term is rounded to 2^-8 of itself; the terms of a row sum to at most this multiple of the largest gradient
+        assert (got - want).abs().max() <= 8 * u * float(want.abs().max())
+
+
+def test_refusals():
+    c = Case(d=64, nq=(40,), hq=2, h=1)
+    q, k, v, s = c.q, c.k, c.v, c.scale
+    o, lse = fm.local_attention(q, k, v, s)
+    cases = [
+        (ValueError, lambda: fm.local_attention(q[0], k, v, s)),
+        (ValueError, lambda: fm.local_attention(q, k, v[:, :-1], s)),
+        (TypeError, lambda: fm.local_attention(q, k.half(), v.half(), s)),
+        (TypeError, lambda: fm.local_attention(q.double(), k.double(), v.double(), s)),
+        (ValueError, lambda: fm.local_attention(torch.cat([q, q[:1]]), torch.cat([k, k]), torch.cat([v, v]), s)),
+        (fm.FastMemError, lambda: fm.local_attention(q[..., :48].contiguous(), k[..., :48].contiguous(), v[..., :48].contiguous(), s)),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, window=-1)),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, window=2.5)),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, softcap=-1.0)),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, softcap=float("nan"))),
+        (TypeError, lambda: fm.local_attention(q, k, v, s, slopes=torch.ones(1, device="cuda"))),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, slopes=torch.ones(2, device="cuda", requires_grad=True))),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, slopes=torch.ones(2))),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, cu_seqlens_k=[0, 40])),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, cu_seqlens_q=[0, 41])),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, cu_seqlens_q=[0, 20, 10])),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, cu_seqlens_q=[0, 20, 40], cu_seqlens_k=[0, 40])),
+        (ValueError, lambda: fm.local_attention(q, k[:, :30], v[:, :30], s, cu_seqlens_q=[0, 40])),
+        (TypeError, lambda: fm.local_attention(q, k, v, s, cu_seqlens_q=torch.tensor([0.0, 40.0], device="cuda"))),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, cu_seqlens_q=torch.tensor([0, 40]))),
+        (ValueError, lambda: fm.local_attention(q, k, v, s, prefix=[1, 2])),
+        (fm.FastMemError, lambda: fm.local_attention(q.cpu(), k, v, s)),
+        (TypeError, lambda: fm.local_attention_backward(q, k, v, s, o.float(), lse, c.d_out)),
+        (TypeError, lambda: fm.local_attention_backward(q, k, v, s, o, lse.bfloat16(), c.d_out)),
+        (ValueError, lambda: fm.local_attention_backward(q, k, v, s, o, lse[:1], c.d_out)),
+        (ValueError, lambda: fm.local_attention_backward(q, k, v, s, o, lse, c.d_out[:, :20])),
+    ]
+    for n, (error, call) in enumerate(cases):
+        with pytest.raises(error):
+            call()
+            print("call", n, "was not refused")
+    assert fm.local_attention(q[:, :0], k, v, s)[0].shape == (2, 0, 64)
+    o, lse = fm.local_attention(q, k[:, :0], v[:, :0], s)
+    assert (o == 0).all() and torch.isinf(lse).all()
+    dq, dk, dv = fm.local_attention_backward(q, k[:, :0], v[:, :0], s, o, lse, c.d_out)
+    assert (dq == 0).all() and dk.shape == (1, 0, 64)
+
+
+def test_wrong_prefix_sums_stay_inside_the_arrays():
+    """Numbers on the device cannot be checked by the host: they are forced into the arrays."""
+    c = Case(d=64, nq=(200,), hq=2, h=1)
+    for cu in ([0, 150, 90, 400], [0, -5, 2 ** 30, 200], [7, 50, 60, 70], [0, 200, 200, 200]):
+        t = torch.tensor(cu, dtype=torch.int32, device="cuda")
+        o, lse = fm.local_attention(c.q, c.k, c.v, c.scale, cu_seqlens_q=t, cu_seqlens_k=t, prefix=torch.tensor([-4, 1000, 3], device="cuda"))
+        fm.local_attention_backward(c.q, c.k, c.v, c.scale, torch.zeros_like(o), torch.zeros_like(lse), c.d_out, cu_seqlens_q=t, cu_seqlens_k=t)
+    torch.cuda.synchronize()

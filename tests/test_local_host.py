@@ -1,0 +1,101 @@
+"""Refusals of the local attention and page cache entry points that need no GPU: every argument is checked before any CUDA call."""
+import ctypes
+
+import pytest
+import torch
+
+import fast_memory_b200 as fm
+from fast_memory_b200 import _lib as L
+
+FAKE = 1 << 20            # an address that is only ever compared with null
+
+
+def _attn(**kw):
+    a = L.LocalAttnArgs(q=FAKE, k=FAKE, v=FAKE, q_stride_head=640, q_stride_row=64, k_stride_head=640, k_stride_row=64, v_stride_head=640,
+                        v_stride_row=64, n_q_rows=10, n_k_rows=10, dtype=L.BF16, d=64, n_q_heads=2, n_kv_heads=1, n_docs=1, window=0, causal=1,
+                        sm_scale=1.0, softcap=0.0)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+BAD = -1
+UNSUPPORTED = -2
+WORKSPACE = -3
+
+
+@pytest.mark.parametrize("kw,status,text", [
+    (dict(dtype=7), BAD, "element type"), (dict(d=48), UNSUPPORTED, "head dim"), (dict(n_q_heads=3, n_kv_heads=2), BAD, "evenly"),
+    (dict(n_kv_heads=0), BAD, "evenly"), (dict(n_docs=0), BAD, "document"), (dict(window=-1), BAD, "window"), (dict(softcap=-1.0), BAD, "cap"),
+    (dict(n_q_rows=-1), BAD, "row counts"), (dict(n_q_rows=1 << 30), BAD, "row counts"), (dict(n_docs=2), BAD, "cu_q"),
+    (dict(n_q_heads=1 << 20, n_q_rows=1 << 20), BAD, "2^31"), (dict(q=None), BAD, "null"), (dict(k=None), BAD, "null"),
+    (dict(page_table=FAKE), BAD, "lengths"),
+    (dict(page_table=FAKE, lengths=FAKE, n_seqs=1, n_pages=1, page_size=24, page_table_width=1, cu_q=FAKE), UNSUPPORTED, "page size"),
+    (dict(page_table=FAKE, lengths=FAKE, n_seqs=1, n_pages=1, page_size=16, page_table_width=1 << 29, cu_q=FAKE), BAD, "too wide"),
+    (dict(page_table=FAKE, lengths=FAKE, n_seqs=1, n_pages=1, page_size=16, page_table_width=1), BAD, "one query a sequence"),
+])
+def test_forward_refuses(kw, status, text):
+    lib = L.lib()
+    rc = lib.fm_local_attn_fwd(ctypes.byref(_attn(**kw)), FAKE, FAKE, FAKE, 1 << 30, None)
+    assert rc == status and text.encode() in lib.fm_last_error(), lib.fm_last_error()
+
+
+def test_other_refusals():
+    lib = L.lib()
+    ref = ctypes.byref
+    assert lib.fm_local_attn_fwd(None, FAKE, FAKE, FAKE, 1 << 30, None) == BAD
+    assert lib.fm_local_attn_fwd(ref(_attn()), None, FAKE, FAKE, 1 << 30, None) == BAD
+    assert lib.fm_local_attn_fwd(ref(_attn(n_q_rows=0)), None, None, None, 0, None) == 0            # nothing to do
+    assert lib.fm_local_attn_bwd(ref(_attn()), FAKE, FAKE, FAKE, 640, 64, None, FAKE, FAKE, FAKE, FAKE, 8, None) == WORKSPACE
+    assert lib.fm_local_attn_bwd(ref(_attn()), FAKE, FAKE, FAKE, 640, 64, None, FAKE, None, FAKE, FAKE, 1 << 30, None) == BAD
+    paged = _attn(page_table=FAKE, lengths=FAKE, n_seqs=1, n_pages=1, page_size=16, page_table_width=1, cu_q=FAKE)
+    assert lib.fm_local_attn_bwd(ref(paged), FAKE, FAKE, FAKE, 640, 64, None, FAKE, FAKE, FAKE, FAKE, 1 << 30, None) == UNSUPPORTED
+
+
+def _cache(**kw):
+    a = L.PageCacheArgs(k_pages=FAKE, v_pages=FAKE, page_table=FAKE, lengths=FAKE, refcounts=FAKE, status=FAKE, n_pages=4, width=2,
+                        dtype=L.BF16, d=64, n_heads=1, page_size=16, n_seqs=3)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+@pytest.mark.parametrize("kw,status,text", [
+    (dict(k_pages=None), BAD, "null"), (dict(status=None), BAD, "null"), (dict(dtype=9), BAD, "element type"), (dict(n_pages=0), BAD, "sizes"),
+    (dict(page_size=8), UNSUPPORTED, "page size"), (dict(page_size=512), UNSUPPORTED, "page size"), (dict(page_size=0), UNSUPPORTED, "page size"),
+    (dict(d=12), UNSUPPORTED, "multiple of 16"), (dict(k_pages=FAKE + 8), BAD, "aligned"), (dict(width=1 << 40), BAD, "wide"),
+])
+def test_cache_refuses(kw, status, text):
+    lib = L.lib()
+    c = ctypes.byref(_cache(**kw))
+    calls = [lib.fm_cache_append(c, FAKE, 1, FAKE, FAKE, FAKE, 1, 64, 64, 64, 64, FAKE, 1 << 30, None),
+             lib.fm_cache_fork(c, FAKE, FAKE, 1, FAKE, 1 << 30, None), lib.fm_cache_free(c, FAKE, 1, FAKE, 1 << 30, None),
+             lib.fm_cache_compact(c, FAKE, 1 << 30, None), lib.fm_cache_copy_pages(c, FAKE, FAKE, 1, None),
+             lib.fm_cache_gather(c, FAKE, FAKE, None, 1, 1, FAKE, FAKE, None)]
+    assert calls == [status] * 6 and text.encode() in lib.fm_last_error(), lib.fm_last_error()
+
+
+def test_cache_calls_refuse():
+    lib = L.lib()
+    c = ctypes.byref(_cache())
+    need = lib.fm_page_cache_workspace_bytes(c, 2)
+    assert lib.fm_cache_append(c, FAKE, 2, FAKE, FAKE, FAKE, 5, 64, 64, 64, 64, FAKE, need - 1, None) == WORKSPACE
+    assert lib.fm_cache_append(c, FAKE, 4, FAKE, FAKE, FAKE, 5, 64, 64, 64, 64, FAKE, 1 << 30, None) == BAD      # more than there are
+    assert lib.fm_cache_append(c, FAKE, 2, None, FAKE, FAKE, 5, 64, 64, 64, 64, FAKE, need, None) == BAD         # one token each
+    assert lib.fm_cache_append(c, FAKE, 2, FAKE, FAKE, FAKE, 5, 64, 60, 64, 64, FAKE, need, None) == BAD         # rows off the 16-byte grid
+    assert lib.fm_cache_append(c, FAKE, 0, None, None, None, 0, 64, 64, 64, 64, None, 0, None) == 0
+    assert lib.fm_cache_fork(c, FAKE, FAKE, 2, FAKE, need - 1, None) == WORKSPACE
+    assert lib.fm_cache_free(c, None, 2, FAKE, need, None) == BAD
+    assert lib.fm_cache_free(c, FAKE, 2, FAKE, need - 1, None) == WORKSPACE
+
+
+def test_cpu_tensors_are_refused():
+    q = torch.zeros(1, 4, 64)
+    with pytest.raises(fm.FastMemError):
+        fm.local_attention(q, q, q, 1.0)
+    with pytest.raises(fm.FastMemError):
+        fm.local_attention_backward(q, q, q, 1.0, q, q[..., 0], q)
+    with pytest.raises(fm.FastMemError):
+        fm.PagedCache(1, 64, n_pages=2, n_seqs=1, max_len=10, device="cpu")
+    with pytest.raises(fm.FastMemError):
+        fm.paged_attention(q, q[None], q[None], torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), 1.0)
