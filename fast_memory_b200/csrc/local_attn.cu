@@ -2,7 +2,7 @@
 //
 // The row kernels hold a query (or a key) in registers and walk the runs of visible rows, one dot product and one shuffle
 // reduction a pair: no tiles, no masks, fp32 throughout.  They serve what the tiled kernels do not.
-#include "local_attn.cuh"
+#include "local_tc.cuh"
 
 #include <type_traits>
 
@@ -117,6 +117,10 @@ static int local_params(const fm_local_attn_args *a, LocalParams &p)
         set_error("local attention: head dim %d (16, 32, 64, 128 and 256 are built)", a->d);
         return FM_ERR_UNSUPPORTED;
     }
+    const int e = elem_bytes(a->dtype);
+    uintptr_t grid = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v);
+    grid |= uintptr_t((a->q_stride_head | a->q_stride_row | a->k_stride_head | a->k_stride_row | a->v_stride_head | a->v_stride_row) * e);
+    FM_REQUIRE(grid % 16 == 0, "local attention: rows must start on 16-byte boundaries");
     p = LocalParams{};
     p.q = a->q; p.k = a->k; p.v = a->v;
     p.q_sh = a->q_stride_head; p.q_st = a->q_stride_row;
@@ -150,7 +154,11 @@ static int local_params(const fm_local_attn_args *a, LocalParams &p)
 
 extern "C" {
 
-size_t fm_local_attn_workspace_bytes(const fm_local_attn_args *a) { (void)a; return 256; }
+size_t fm_local_attn_workspace_bytes(const fm_local_attn_args *a)
+{
+    fm::LocalParams p;
+    return fm::local_params(a, p) ? 0 : fm::local_tc_fwd_workspace(p, a->dtype) + 256;
+}
 
 int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *workspace, size_t workspace_bytes, fm_stream_t stream)
 {
@@ -159,10 +167,16 @@ int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *wo
     if (int rc = local_params(a, p)) return rc;
     if (p.S == 0) return FM_OK;
     FM_REQUIRE(p.q && o && lse && (p.table || p.N == 0 || (p.k && p.v)), "fm_local_attn_fwd: null pointer");
-    (void)workspace; (void)workspace_bytes;
+    if (workspace_bytes < fm_local_attn_workspace_bytes(a) || !workspace) {
+        set_error("fm_local_attn_fwd: workspace of %zu bytes, %zu are needed", workspace_bytes, fm_local_attn_workspace_bytes(a));
+        return FM_ERR_WORKSPACE;
+    }
+    FM_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0, "fm_local_attn_fwd: misaligned buffer");
     p.o = o;
     p.lse = lse;
-    return local_rows_fwd(p, a->dtype, static_cast<cudaStream_t>(stream));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (local_tc_fits(p, a->dtype)) return local_tc_fwd(p, a->dtype, workspace, workspace_bytes, st);
+    return local_rows_fwd(p, a->dtype, st);
 }
 
 size_t fm_local_attn_bwd_workspace_bytes(const fm_local_attn_args *a)
@@ -189,6 +203,8 @@ int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *l
         set_error("fm_local_attn_bwd: workspace of %zu bytes, %zu are needed", workspace_bytes, fm_local_attn_bwd_workspace_bytes(a));
         return FM_ERR_WORKSPACE;
     }
+    FM_REQUIRE((reinterpret_cast<uintptr_t>(d_o) | reinterpret_cast<uintptr_t>(o) | uintptr_t((do_stride_head | do_stride_row) * elem_bytes(a->dtype))) % 16 == 0,
+               "fm_local_attn_bwd: rows must start on 16-byte boundaries");
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     float *delta = static_cast<float *>(workspace);
     BwdParams g{d_o, do_stride_head, do_stride_row, lse, delta, dq, dk, dv};

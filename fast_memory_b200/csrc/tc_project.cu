@@ -300,27 +300,39 @@ static EncodeTiledFn encode_tiled_fn()
     return fn;
 }
 
-int make_tensor_map_2d(CUtensorMap *map, const void *base_ptr, int dtype, uint64_t rows, uint64_t d, uint64_t row_stride_bytes,
-                       uint32_t box_rows)
+int make_tensor_map(CUtensorMap *map, const void *base_ptr, int dtype, int rank, const uint64_t *dims, const uint64_t *stride_bytes,
+                    const uint32_t *box)
 {
     EncodeTiledFn fn = encode_tiled_fn();
     if (!fn) {
         set_error("cuTensorMapEncodeTiled is not available from the driver");
         return FM_ERR_CUDA;
     }
-    cuuint64_t dims[2] = {d, rows};
-    cuuint64_t strides[1] = {row_stride_bytes};
-    cuuint32_t box[2] = {64, box_rows};
-    cuuint32_t estr[2] = {1, 1};
-    CUresult r = fn(map, dtype == FM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
-                    const_cast<void *>(base_ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    cuuint64_t d[5], s[4];
+    cuuint32_t b[5], estr[5];
+    for (int i = 0; i < rank; ++i) {
+        d[i] = dims[i];
+        b[i] = box[i];
+        estr[i] = 1;
+        if (i) s[i - 1] = stride_bytes[i - 1];
+    }
+    CUresult r = fn(map, dtype == FM_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, rank,
+                    const_cast<void *>(base_ptr), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
-        set_error("cuTensorMapEncodeTiled failed with %d (rows %llu, d %llu, stride %llu)", (int)r, (unsigned long long)rows,
-                  (unsigned long long)d, (unsigned long long)row_stride_bytes);
+        set_error("cuTensorMapEncodeTiled failed with %d (rank %d, rows %llu, d %llu, stride %llu)", (int)r, rank, (unsigned long long)dims[1],
+                  (unsigned long long)dims[0], (unsigned long long)stride_bytes[0]);
         return FM_ERR_CUDA;
     }
     return FM_OK;
+}
+
+int make_tensor_map_2d(CUtensorMap *map, const void *base_ptr, int dtype, uint64_t rows, uint64_t d, uint64_t row_stride_bytes,
+                       uint32_t box_rows)
+{
+    const uint64_t dims[2] = {d, rows};
+    const uint32_t box[2] = {64, box_rows};
+    return make_tensor_map(map, base_ptr, dtype, 2, dims, &row_stride_bytes, box);
 }
 
 template <int D, bool DENSE>

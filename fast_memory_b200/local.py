@@ -35,7 +35,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     d = t.shape[2]
     ok = sd == 1 and (st * e) % 16 == 0 and (sh * e) % 16 == 0 and t.data_ptr() % 16 == 0 and \
         (t.shape[1] == 1 or st >= d) and (t.shape[0] == 1 or sh >= d)
-    return t if ok else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def _int32(values: Optional[Prefix], dev: torch.device, name: str, count: Optional[int] = None) -> Optional[torch.Tensor]:

@@ -48,6 +48,11 @@ def test_other_refusals():
     assert lib.fm_local_attn_fwd(ref(_attn(n_q_rows=0)), None, None, None, 0, None) == 0            # nothing to do
     assert lib.fm_local_attn_bwd(ref(_attn()), FAKE, FAKE, FAKE, 640, 64, None, FAKE, FAKE, FAKE, FAKE, 8, None) == WORKSPACE
     assert lib.fm_local_attn_bwd(ref(_attn()), FAKE, FAKE, FAKE, 640, 64, None, FAKE, None, FAKE, FAKE, 1 << 30, None) == BAD
+    for kw in (dict(n_q_rows=0), dict(n_k_rows=0), dict(n_q_heads=300), dict(n_q_rows=0, n_k_rows=0), dict(d=48), dict(n_kv_heads=0)):
+        lib.fm_local_attn_workspace_bytes(ref(_attn(**kw)))                                           # any numbers: a size, no crash
+        lib.fm_local_attn_bwd_workspace_bytes(ref(_attn(**kw)))
+    assert lib.fm_local_attn_fwd(ref(_attn(q=FAKE + 2)), FAKE, FAKE, FAKE, 1 << 30, None) == BAD
+    assert lib.fm_local_attn_fwd(ref(_attn(k_stride_row=60)), FAKE, FAKE, FAKE, 1 << 30, None) == BAD
     paged = _attn(page_table=FAKE, lengths=FAKE, n_seqs=1, n_pages=1, page_size=16, page_table_width=1, cu_q=FAKE)
     assert lib.fm_local_attn_bwd(ref(paged), FAKE, FAKE, FAKE, 640, 64, None, FAKE, FAKE, FAKE, FAKE, 1 << 30, None) == UNSUPPORTED
 
