@@ -203,6 +203,7 @@ int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *l
         set_error("fm_local_attn_bwd: workspace of %zu bytes, %zu are needed", workspace_bytes, fm_local_attn_bwd_workspace_bytes(a));
         return FM_ERR_WORKSPACE;
     }
+    FM_REQUIRE((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) % 16 == 0, "fm_local_attn_bwd: misaligned buffer");
     FM_REQUIRE((reinterpret_cast<uintptr_t>(d_o) | reinterpret_cast<uintptr_t>(o) | uintptr_t((do_stride_head | do_stride_row) * elem_bytes(a->dtype))) % 16 == 0,
                "fm_local_attn_bwd: rows must start on 16-byte boundaries");
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -217,6 +218,7 @@ int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *l
         });
         if (rc) return rc;
     }
+    if (p.S > 0 && local_tc_fits(p, a->dtype)) return local_tc_bwd(p, g, a->dtype, st);
     return local_rows_bwd(p, g, a->dtype, st);
 }
 

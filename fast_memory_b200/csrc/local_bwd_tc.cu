@@ -1,0 +1,736 @@
+// Gradients of local attention on the 5th-generation tensor cores, 16-bit types, head dim 64 or 128.
+//
+//   P = e^(b - lse),  dP = dO V^T,  dS = P (dP - delta) (1 - tanh^2),  dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K
+// Two kernels, seven products instead of the five that one kernel with global reductions of dQ would do: no atomics, the same
+// bits every time, and no fp32 copy of dQ (twice its size, written and read back).
+//
+// local_dkv_kernel: a CTA owns 128 keys of one KV head and walks the query tiles (128 rows = tokens x heads of the group, so
+// that the sum over the group is part of the contraction) that see them.  Everything is transposed - lane = key:
+//     S^T = K Q^T    dP^T = V dO^T    (SS)      P^T, dS^T go back to TMEM over S^T, dP^T as 16-bit A operands
+//     dV += P^T dO   dK += dS^T Q     (TS, B read MN-major from the very tiles that served K-major above)
+// S^T | dP^T | dV | dK fill the 512 columns.  The order S(j+1) behind dV(j) and dP(j+1) behind dK(j) lets the exponentials of one
+// tile run under the products of its neighbours although nothing is double-buffered in TMEM.  Two warpgroups share the 128
+// lanes, 64 columns (queries) each; lse and delta of a column come from shared memory as broadcasts.
+//
+// local_dq_kernel: a CTA owns one query tile and walks its key tiles; lane = query row.  S is double-buffered: S(j+2), dP(j+1)
+// and dQ(j) are under way while tile j+1 is worked on.  dS overwrites S.
+//
+// P and dS are rounded to the element type because the products take 16-bit operands; sums are fp32 (TMEM) and rounded once.
+// scale is applied to the sums.  Rows of a tile that are not the document's are zero where a contraction runs over them; a
+// hidden NaN inside the document shows as a result that is not finite, and such rows are computed again one pair at a time, as
+// are all rows of a CTA whose pipeline wait gave up.
+#include "local_tc.cuh"
+
+namespace fm {
+
+namespace {
+
+using namespace ltc;
+
+constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kStatWarp = 10;
+
+template <int D> struct Bytes {
+    static constexpr uint32_t kTileB = uint32_t(D / 64) * kBlock;
+};
+
+// ---- one pair's exponent ------------------------------------------------------------------------------------------------
+// From the product: x = score in log2 units, dcap = derivative of the cap.
+__device__ __forceinline__ float shape_one(const LocalParams &p, float qk, float k1, float c2, float &dcap)
+{
+    // cap: t = tanh(s / cap) = 1 - 2 / (1 + e^2x), k1 = 2 scale / cap log2 e, c2 = cap log2 e
+    const float e = fast_exp2(qk * k1);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    const float t = fmaf(-2.f, r, 1.f);
+    dcap = fmaf(-t, t, 1.f);
+    return t * c2;
+}
+
+// ======================================================= dK, dV ============================================================
+template <int D> struct DkvCfg {
+    static constexpr uint32_t kTileB = Bytes<D>::kTileB;
+    static constexpr int kStages = D == 128 ? 2 : 4;             // query tiles (Q and dO) in flight or in use
+    static constexpr uint32_t kSmem = (2 + 2 * kStages) * kTileB + 1024;
+};
+
+template <int DIM> struct DkvShared {
+    uint64_t kv_full, full[DkvCfg<DIM>::kStages], empty[DkvCfg<DIM>::kStages], tail;
+    uint64_t stat_full[2], stat_empty[2];
+    uint64_t s_full, p_full, dp_full, ds_full, drain;
+    uint32_t tmem_slot;
+    int abort;
+    int h, j0, q_lo, n_q;                                        // head, first key, first query tile, query tiles
+    Doc D;
+    alignas(16) float lse2[2][kTile], delta[2][kTile];
+    alignas(16) float slope2[kTile];
+    alignas(16) int token[kTile];                                // of a column, from the tile's first
+};
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kThreads, 1)
+local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ BwdParams g, const __grid_constant__ CUtensorMap tm_q,
+                 const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                 uint32_t idesc_s, uint32_t idesc_o)
+{
+    extern __shared__ unsigned char smem_dyn[];
+    __shared__ __align__(16) DkvShared<DIM> sh;
+    using C = DkvCfg<DIM>;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t base = (tc::smem_addr(smem_dyn) + 1023u) & ~1023u;
+    unsigned char *base_ptr = smem_dyn + (base - tc::smem_addr(smem_dyn));
+    const uint32_t s_k = base, s_v = base + C::kTileB, s_q0 = base + 2 * C::kTileB;      // stage i: Q, then dO
+    volatile int *abort_flag = &sh.abort;
+    const int tokens = kTile / p.G, rows = tokens * p.G;
+
+    if (warp == 0) {
+        const int nb = gridDim.x / p.H, h = blockIdx.x / nb;
+        const int2 at = find_block<true>(p, kTile, blockIdx.x % nb);
+        if (lane == 0) {
+            sh.h = h;
+            sh.n_q = 0;
+            sh.j0 = -1;
+            if (at.x >= 0) {
+                sh.D = local_doc<true>(p, at.x);
+                sh.j0 = at.y * kTile;
+                const int last = min(sh.j0 + kTile, sh.D.nk) - 1;
+                int2 run = make_int2(local_query_run(p, sh.D, sh.j0).x, local_query_run(p, sh.D, last).y);
+                if (sh.j0 < sh.D.prefix) run = make_int2(0, sh.D.nq);
+                sh.q_lo = run.x / tokens;
+                sh.n_q = run.y > run.x ? (run.y + tokens - 1) / tokens - sh.q_lo : 0;
+            }
+        }
+    }
+    if (warp == kMmaWarp) tc::tmem_alloc(tc::smem_addr(&sh.tmem_slot), 512);
+    if (warp == kLoadWarp && lane == 0) {
+        tc::mbar_init(bar_addr(&sh.kv_full), 1);
+        for (int i = 0; i < C::kStages; ++i) {
+            tc::mbar_init(bar_addr(&sh.full[i]), 1);
+            tc::mbar_init(bar_addr(&sh.empty[i]), 1);
+        }
+        tc::mbar_init(bar_addr(&sh.tail), 1);
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(bar_addr(&sh.stat_full[i]), 1);
+            tc::mbar_init(bar_addr(&sh.stat_empty[i]), 8);
+        }
+        tc::mbar_init(bar_addr(&sh.s_full), 1);
+        tc::mbar_init(bar_addr(&sh.p_full), 8);
+        tc::mbar_init(bar_addr(&sh.dp_full), 1);
+        tc::mbar_init(bar_addr(&sh.ds_full), 8);
+        tc::mbar_init(bar_addr(&sh.drain), 1);
+        tc::mbar_fence_init();
+        sh.abort = 0;
+        tc::prefetch_tensormap(&tm_q);
+        tc::prefetch_tensormap(&tm_do);
+        tc::prefetch_tensormap(&tm_k);
+        tc::prefetch_tensormap(&tm_v);
+    }
+    if (tid < kTile) {
+        sh.token[tid] = tid / p.G;
+        sh.slope2[tid] = 0.f;
+    }
+    // rows that no load writes: a group that does not divide the tile
+    for (int i = rows * 8 + tid; i < kTile * 8; i += kThreads)
+        for (int c = 0; c < 2 * C::kStages * (DIM / 64); ++c)
+            *reinterpret_cast<uint4 *>(base_ptr + 2 * C::kTileB + c * kBlock + i * 16) = make_uint4(0, 0, 0, 0);
+    tc::fence_proxy_async_smem();
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = sh.tmem_slot;
+    const int n_q = sh.n_q, q_lo = sh.q_lo, h = sh.h, j0 = sh.j0;
+    const Doc &D = sh.D;
+
+    if (warp >= 8) {
+        tc::set_registers_down<72>();
+        if (warp == kLoadWarp) {
+            if (n_q > 0) {
+                if (lane == 0) {
+                    tc::mbar_arrive_expect_tx(bar_addr(&sh.kv_full), 2 * C::kTileB);
+                    for (int c = 0; c < DIM / 64; ++c) {
+                        tc::tma_load_3d(s_k + c * kBlock, &tm_k, c * 64, D.k0 + j0, h, bar_addr(&sh.kv_full));
+                        tc::tma_load_3d(s_v + c * kBlock, &tm_v, c * 64, D.k0 + j0, h, bar_addr(&sh.kv_full));
+                    }
+                }
+                bool ok = true;
+                int i = 0;
+                for (; i < n_q; ++i) {
+                    const int slot = i % C::kStages, t0 = (q_lo + i) * tokens;
+                    if (i >= C::kStages) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((i / C::kStages) & 1) ^ 1, abort_flag);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    const bool cut = t0 + tokens > D.nq;                       // the document's last queries
+                    const uint32_t bar = bar_addr(cut ? &sh.tail : &sh.full[slot]);
+                    const uint32_t dst = s_q0 + slot * 2 * C::kTileB;
+                    if (lane == 0) {
+                        tc::mbar_arrive_expect_tx(bar, 2u * (DIM / 64) * 128u * rows);
+                        for (int c = 0; c < DIM / 64; ++c) {
+                            tc::tma_load_4d(dst + c * kBlock, &tm_q, c * 64, 0, D.q0 + t0, h, bar);
+                            tc::tma_load_4d(dst + C::kTileB + c * kBlock, &tm_do, c * 64, 0, D.q0 + t0, h, bar);
+                        }
+                    }
+                    if (cut) {
+                        ok = tc::mbar_wait_or_abort(bar, 0, abort_flag);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        for (int x = (D.nq - t0) * p.G * 8 + lane; x < rows * 8; x += 32)
+                            for (int c = 0; c < 2 * (DIM / 64); ++c)
+                                *reinterpret_cast<uint4 *>(base_ptr + (dst - base) + c * kBlock + x * 16) = make_uint4(0, 0, 0, 0);
+                        tc::fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(bar_addr(&sh.full[slot]));
+                    }
+                }
+                if (!ok) {
+                    if (lane == 0) *abort_flag = 1;
+                    tc::mbar_wait(bar_addr(&sh.kv_full), 0);
+                    for (int x = max(i - C::kStages, 0); x < i; ++x) tc::mbar_wait(bar_addr(&sh.full[x % C::kStages]), (x / C::kStages) & 1);
+                }
+            }
+        } else if (warp == kStatWarp) {
+            bool ok = true;
+            for (int i = 0; i < n_q; ++i) {
+                const int buf = i & 1, t0 = (q_lo + i) * tokens;
+                if (i >= 2) ok = tc::mbar_wait_or_abort(bar_addr(&sh.stat_empty[buf]), ((i >> 1) & 1) ^ 1, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int r = lane + 32 * x, token = t0 + r / p.G, head = h * p.G + r % p.G;
+                    const bool valid = r < rows && token < D.nq;
+                    float lse = -INFINITY, delta = 0.f;
+                    if (valid) {
+                        lse = g.lse[int64_t(head) * p.S + D.q0 + token];
+                        delta = g.delta[int64_t(head) * p.S + D.q0 + token];
+                    }
+                    sh.lse2[buf][r] = lse == -INFINITY ? INFINITY : lse * kLog2e;          // no such row, or one that sees nothing: P = 0
+                    sh.delta[buf][r] = delta;
+                    if (i == 0 && p.slopes && r < rows) sh.slope2[r] = p.slopes[head] * kLog2e;
+                }
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(bar_addr(&sh.stat_full[buf]));
+            }
+            if (!ok && lane == 0) *abort_flag = 1;
+        } else if (warp == kMmaWarp && lane == 0 && n_q > 0) {
+            bool ok = tc::mbar_wait_or_abort(bar_addr(&sh.kv_full), 0, abort_flag);
+            auto q_tile = [&](int i) { return s_q0 + (i % C::kStages) * 2 * C::kTileB; };
+            auto wait_q = [&](int i) { ok = ok && tc::mbar_wait_or_abort(bar_addr(&sh.full[i % C::kStages]), (i / C::kStages) & 1, abort_flag); };
+            auto scores = [&](int i) {
+#pragma unroll
+                for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16(tmem, desc_k(s_k, ks), desc_k(q_tile(i), ks), idesc_s, ks > 0);
+                tc::umma_commit(bar_addr(&sh.s_full));
+            };
+            auto dprob = [&](int i) {
+#pragma unroll
+                for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16(tmem + 128, desc_k(s_v, ks), desc_k(q_tile(i) + C::kTileB, ks), idesc_s, ks > 0);
+                tc::umma_commit(bar_addr(&sh.dp_full));
+            };
+            wait_q(0);
+            if (ok) {
+                scores(0);
+                dprob(0);
+            }
+            for (int i = 0; i < n_q && ok; ++i) {
+                ok = tc::mbar_wait_or_abort(bar_addr(&sh.p_full), i & 1, abort_flag);
+                if (!ok) break;
+                tc::fence_after_sync();
+#pragma unroll
+                for (int ks = 0; ks < kTile / 16; ++ks)
+                    tc::umma_f16_ts(tmem + 256, tmem + (ks >> 2) * 64 + (ks & 3) * 8, desc_mn(q_tile(i) + C::kTileB, ks), idesc_o, i > 0 || ks > 0);
+                if (i + 1 < n_q) {
+                    wait_q(i + 1);
+                    if (!ok) break;
+                    scores(i + 1);
+                }
+                ok = tc::mbar_wait_or_abort(bar_addr(&sh.ds_full), i & 1, abort_flag);
+                if (!ok) break;
+                tc::fence_after_sync();
+#pragma unroll
+                for (int ks = 0; ks < kTile / 16; ++ks)
+                    tc::umma_f16_ts(tmem + 384, tmem + 128 + (ks >> 2) * 64 + (ks & 3) * 8, desc_mn(q_tile(i), ks), idesc_o, i > 0 || ks > 0);
+                tc::umma_commit(bar_addr(&sh.empty[i % C::kStages]));
+                if (i + 1 < n_q) dprob(i + 1);
+            }
+            if (!ok) *abort_flag = 1;
+            tc::umma_commit(bar_addr(&sh.drain));
+            tc::mbar_wait(bar_addr(&sh.drain), 0);
+        }
+    } else {
+        tc::set_registers_up<216>();
+        const int half = warp >> 2, row = tid & 127, j = j0 + row;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem + half * 64 + lanes, t_dp = tmem + 128 + half * 64 + lanes;
+        const bool valid = j0 >= 0 && j < D.nk;
+        int2 run = make_int2(0, 0), all = make_int2(0, 0);       // queries that see this key; that see every key of the tile
+        if (n_q > 0) {
+            const int last = min(j0 + kTile, D.nk) - 1;
+            if (valid) run = local_query_run(p, D, j);
+            all = make_int2(local_query_run(p, D, last).x, local_query_run(p, D, max(j0, min(D.prefix, last))).y);
+        }
+        const float scale2 = p.scale * kLog2e, k1 = p.cap > 0.f ? 2.f * kLog2e * p.scale / p.cap : 0.f, c2 = p.cap * kLog2e;
+        bool ok = true;
+        for (int i = 0; i < n_q; ++i) {
+            const int buf = i & 1, t0 = (q_lo + i) * tokens;
+            const bool masked = !(all.x <= t0 && min(t0 + tokens, D.nq) <= all.y);
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.stat_full[buf]), (i >> 1) & 1, abort_flag) &&
+                 tc::mbar_wait_or_abort(bar_addr(&sh.s_full), i & 1, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc::fence_after_sync();
+            float pr[64];
+            unsigned seen[2] = {0xffffffffu, 0xffffffffu};
+            if (masked) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    unsigned m = 0;
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        const int token = t0 + sh.token[half * 64 + x * 32 + c];
+                        m |= (token >= run.x && token < run.y) ? 1u << c : 0u;
+                    }
+                    seen[x] = m;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                uint32_t s[32];
+                tc::tmem_ld_x32(t_s + x * 32, s);
+                tc::tmem_ld_wait(s);
+                const float *lse2 = &sh.lse2[buf][half * 64 + x * 32];
+                if (p.cap > 0.f || p.slopes) {
+                    const float dist0 = float(D.nk - D.nq + t0 - j);
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        float w[2], dcap[2] = {1.f, 1.f};
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {
+                            const int col = half * 64 + x * 32 + c + y;
+                            float b = __uint_as_float(s[c + y]);
+                            b = p.cap > 0.f ? shape_one(p, b, k1, c2, dcap[y]) : b * scale2;
+                            b = fmaf(-sh.slope2[col], fabsf(dist0 + float(sh.token[col])), b);
+                            w[y] = (seen[x] >> (c + y) & 1u) ? fast_exp2(b - lse2[c + y]) : 0.f;
+                            pr[x * 32 + c + y] = w[y] * dcap[y];
+                        }
+                        pk[c >> 1] = pack2<T>(w[0], w[1]);
+                    }
+                    tc::tmem_st_x16(t_s + x * 16, pk);
+                } else {
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4) {
+                        const float4 L = *reinterpret_cast<const float4 *>(lse2 + c);
+                        pr[x * 32 + c] = fast_exp2(fmaf(__uint_as_float(s[c]), scale2, -L.x));
+                        pr[x * 32 + c + 1] = fast_exp2(fmaf(__uint_as_float(s[c + 1]), scale2, -L.y));
+                        pr[x * 32 + c + 2] = fast_exp2(fmaf(__uint_as_float(s[c + 2]), scale2, -L.z));
+                        pr[x * 32 + c + 3] = fast_exp2(fmaf(__uint_as_float(s[c + 3]), scale2, -L.w));
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) pr[x * 32 + c] = (seen[x] >> c & 1u) ? pr[x * 32 + c] : 0.f;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) pk[c] = pack2<T>(pr[x * 32 + 2 * c], pr[x * 32 + 2 * c + 1]);
+                    tc::tmem_st_x16(t_s + x * 16, pk);
+                }
+            }
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(bar_addr(&sh.p_full));
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.dp_full), i & 1, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc::fence_after_sync();
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                uint32_t s[32], pk[16];
+                tc::tmem_ld_x32(t_dp + x * 32, s);
+                tc::tmem_ld_wait(s);
+                const float *delta = &sh.delta[buf][half * 64 + x * 32];
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                    const float4 dl = *reinterpret_cast<const float4 *>(delta + c);
+                    s[c] = __float_as_uint(pr[x * 32 + c] * (__uint_as_float(s[c]) - dl.x));
+                    s[c + 1] = __float_as_uint(pr[x * 32 + c + 1] * (__uint_as_float(s[c + 1]) - dl.y));
+                    s[c + 2] = __float_as_uint(pr[x * 32 + c + 2] * (__uint_as_float(s[c + 2]) - dl.z));
+                    s[c + 3] = __float_as_uint(pr[x * 32 + c + 3] * (__uint_as_float(s[c + 3]) - dl.w));
+                }
+                if (masked) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) s[c] = (seen[x] >> c & 1u) ? s[c] : 0u;
+                }
+#pragma unroll
+                for (int c = 0; c < 16; ++c) pk[c] = pack2<T>(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
+                tc::tmem_st_x16(t_dp + x * 16, pk);
+            }
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                tc::mbar_arrive(bar_addr(&sh.ds_full));
+                tc::mbar_arrive(bar_addr(&sh.stat_empty[buf]));
+            }
+        }
+        if (ok && n_q > 0) {
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.drain), 0, abort_flag);
+            ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) *abort_flag = 1;
+        tc::fence_after_sync();
+        // first warpgroup: dV, second: dK
+        bool fine = ok;
+        const float f = half ? p.scale : 1.f;
+        T *out = static_cast<T *>(half ? g.dk : g.dv) + (int64_t(h) * p.N + D.k0 + j) * DIM;
+        if (ok && j0 >= 0) {
+#pragma unroll
+            for (int c = 0; c < DIM / 32; ++c) {
+                uint32_t o[32];
+                if (n_q > 0) {
+                    tc::tmem_ld_x32(tmem + 256 + half * 128 + lanes + c * 32, o);
+                    tc::tmem_ld_wait(o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0;
+                }
+                float worst = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float x = __uint_as_float(o[i]) * f;
+                    o[i] = __float_as_uint(x);
+                    worst = fmaf(x, 0.f, worst);
+                }
+                fine = fine && worst == 0.f;
+                if (valid) {
+                    uint4 *dst = reinterpret_cast<uint4 *>(out + c * 32);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        dst[i] = make_uint4(pack2<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1])),
+                                            pack2<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3])),
+                                            pack2<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5])),
+                                            pack2<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7])));
+                }
+            }
+        }
+        unsigned again = __ballot_sync(0xffffffffu, valid && !fine);
+        tc::named_barrier(1, 256);                                             // a row's dV and dK have been written before either is redone
+        while (again) {
+            const int r = (row & ~31) + __ffs(again) - 1;
+            again &= again - 1;
+            local_row_dkv<T, DIM>(p, g, D, h, j0 + r);
+        }
+        tc::fence_before_sync();
+    }
+    __syncthreads();
+    if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
+}
+
+// ========================================================= dQ ==============================================================
+template <int D> struct DqCfg {
+    static constexpr uint32_t kTileB = Bytes<D>::kTileB;
+    static constexpr int kRing = D == 128 ? 5 : 8;               // K and V tiles in flight or in use
+    static constexpr uint32_t kSmem = (2 + kRing) * kTileB + 1024;
+};
+
+template <int DIM> struct DqShared {
+    uint64_t q_full, full[DqCfg<DIM>::kRing], empty[DqCfg<DIM>::kRing], tail;
+    uint64_t s_full[2], dp_full, ds_full, drain;
+    uint32_t tmem_slot;
+    int abort;
+    int h, t0, t1, n_pre, lo, n_k;                               // query tokens [t0, t1); key tiles: prefix, then lo ..; n_k in all
+    Doc D;
+};
+
+template <typename T, int DIM>
+__global__ void __launch_bounds__(kThreads, 1)
+local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ BwdParams g, const __grid_constant__ CUtensorMap tm_q,
+                const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                uint32_t idesc_s, uint32_t idesc_o)
+{
+    extern __shared__ unsigned char smem_dyn[];
+    __shared__ __align__(16) DqShared<DIM> sh;
+    using C = DqCfg<DIM>;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t base = (tc::smem_addr(smem_dyn) + 1023u) & ~1023u;
+    unsigned char *base_ptr = smem_dyn + (base - tc::smem_addr(smem_dyn));
+    const uint32_t s_q = base, s_do = base + C::kTileB, ring0 = base + 2 * C::kTileB;
+    volatile int *abort_flag = &sh.abort;
+    const int tokens = kTile / p.G, rows = tokens * p.G;
+
+    if (warp == 0) {
+        const int nb = gridDim.x / p.H, h = blockIdx.x / nb;
+        const int2 at = find_block<false>(p, tokens, nb - 1 - int(blockIdx.x % nb));       // (the most keys first)
+        if (lane == 0) {
+            sh.h = h;
+            sh.t0 = sh.t1 = sh.n_pre = sh.lo = sh.n_k = 0;
+            if (at.x >= 0) {
+                sh.D = local_doc(p, at.x);
+                const Doc &D = sh.D;
+                sh.t0 = at.y * tokens;
+                sh.t1 = min(sh.t0 + tokens, D.nq);
+                const int lo = local_run(p, D.nk - D.nq + sh.t0, D.nk).x, hi = local_run(p, D.nk - D.nq + sh.t1 - 1, D.nk).y;
+                sh.n_pre = (D.prefix + kTile - 1) / kTile;
+                sh.lo = max(lo / kTile, sh.n_pre);
+                sh.n_k = sh.n_pre + (hi > lo ? max((hi + kTile - 1) / kTile - sh.lo, 0) : 0);
+            }
+        }
+    }
+    if (warp == kMmaWarp) tc::tmem_alloc(tc::smem_addr(&sh.tmem_slot), 512);
+    if (warp == kLoadWarp && lane == 0) {
+        tc::mbar_init(bar_addr(&sh.q_full), 1);
+        for (int i = 0; i < C::kRing; ++i) {
+            tc::mbar_init(bar_addr(&sh.full[i]), 1);
+            tc::mbar_init(bar_addr(&sh.empty[i]), 1);
+        }
+        tc::mbar_init(bar_addr(&sh.tail), 1);
+        tc::mbar_init(bar_addr(&sh.s_full[0]), 1);
+        tc::mbar_init(bar_addr(&sh.s_full[1]), 1);
+        tc::mbar_init(bar_addr(&sh.dp_full), 1);
+        tc::mbar_init(bar_addr(&sh.ds_full), 8);
+        tc::mbar_init(bar_addr(&sh.drain), 1);
+        tc::mbar_fence_init();
+        sh.abort = 0;
+        tc::prefetch_tensormap(&tm_q);
+        tc::prefetch_tensormap(&tm_do);
+        tc::prefetch_tensormap(&tm_k);
+        tc::prefetch_tensormap(&tm_v);
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = sh.tmem_slot;                          // S0, S1, dP, dQ
+    const int n_k = sh.n_k, n_pre = sh.n_pre, lo = sh.lo, h = sh.h, t0 = sh.t0, t1 = sh.t1;
+    const Doc &D = sh.D;
+    auto key_tile = [&](int n) { return n < n_pre ? n : lo + n - n_pre; };
+
+    if (warp >= 8) {
+        tc::set_registers_down<72>();
+        if (warp == kLoadWarp) {
+            if (lane == 0 && n_k > 0) {
+                tc::mbar_arrive_expect_tx(bar_addr(&sh.q_full), 2u * (DIM / 64) * 128u * rows);
+                for (int c = 0; c < DIM / 64; ++c) {
+                    tc::tma_load_4d(s_q + c * kBlock, &tm_q, c * 64, 0, D.q0 + t0, h, bar_addr(&sh.q_full));
+                    tc::tma_load_4d(s_do + c * kBlock, &tm_do, c * 64, 0, D.q0 + t0, h, bar_addr(&sh.q_full));
+                }
+            }
+            bool ok = true;
+            int i = 0;
+            for (; i < 2 * n_k; ++i) {
+                const int slot = i % C::kRing, kt = key_tile(i >> 1), live = D.nk - kt * kTile;
+                if (i >= C::kRing) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((i / C::kRing) & 1) ^ 1, abort_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const bool cut = !(i & 1) && live < kTile;                     // the K tile's rows behind the last key meet dS = 0
+                const uint32_t bar = bar_addr(cut ? &sh.tail : &sh.full[slot]), dst = ring0 + slot * C::kTileB;
+                if (lane == 0) {
+                    tc::mbar_arrive_expect_tx(bar, C::kTileB);
+                    for (int c = 0; c < DIM / 64; ++c) tc::tma_load_3d(dst + c * kBlock, (i & 1) ? &tm_v : &tm_k, c * 64, D.k0 + kt * kTile, h, bar);
+                }
+                if (cut) {
+                    ok = tc::mbar_wait_or_abort(bar, 0, abort_flag);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    for (int x = live * 8 + lane; x < kTile * 8; x += 32)
+                        for (int c = 0; c < DIM / 64; ++c)
+                            *reinterpret_cast<uint4 *>(base_ptr + (dst - base) + c * kBlock + x * 16) = make_uint4(0, 0, 0, 0);
+                    tc::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(bar_addr(&sh.full[slot]));
+                }
+            }
+            if (!ok) {
+                if (lane == 0) *abort_flag = 1;
+                tc::mbar_wait(bar_addr(&sh.q_full), 0);
+                for (int x = max(i - C::kRing, 0); x < i; ++x) tc::mbar_wait(bar_addr(&sh.full[x % C::kRing]), (x / C::kRing) & 1);
+            }
+        } else if (warp == kMmaWarp && lane == 0 && n_k > 0) {
+            bool ok = tc::mbar_wait_or_abort(bar_addr(&sh.q_full), 0, abort_flag);
+            auto tile = [&](int i) { return ring0 + (i % C::kRing) * C::kTileB; };          // i = 2 n: K, 2 n + 1: V
+            auto wait_tile = [&](int i) { ok = ok && tc::mbar_wait_or_abort(bar_addr(&sh.full[i % C::kRing]), (i / C::kRing) & 1, abort_flag); };
+            auto scores = [&](int n) {
+                wait_tile(2 * n);
+                if (!ok) return;
+#pragma unroll
+                for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16(tmem + (n & 1) * 128, desc_k(s_q, ks), desc_k(tile(2 * n), ks), idesc_s, ks > 0);
+                tc::umma_commit(bar_addr(&sh.s_full[n & 1]));
+            };
+            auto dprob = [&](int n) {
+                wait_tile(2 * n + 1);
+                if (!ok) return;
+#pragma unroll
+                for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16(tmem + 256, desc_k(s_do, ks), desc_k(tile(2 * n + 1), ks), idesc_s, ks > 0);
+                tc::umma_commit(bar_addr(&sh.dp_full));
+                tc::umma_commit(bar_addr(&sh.empty[(2 * n + 1) % C::kRing]));
+            };
+            scores(0);
+            dprob(0);
+            if (n_k > 1) scores(1);
+            for (int n = 0; n < n_k && ok; ++n) {
+                ok = tc::mbar_wait_or_abort(bar_addr(&sh.ds_full), n & 1, abort_flag);
+                if (!ok) break;
+                tc::fence_after_sync();
+                if (n + 1 < n_k) dprob(n + 1);
+                if (!ok) break;
+#pragma unroll
+                for (int ks = 0; ks < kTile / 16; ++ks)
+                    tc::umma_f16_ts(tmem + 384, tmem + (n & 1) * 128 + (ks >> 2) * 64 + (ks & 3) * 8, desc_mn(tile(2 * n), ks), idesc_o, n > 0 || ks > 0);
+                tc::umma_commit(bar_addr(&sh.empty[(2 * n) % C::kRing]));
+                if (n + 2 < n_k) scores(n + 2);
+            }
+            if (!ok) *abort_flag = 1;
+            tc::umma_commit(bar_addr(&sh.drain));
+            tc::mbar_wait(bar_addr(&sh.drain), 0);
+        }
+    } else {
+        tc::set_registers_up<216>();
+        const int half = warp >> 2, row = tid & 127, token = t0 + row / p.G, head = h * p.G + row % p.G;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const uint32_t t_dp = tmem + 256 + half * 64 + lanes;
+        const bool valid = row < rows && token < t1;
+        const int64_t out_row = int64_t(head) * p.S + D.q0 + token;
+        const int shift = D.nk - D.nq, pos = shift + token;
+        float lse2 = INFINITY, delta = 0.f, slope2 = 0.f;
+        if (valid) {
+            const float x = g.lse[out_row];
+            lse2 = x == -INFINITY ? INFINITY : x * kLog2e;
+            delta = g.delta[out_row];
+            slope2 = p.slopes ? p.slopes[head] * kLog2e : 0.f;
+        }
+        const int2 run = valid ? local_run(p, pos, D.nk) : make_int2(0, 0);
+        const int pre = valid ? D.prefix : 0;
+        const int safe_lo = p.window ? shift + t1 - p.window : 0, safe_hi = n_k > 0 ? local_run(p, shift + t0, D.nk).y : 0;
+        const float scale2 = p.scale * kLog2e, k1 = p.cap > 0.f ? 2.f * kLog2e * p.scale / p.cap : 0.f, c2 = p.cap * kLog2e;
+        bool ok = true;
+        for (int n = 0; n < n_k; ++n) {
+            const int j0 = key_tile(n) * kTile, b = n & 1, col0 = j0 + half * 64;
+            const bool masked = !(j0 + kTile <= D.prefix || (j0 >= safe_lo && j0 + kTile <= safe_hi));
+            const uint32_t t_s = tmem + b * 128 + half * 64 + lanes;
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.s_full[b]), (n >> 1) & 1, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc::fence_after_sync();
+            float pr[64];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                uint32_t s[32];
+                tc::tmem_ld_x32(t_s + x * 32, s);
+                tc::tmem_ld_wait(s);
+                if (p.cap > 0.f || p.slopes) {
+                    const float dist0 = float(pos - col0);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) {
+                        float dcap = 1.f, y = __uint_as_float(s[c]);
+                        y = p.cap > 0.f ? shape_one(p, y, k1, c2, dcap) : y * scale2;
+                        y = fmaf(-slope2, fabsf(dist0 - float(x * 32 + c)), y);
+                        pr[x * 32 + c] = fast_exp2(y - lse2) * dcap;
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) pr[x * 32 + c] = fast_exp2(fmaf(__uint_as_float(s[c]), scale2, -lse2));
+                }
+            }
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.dp_full), n & 1, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc::fence_after_sync();
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                uint32_t s[32], pk[16];
+                tc::tmem_ld_x32(t_dp + x * 32, s);
+                tc::tmem_ld_wait(s);
+#pragma unroll
+                for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(pr[x * 32 + c] * (__uint_as_float(s[c]) - delta));
+                if (masked) {
+                    const int a = run.x - col0 - x * 32, e = run.y - col0 - x * 32, q = pre - col0 - x * 32;
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (!((c >= a && c < e) || c < q)) s[c] = 0u;
+                }
+#pragma unroll
+                for (int c = 0; c < 16; ++c) pk[c] = pack2<T>(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
+                tc::tmem_st_x16(t_s + x * 16, pk);
+            }
+            tc::tmem_st_wait();
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(bar_addr(&sh.ds_full));
+        }
+        if (ok && n_k > 0) {
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.drain), 0, abort_flag);
+            ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) *abort_flag = 1;
+        tc::fence_after_sync();
+        bool fine = ok;
+        // each warpgroup writes its half of the columns
+        if (ok && t0 < t1) {
+#pragma unroll
+            for (int c = 0; c < DIM / 64; ++c) {
+                const int col = half * (DIM / 2) + c * 32;
+                uint32_t o[32];
+                if (n_k > 0) {
+                    tc::tmem_ld_x32(tmem + 384 + lanes + col, o);
+                    tc::tmem_ld_wait(o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0;
+                }
+                float worst = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const float x = __uint_as_float(o[i]) * p.scale;
+                    o[i] = __float_as_uint(x);
+                    worst = fmaf(x, 0.f, worst);
+                }
+                fine = fine && worst == 0.f;
+                if (valid) {
+                    uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(g.dq) + out_row * DIM + col);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        dst[i] = make_uint4(pack2<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1])),
+                                            pack2<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3])),
+                                            pack2<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5])),
+                                            pack2<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7])));
+                }
+            }
+        }
+        unsigned again = __ballot_sync(0xffffffffu, valid && !fine);
+        tc::named_barrier(1, 256);
+        while (again) {
+            const int r = (row & ~31) + __ffs(again) - 1;
+            again &= again - 1;
+            local_row_dq<T, DIM>(p, g, D, h * p.G + r % p.G, t0 + r / p.G);
+        }
+        tc::fence_before_sync();
+    }
+    __syncthreads();
+    if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int DIM> int launch(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st)
+{
+    const int tokens = kTile / p.G, docs = p.n_docs + (p.cu_q ? 1 : 0);
+    CUtensorMap tm_q, tm_do, tm_k, tm_v;
+    if (int rc = local_query_map(&tm_q, p, p.q, p.q_sh, p.q_st, dtype)) return rc;
+    if (int rc = local_query_map(&tm_do, p, g.dout, g.do_sh, g.do_st, dtype)) return rc;
+    if (int rc = local_key_map(&tm_k, p, p.k, p.k_sh, p.k_st, dtype)) return rc;
+    if (int rc = local_key_map(&tm_v, p, p.v, p.v_sh, p.v_st, dtype)) return rc;
+    const bool bf16 = dtype == FM_BF16;
+    const uint32_t idesc_s = tc::instr_desc_f16(bf16, kTile, kTile), idesc_o = tc::instr_desc_f16(bf16, kTile, DIM, false, true);
+    const int64_t q_blocks = std::min<int64_t>(p.S, (int64_t(p.S) + int64_t(docs) * (tokens - 1)) / tokens) * p.H;
+    const int64_t k_blocks = std::min<int64_t>(p.N, (int64_t(p.N) + int64_t(docs) * (kTile - 1)) / kTile) * p.H;
+    FM_CUDA_OK(func_attr_cached((const void *)local_dq_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DqCfg<DIM>::kSmem));
+    FM_CUDA_OK(func_attr_cached((const void *)local_dkv_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DkvCfg<DIM>::kSmem));
+    local_dkv_kernel<T, DIM><<<unsigned(k_blocks), kThreads, DkvCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, idesc_s, idesc_o);
+    FM_LAUNCHED("local_dkv_kernel");
+    local_dq_kernel<T, DIM><<<unsigned(q_blocks), kThreads, DqCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, idesc_s, idesc_o);
+    FM_LAUNCHED("local_dq_kernel");
+    return FM_OK;
+}
+
+}  // namespace
+
+int local_tc_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st)
+{
+    if (dtype == FM_BF16) return p.d == 128 ? launch<__nv_bfloat16, 128>(p, g, dtype, st) : launch<__nv_bfloat16, 64>(p, g, dtype, st);
+    return p.d == 128 ? launch<__half, 128>(p, g, dtype, st) : launch<__half, 64>(p, g, dtype, st);
+}
+
+}  // namespace fm

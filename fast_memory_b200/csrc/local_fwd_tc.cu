@@ -508,22 +508,10 @@ template <typename T, int D> int launch(const LocalParams &p, int dtype, void *w
 {
     using C = Cfg<D>;
     const Shape sh = shape_of(p);
-    const int tokens = ltc::kTile / p.G;
     CUtensorMap tm_q, tm_k, tm_v;
-    auto pos = [](int64_t stride) { return uint64_t(stride > 0 ? stride * 2 : 16); };   // a dim of size one may have any stride
-    {
-        const uint64_t dims[4] = {uint64_t(D), uint64_t(p.G), uint64_t(p.S), uint64_t(p.H)};
-        const uint64_t strides[3] = {pos(p.q_sh), pos(p.q_st), pos(p.q_sh * p.G)};
-        const uint32_t box[4] = {64, uint32_t(p.G), uint32_t(tokens), 1};
-        if (int rc = make_tensor_map(&tm_q, p.q, dtype, 4, dims, strides, box)) return rc;
-    }
-    for (int i = 0; i < 2; ++i) {
-        const int64_t page = int64_t(1) << p.page_shift;
-        const uint64_t dims[3] = {uint64_t(D), uint64_t(p.table ? page : p.N), uint64_t(p.table ? int64_t(p.n_pages) * p.H : p.H)};
-        const uint64_t strides[2] = {p.table ? uint64_t(D * 2) : pos(i ? p.v_st : p.k_st), p.table ? uint64_t(page * D * 2) : pos(i ? p.v_sh : p.k_sh)};
-        const uint32_t box[3] = {64, uint32_t(p.table ? std::min<int64_t>(page, ltc::kTile) : ltc::kTile), 1};
-        if (int rc = make_tensor_map(i ? &tm_v : &tm_k, i ? p.v : p.k, dtype, 3, dims, strides, box)) return rc;
-    }
+    if (int rc = local_query_map(&tm_q, p, p.q, p.q_sh, p.q_st, dtype)) return rc;
+    if (int rc = local_key_map(&tm_k, p, p.k, p.k_sh, p.k_st, dtype)) return rc;
+    if (int rc = local_key_map(&tm_v, p, p.v, p.v_sh, p.v_st, dtype)) return rc;
     float *part_lse = static_cast<float *>(ws), *part_o = part_lse + (size_t(sh.parts) * p.Hq * p.S + 31) / 32 * 32;
     const bool bf16 = dtype == FM_BF16;
     FM_CUDA_OK(func_attr_cached((const void *)local_fwd_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem));
@@ -538,6 +526,28 @@ template <typename T, int D> int launch(const LocalParams &p, int dtype, void *w
 }
 
 }  // namespace
+
+// Queries as (d, head of the group, token, KV head): a box is one tile of rows (token, head).  A dim of size one may have any
+// stride, so that 0 becomes something a tensor map takes.
+int local_query_map(CUtensorMap *map, const LocalParams &p, const void *q, int64_t sh, int64_t st, int dtype)
+{
+    auto bytes = [](int64_t stride) { return uint64_t(stride > 0 ? stride * 2 : 16); };
+    const uint64_t dims[4] = {uint64_t(p.d), uint64_t(p.G), uint64_t(p.S), uint64_t(p.H)};
+    const uint64_t strides[3] = {bytes(sh), bytes(st), bytes(sh * p.G)};
+    const uint32_t box[4] = {64, uint32_t(p.G), uint32_t(ltc::kTile / p.G), 1};
+    return make_tensor_map(map, q, dtype, 4, dims, strides, box);
+}
+
+// Keys as (d, row, KV head), or pages as (d, row of the page, page x head): a box is one tile, or the part of it in one page.
+int local_key_map(CUtensorMap *map, const LocalParams &p, const void *k, int64_t sh, int64_t st, int dtype)
+{
+    auto bytes = [](int64_t stride) { return uint64_t(stride > 0 ? stride * 2 : 16); };
+    const int64_t page = int64_t(1) << p.page_shift;
+    const uint64_t dims[3] = {uint64_t(p.d), uint64_t(p.table ? page : p.N), uint64_t(p.table ? int64_t(p.n_pages) * p.H : p.H)};
+    const uint64_t strides[2] = {p.table ? uint64_t(p.d) * 2 : bytes(st), p.table ? uint64_t(page) * p.d * 2 : bytes(sh)};
+    const uint32_t box[3] = {64, uint32_t(p.table ? std::min<int64_t>(page, ltc::kTile) : ltc::kTile), 1};
+    return make_tensor_map(map, k, dtype, 3, dims, strides, box);
+}
 
 // 16-bit types, head dim 64 or 128, a group that fits a tile, and at least one key (a tensor map has no empty dims).
 bool local_tc_fits(const LocalParams &p, int dtype)

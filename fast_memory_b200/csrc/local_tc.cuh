@@ -54,7 +54,10 @@ template <bool KEYS> __device__ __forceinline__ int2 find_block(const LocalParam
 
 }  // namespace ltc
 
-// Launch paths; FM_ERR_UNSUPPORTED (without a message) where the shape is not theirs.
+// Whether a call goes to the tcgen05 kernels, their launches and tensor maps.
+int local_query_map(CUtensorMap *map, const LocalParams &p, const void *q, int64_t sh, int64_t st, int dtype);
+int local_key_map(CUtensorMap *map, const LocalParams &p, const void *k, int64_t sh, int64_t st, int dtype);
+int local_tc_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st);
 int local_tc_fwd(const LocalParams &p, int dtype, void *ws, size_t ws_bytes, cudaStream_t st);
 size_t local_tc_fwd_workspace(const LocalParams &p, int dtype);
 bool local_tc_fits(const LocalParams &p, int dtype);
