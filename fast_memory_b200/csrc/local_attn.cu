@@ -1,7 +1,8 @@
-// Local attention, entry points and the one-row-a-warp kernels (local_attn.cuh has the mathematics).
+// Local attention: entry points, the kernels around the tiled ones (delta, joining of key parts), and the backward pass a row
+// a warp for head dim 256 (local_attn.cuh has the mathematics).
 //
 // The row kernels hold a query (or a key) in registers and walk the runs of visible rows, one dot product and one shuffle
-// reduction a pair: no tiles, no masks, fp32 throughout.  They serve what the tiled kernels do not.
+// reduction a pair: no tiles, no masks, fp32 throughout.
 #include "local_tc.cuh"
 
 #include <type_traits>
@@ -12,13 +13,46 @@ namespace {
 
 constexpr int kRowThreads = 256;
 
-template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) local_rows_fwd_kernel(LocalParams p)
+// One warp a row: the parts' rows weighted by e^(lse_part - max).  A part that was not finite sends the row through
+// local_row_forward.
+template <typename T, int D>
+__global__ void __launch_bounds__(kRowThreads) local_combine_kernel(const __grid_constant__ LocalParams p, const float *part_o, const float *part_lse, int parts)
 {
-    const int64_t w = (int64_t(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
-    if (w >= int64_t(p.Hq) * p.S) return;
-    const int head = int(w / p.S), r = int(w % p.S);
-    const Doc doc = local_doc(p, p.cu_q ? local_find(p.cu_q, p.n_docs, r) : p.table ? r : 0);
-    local_row_forward<T, D>(p, doc, head, r - doc.q0);
+    const int64_t row = (int64_t(blockIdx.x) * kRowThreads + threadIdx.x) >> 5, rows = int64_t(p.Hq) * p.S;
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 31;
+    float m = -INFINITY;
+    bool bad = false;
+    for (int i = lane; i < parts; i += 32) {
+        const float x = part_lse[i * rows + row];
+        bad = bad || x != x;
+        m = fmaxf(m, x);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (__any_sync(0xffffffffu, bad)) {
+        const int r = int(row % p.S);
+        const Doc doc = local_doc(p, p.cu_q ? local_find(p.cu_q, p.n_docs, r) : p.table ? r : 0);
+        local_row_forward<T, D>(p, doc, int(row / p.S), r - doc.q0);
+        return;
+    }
+    constexpr int N = (D + 31) / 32;                                           // N consecutive columns a lane
+    if (lane * N >= D) return;
+    float acc[N] = {}, total = 0.f;
+    if (m > -INFINITY)
+        for (int i = 0; i < parts; ++i) {
+            const float w = expf(part_lse[i * rows + row] - m);
+            if (w == 0.f) continue;
+            total += w;
+            const float *src = part_o + (i * rows + row) * D + lane * N;
+#pragma unroll
+            for (int c = 0; c < N; ++c) acc[c] = fmaf(w, src[c], acc[c]);
+        }
+    const float inv = total > 0.f ? 1.f / total : 0.f;
+    T *dst = static_cast<T *>(p.o) + row * D + lane * N;
+#pragma unroll
+    for (int c = 0; c < N; ++c) dst[c] = Elem<T>::from_f32(acc[c] * inv);
+    if (lane == 0) p.lse[row] = total > 0.f ? m + logf(total) : -INFINITY;
 }
 
 // delta[row] = dO . O - d_lse
@@ -74,12 +108,11 @@ template <typename F> int with_type(int dtype, int d, F &&f)
 
 }  // namespace
 
-int local_rows_fwd(const LocalParams &p, int dtype, cudaStream_t st)
+int local_combine(const LocalParams &p, int dtype, const float *part_o, const float *part_lse, int parts, cudaStream_t st)
 {
     return with_type(dtype, p.d, [&](auto t, auto dim) -> int {
-        using T = decltype(t);
-        local_rows_fwd_kernel<T, decltype(dim)::value><<<row_grid(int64_t(p.Hq) * p.S), kRowThreads, 0, st>>>(p);
-        FM_LAUNCHED("local_rows_fwd_kernel");
+        local_combine_kernel<decltype(t), decltype(dim)::value><<<row_grid(int64_t(p.Hq) * p.S), kRowThreads, 0, st>>>(p, part_o, part_lse, parts);
+        FM_LAUNCHED("local_combine_kernel");
         return FM_OK;
     });
 }
@@ -157,7 +190,8 @@ extern "C" {
 size_t fm_local_attn_workspace_bytes(const fm_local_attn_args *a)
 {
     fm::LocalParams p;
-    return fm::local_params(a, p) ? 0 : fm::local_tc_fwd_workspace(p, a->dtype) + 256;
+    if (fm::local_params(a, p) || p.S == 0) return 256;
+    return (fm::local_tc_fits(p, a->dtype) ? fm::local_tc_fwd_workspace(p) : fm::local_simt_fwd_workspace(p)) + 256;
 }
 
 int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *workspace, size_t workspace_bytes, fm_stream_t stream)
@@ -175,8 +209,8 @@ int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *wo
     p.o = o;
     p.lse = lse;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (local_tc_fits(p, a->dtype)) return local_tc_fwd(p, a->dtype, workspace, workspace_bytes, st);
-    return local_rows_fwd(p, a->dtype, st);
+    if (local_tc_fits(p, a->dtype)) return local_tc_fwd(p, a->dtype, workspace, st);
+    return local_simt_fwd(p, a->dtype, workspace, st);
 }
 
 size_t fm_local_attn_bwd_workspace_bytes(const fm_local_attn_args *a)
@@ -219,7 +253,7 @@ int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *l
         if (rc) return rc;
     }
     if (p.S > 0 && local_tc_fits(p, a->dtype)) return local_tc_bwd(p, g, a->dtype, st);
-    return local_rows_bwd(p, g, a->dtype, st);
+    return local_simt_bwd(p, g, a->dtype, st);
 }
 
 }  // extern "C"

@@ -261,8 +261,7 @@ template <typename T, int DIM> __device__ __forceinline__ void local_row_dkv(con
     dv.store(static_cast<T *>(g.dv) + row * DIM, 1.f);
 }
 
-// ---- launch paths ------------------------------------------------------------------------------------------------------
-int local_rows_fwd(const LocalParams &p, int dtype, cudaStream_t st);
+// ---- backward a row a warp ------------------------------------------------------------------------------------------------------
 int local_rows_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st);
 
 }  // namespace fm

@@ -443,47 +443,6 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
     if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
 }
 
-// One warp a row: the parts' rows weighted by e^(lse_part - max).  A part that was not finite sends the row through
-// local_row_forward.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) local_combine_kernel(const __grid_constant__ LocalParams p, const float *part_o, const float *part_lse, int parts)
-{
-    const int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> 5, rows = int64_t(p.Hq) * p.S;
-    if (row >= rows) return;
-    const int lane = threadIdx.x & 31;
-    float m = -INFINITY;
-    bool bad = false;
-    for (int i = lane; i < parts; i += 32) {
-        const float x = part_lse[i * rows + row];
-        bad = bad || x != x;
-        m = fmaxf(m, x);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (__any_sync(0xffffffffu, bad)) {
-        const int r = int(row % p.S);
-        const Doc doc = local_doc(p, p.cu_q ? local_find(p.cu_q, p.n_docs, r) : p.table ? r : 0);
-        local_row_forward<T, D>(p, doc, int(row / p.S), r - doc.q0);
-        return;
-    }
-    constexpr int N = D / 32;                                                  // N consecutive columns a lane
-    float acc[N] = {}, total = 0.f;
-    if (m > -INFINITY)
-        for (int i = 0; i < parts; ++i) {
-            const float w = expf(part_lse[i * rows + row] - m);
-            if (w == 0.f) continue;
-            total += w;
-            const float *src = part_o + (i * rows + row) * D + lane * N;
-#pragma unroll
-            for (int c = 0; c < N; ++c) acc[c] = fmaf(w, src[c], acc[c]);
-        }
-    const float inv = total > 0.f ? 1.f / total : 0.f;
-    T *dst = static_cast<T *>(p.o) + row * D + lane * N;
-#pragma unroll
-    for (int c = 0; c < N; ++c) dst[c] = Elem<T>::from_f32(acc[c] * inv);
-    if (lane == 0) p.lse[row] = total > 0.f ? m + logf(total) : -INFINITY;
-}
-
 // Blocks of query tiles, at most, and the parts that their key tiles are cut into: only where the blocks fill less than half
 // of the SMs, with at least four key tiles a part.
 struct Shape {
@@ -518,11 +477,7 @@ template <typename T, int D> int launch(const LocalParams &p, int dtype, void *w
     local_fwd_kernel<T, D><<<dim3(unsigned(sh.blocks), unsigned(sh.parts)), kThreads, C::kSmem, st>>>(
         p, tm_q, tm_k, tm_v, tc::instr_desc_f16(bf16, ltc::kTile, ltc::kTile), tc::instr_desc_f16(bf16, ltc::kTile, D, false, true), part_o, part_lse);
     FM_LAUNCHED("local_fwd_kernel");
-    if (sh.parts > 1) {
-        local_combine_kernel<T, D><<<unsigned(ceil_div(int64_t(p.Hq) * p.S * 32, 256)), 256, 0, st>>>(p, part_o, part_lse, sh.parts);
-        FM_LAUNCHED("local_combine_kernel");
-    }
-    return FM_OK;
+    return sh.parts > 1 ? local_combine(p, dtype, part_o, part_lse, sh.parts, st) : FM_OK;
 }
 
 }  // namespace
@@ -556,16 +511,14 @@ bool local_tc_fits(const LocalParams &p, int dtype)
            (p.table ? p.table_ld > 0 && int64_t(p.n_pages) * p.H < (int64_t(1) << 31) : p.N > 0);
 }
 
-size_t local_tc_fwd_workspace(const LocalParams &p, int dtype)
+size_t local_tc_fwd_workspace(const LocalParams &p)
 {
-    if (!local_tc_fits(p, dtype)) return 0;
     const Shape s = shape_of(p);
     return s.parts > 1 ? (size_t(s.parts) * p.Hq * p.S * (p.d + 1) + 64) * sizeof(float) : 0;
 }
 
-int local_tc_fwd(const LocalParams &p, int dtype, void *ws, size_t ws_bytes, cudaStream_t st)
+int local_tc_fwd(const LocalParams &p, int dtype, void *ws, cudaStream_t st)
 {
-    (void)ws_bytes;
     if (dtype == FM_BF16) return p.d == 128 ? launch<__nv_bfloat16, 128>(p, dtype, ws, st) : launch<__nv_bfloat16, 64>(p, dtype, ws, st);
     return p.d == 128 ? launch<__half, 128>(p, dtype, ws, st) : launch<__half, 64>(p, dtype, ws, st);
 }

@@ -54,12 +54,19 @@ template <bool KEYS> __device__ __forceinline__ int2 find_block(const LocalParam
 
 }  // namespace ltc
 
+// CUDA-core tiles: every type and head dim.
+size_t local_simt_fwd_workspace(const LocalParams &p);
+int local_simt_fwd(const LocalParams &p, int dtype, void *ws, cudaStream_t st);
+int local_simt_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st);
+// Joins the parts [parts, Hq S, d], fp32 rows and their LSE, that a forward kernel left (local_attn.cu).
+int local_combine(const LocalParams &p, int dtype, const float *part_o, const float *part_lse, int parts, cudaStream_t st);
+
 // Whether a call goes to the tcgen05 kernels, their launches and tensor maps.
 int local_query_map(CUtensorMap *map, const LocalParams &p, const void *q, int64_t sh, int64_t st, int dtype);
 int local_key_map(CUtensorMap *map, const LocalParams &p, const void *k, int64_t sh, int64_t st, int dtype);
 int local_tc_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st);
-int local_tc_fwd(const LocalParams &p, int dtype, void *ws, size_t ws_bytes, cudaStream_t st);
-size_t local_tc_fwd_workspace(const LocalParams &p, int dtype);
+int local_tc_fwd(const LocalParams &p, int dtype, void *ws, cudaStream_t st);
+size_t local_tc_fwd_workspace(const LocalParams &p);
 bool local_tc_fits(const LocalParams &p, int dtype);
 
 }  // namespace fm
