@@ -20,7 +20,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib as L
-from .local import _int32, _on, _prefix_sums, _rows, paged_attention
+from .local import _int32, _on, _prefix_sums, _rows, _scratch, _stream, paged_attention
 
 Seqs = Union[torch.Tensor, Sequence[int]]
 
@@ -76,8 +76,7 @@ class PagedCache:
         self._ref = ctypes.byref(self._args)
 
     def _workspace(self, n: int) -> torch.Tensor:
-        # one a call: a captured graph keeps its own
-        return torch.empty(L.lib().fm_page_cache_workspace_bytes(self._ref, n), dtype=torch.uint8, device=self.device)
+        return _scratch(L.lib().fm_page_cache_workspace_bytes(self._ref, n), self.device)
 
     def _seqs(self, seqs: Seqs, name: str = "seqs") -> torch.Tensor:
         t = _int32(seqs, self.device, name)
@@ -109,7 +108,7 @@ class PagedCache:
             ws = self._workspace(seqs.numel())
             L.check(L.lib().fm_cache_append(self._ref, seqs.data_ptr(), seqs.numel(), L.ptr(cu), k_new.data_ptr(), v_new.data_ptr(),
                                             k_new.shape[1], k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1),
-                                            ws.data_ptr(), ws.numel(), L.stream_ptr(dev)), "fm_cache_append")
+                                            ws.data_ptr(), ws.numel(), _stream(dev)), "fm_cache_append")
 
     def fork(self, parents: Seqs, children: Seqs) -> None:
         """The empty sequence ``children[i]`` becomes a copy of ``parents[i]``: full pages are shared, the rows of a last page
@@ -120,21 +119,21 @@ class PagedCache:
         with _on(self.device):
             ws = self._workspace(children.numel())
             L.check(L.lib().fm_cache_fork(self._ref, parents.data_ptr(), children.data_ptr(), children.numel(), ws.data_ptr(), ws.numel(),
-                                          L.stream_ptr(self.device)), "fm_cache_fork")
+                                          _stream(self.device)), "fm_cache_fork")
 
     def free(self, seqs: Seqs) -> None:
         """Empty these sequences; pages that no other sequence shares become free."""
         seqs = self._seqs(seqs)
         with _on(self.device):
             ws = self._workspace(seqs.numel())
-            L.check(L.lib().fm_cache_free(self._ref, seqs.data_ptr(), seqs.numel(), ws.data_ptr(), ws.numel(), L.stream_ptr(self.device)),
+            L.check(L.lib().fm_cache_free(self._ref, seqs.data_ptr(), seqs.numel(), ws.data_ptr(), ws.numel(), _stream(self.device)),
                     "fm_cache_free")
 
     def compact(self) -> None:
         """Move the used pages to the low end of the pool (the fewest moves that do it); tables follow."""
         with _on(self.device):
             ws = self._workspace(0)
-            L.check(L.lib().fm_cache_compact(self._ref, ws.data_ptr(), ws.numel(), L.stream_ptr(self.device)), "fm_cache_compact")
+            L.check(L.lib().fm_cache_compact(self._ref, ws.data_ptr(), ws.numel(), _stream(self.device)), "fm_cache_compact")
 
     def copy_pages(self, src: Seqs, dst: Seqs) -> None:
         """Contents of pages ``src[i]`` to ``dst[i]`` (keys and values), tables untouched.  ``dst`` names no page twice and none
@@ -143,7 +142,7 @@ class PagedCache:
         if src.numel() != dst.numel():
             raise ValueError("src and dst must pair up")
         with _on(self.device):
-            L.check(L.lib().fm_cache_copy_pages(self._ref, src.data_ptr(), dst.data_ptr(), src.numel(), L.stream_ptr(self.device)),
+            L.check(L.lib().fm_cache_copy_pages(self._ref, src.data_ptr(), dst.data_ptr(), src.numel(), _stream(self.device)),
                     "fm_cache_copy_pages")
 
     def gather(self, seqs: Seqs, cu: Seqs, starts: Optional[Seqs] = None, n_tokens: Optional[int] = None
@@ -162,7 +161,7 @@ class PagedCache:
         k, v = (torch.empty(self.n_heads, n_tokens, self.d, dtype=self.k_pages.dtype, device=self.device) for _ in range(2))
         with _on(self.device):
             L.check(L.lib().fm_cache_gather(self._ref, seqs.data_ptr(), cu.data_ptr(), L.ptr(starts), seqs.numel(), n_tokens, k.data_ptr(),
-                                            v.data_ptr(), L.stream_ptr(self.device)), "fm_cache_gather")
+                                            v.data_ptr(), _stream(self.device)), "fm_cache_gather")
         return k, v
 
     # ---- attention ---------------------------------------------------------------------------------

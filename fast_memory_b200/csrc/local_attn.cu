@@ -190,8 +190,8 @@ extern "C" {
 size_t fm_local_attn_workspace_bytes(const fm_local_attn_args *a)
 {
     fm::LocalParams p;
-    if (fm::local_params(a, p) || p.S == 0) return 256;
-    return (fm::local_tc_fits(p, a->dtype) ? fm::local_tc_fwd_workspace(p) : fm::local_simt_fwd_workspace(p)) + 256;
+    if (fm::local_params(a, p) || p.S == 0) return 0;
+    return fm::local_tc_fits(p, a->dtype) ? fm::local_tc_fwd_workspace(p) : fm::local_simt_fwd_workspace(p);
 }
 
 int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *workspace, size_t workspace_bytes, fm_stream_t stream)
@@ -201,8 +201,9 @@ int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *wo
     if (int rc = local_params(a, p)) return rc;
     if (p.S == 0) return FM_OK;
     FM_REQUIRE(p.q && o && lse && (p.table || p.N == 0 || (p.k && p.v)), "fm_local_attn_fwd: null pointer");
-    if (workspace_bytes < fm_local_attn_workspace_bytes(a) || !workspace) {
-        set_error("fm_local_attn_fwd: workspace of %zu bytes, %zu are needed", workspace_bytes, fm_local_attn_workspace_bytes(a));
+    const size_t need = local_tc_fits(p, a->dtype) ? local_tc_fwd_workspace(p) : local_simt_fwd_workspace(p);
+    if (need && (workspace_bytes < need || !workspace)) {
+        set_error("fm_local_attn_fwd: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
         return FM_ERR_WORKSPACE;
     }
     FM_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0 && reinterpret_cast<uintptr_t>(o) % 16 == 0, "fm_local_attn_fwd: misaligned buffer");

@@ -210,48 +210,44 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 if (lane == 0) tc::mbar_arrive(bar_addr(&sh.stat_full[buf]));
             }
             if (!ok && lane == 0) *abort_flag = 1;
-        } else if (warp == kMmaWarp && lane == 0 && n_q > 0) {
-            bool ok = tc::mbar_wait_or_abort(bar_addr(&sh.kv_full), 0, abort_flag);
+        } else if (warp == kMmaWarp && n_q > 0) {
+            const uint32_t tm = uniform(int(tmem));
+            const int n = uniform(n_q);
+            const bool leader = tc::elect_one();
+            bool ok = true;
+            auto wait = [&](uint64_t *bar, int parity) { ok = ok && tc::mbar_wait_or_abort(bar_addr(bar), parity, abort_flag); };
             auto q_tile = [&](int i) { return s_q0 + (i % C::kStages) * 2 * C::kTileB; };
-            auto wait_q = [&](int i) { ok = ok && tc::mbar_wait_or_abort(bar_addr(&sh.full[i % C::kStages]), (i / C::kStages) & 1, abort_flag); };
-            auto scores = [&](int i) {
+            auto wait_q = [&](int i) { wait(&sh.full[i % C::kStages], (i / C::kStages) & 1); };
+            auto product = [&](uint32_t d, uint32_t a_tile, uint32_t b_tile, uint64_t *bar) {            // S^T or dP^T
+                const uint64_t a = desc_k(a_tile, 0), b = desc_k(b_tile, 0);
 #pragma unroll
-                for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16(tmem, desc_k(s_k, ks), desc_k(q_tile(i), ks), idesc_s, ks > 0);
-                tc::umma_commit(bar_addr(&sh.s_full));
+                for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16_if(leader && ok, d, a + step_k(ks), b + step_k(ks), idesc_s, ks > 0);
+                tc::umma_commit_if(leader, bar_addr(bar));
             };
-            auto dprob = [&](int i) {
+            auto gather = [&](uint32_t d, uint32_t a, uint32_t b_tile, bool more) {                       // dV or dK
+                const uint64_t b = desc_mn(b_tile, 0);
 #pragma unroll
-                for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16(tmem + 128, desc_k(s_v, ks), desc_k(q_tile(i) + C::kTileB, ks), idesc_s, ks > 0);
-                tc::umma_commit(bar_addr(&sh.dp_full));
+                for (int ks = 0; ks < kTile / 16; ++ks)
+                    tc::umma_f16_ts_if(leader && ok, d, a + (ks >> 2) * 64 + (ks & 3) * 8, b + step_mn(ks), idesc_o, more || ks > 0);
             };
+            wait(&sh.kv_full, 0);
             wait_q(0);
-            if (ok) {
-                scores(0);
-                dprob(0);
-            }
-            for (int i = 0; i < n_q && ok; ++i) {
-                ok = tc::mbar_wait_or_abort(bar_addr(&sh.p_full), i & 1, abort_flag);
-                if (!ok) break;
+            product(tm, s_k, q_tile(0), &sh.s_full);
+            product(tm + 128, s_v, q_tile(0) + C::kTileB, &sh.dp_full);
+            for (int i = 0; i < n; ++i) {
+                if (i + 1 < n) wait_q(i + 1);                                  // there long before P is
+                wait(&sh.p_full, i & 1);
                 tc::fence_after_sync();
-#pragma unroll
-                for (int ks = 0; ks < kTile / 16; ++ks)
-                    tc::umma_f16_ts(tmem + 256, tmem + (ks >> 2) * 64 + (ks & 3) * 8, desc_mn(q_tile(i) + C::kTileB, ks), idesc_o, i > 0 || ks > 0);
-                if (i + 1 < n_q) {
-                    wait_q(i + 1);
-                    if (!ok) break;
-                    scores(i + 1);
-                }
-                ok = tc::mbar_wait_or_abort(bar_addr(&sh.ds_full), i & 1, abort_flag);
-                if (!ok) break;
+                gather(tm + 256, tm, q_tile(i) + C::kTileB, i > 0);
+                if (i + 1 < n) product(tm, s_k, q_tile(i + 1), &sh.s_full);
+                wait(&sh.ds_full, i & 1);
                 tc::fence_after_sync();
-#pragma unroll
-                for (int ks = 0; ks < kTile / 16; ++ks)
-                    tc::umma_f16_ts(tmem + 384, tmem + 128 + (ks >> 2) * 64 + (ks & 3) * 8, desc_mn(q_tile(i), ks), idesc_o, i > 0 || ks > 0);
-                tc::umma_commit(bar_addr(&sh.empty[i % C::kStages]));
-                if (i + 1 < n_q) dprob(i + 1);
+                gather(tm + 384, tm + 128, q_tile(i), i > 0);
+                tc::umma_commit_if(leader, bar_addr(&sh.empty[i % C::kStages]));
+                if (i + 1 < n) product(tm + 128, s_v, q_tile(i + 1) + C::kTileB, &sh.dp_full);
             }
-            if (!ok) *abort_flag = 1;
-            tc::umma_commit(bar_addr(&sh.drain));
+            if (leader && !ok) *abort_flag = 1;
+            tc::umma_commit_if(leader, bar_addr(&sh.drain));
             tc::mbar_wait(bar_addr(&sh.drain), 0);
         }
     } else {
@@ -541,42 +537,38 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
                 tc::mbar_wait(bar_addr(&sh.q_full), 0);
                 for (int x = max(i - C::kRing, 0); x < i; ++x) tc::mbar_wait(bar_addr(&sh.full[x % C::kRing]), (x / C::kRing) & 1);
             }
-        } else if (warp == kMmaWarp && lane == 0 && n_k > 0) {
-            bool ok = tc::mbar_wait_or_abort(bar_addr(&sh.q_full), 0, abort_flag);
-            auto tile = [&](int i) { return ring0 + (i % C::kRing) * C::kTileB; };          // i = 2 n: K, 2 n + 1: V
-            auto wait_tile = [&](int i) { ok = ok && tc::mbar_wait_or_abort(bar_addr(&sh.full[i % C::kRing]), (i / C::kRing) & 1, abort_flag); };
-            auto scores = [&](int n) {
-                wait_tile(2 * n);
-                if (!ok) return;
+        } else if (warp == kMmaWarp && n_k > 0) {
+            const uint32_t tm = uniform(int(tmem));
+            const int tiles = uniform(n_k);
+            const bool leader = tc::elect_one();
+            bool ok = true;
+            auto wait = [&](uint64_t *bar, int parity) { ok = ok && tc::mbar_wait_or_abort(bar_addr(bar), parity, abort_flag); };
+            auto tile = [&](int i) { return ring0 + (i % C::kRing) * C::kTileB; };                        // i = 2 n: K, 2 n + 1: V
+            auto product = [&](uint32_t d, uint32_t a_tile, int i, uint64_t *bar) {                       // S or dP
+                wait(&sh.full[i % C::kRing], (i / C::kRing) & 1);
+                const uint64_t a = desc_k(a_tile, 0), b = desc_k(tile(i), 0);
 #pragma unroll
-                for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16(tmem + (n & 1) * 128, desc_k(s_q, ks), desc_k(tile(2 * n), ks), idesc_s, ks > 0);
-                tc::umma_commit(bar_addr(&sh.s_full[n & 1]));
+                for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16_if(leader && ok, d, a + step_k(ks), b + step_k(ks), idesc_s, ks > 0);
+                tc::umma_commit_if(leader, bar_addr(bar));
+                if (i & 1) tc::umma_commit_if(leader, bar_addr(&sh.empty[i % C::kRing]));
             };
-            auto dprob = [&](int n) {
-                wait_tile(2 * n + 1);
-                if (!ok) return;
-#pragma unroll
-                for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16(tmem + 256, desc_k(s_do, ks), desc_k(tile(2 * n + 1), ks), idesc_s, ks > 0);
-                tc::umma_commit(bar_addr(&sh.dp_full));
-                tc::umma_commit(bar_addr(&sh.empty[(2 * n + 1) % C::kRing]));
-            };
-            scores(0);
-            dprob(0);
-            if (n_k > 1) scores(1);
-            for (int n = 0; n < n_k && ok; ++n) {
-                ok = tc::mbar_wait_or_abort(bar_addr(&sh.ds_full), n & 1, abort_flag);
-                if (!ok) break;
+            wait(&sh.q_full, 0);
+            product(tm, s_q, 0, &sh.s_full[0]);
+            product(tm + 256, s_do, 1, &sh.dp_full);
+            if (tiles > 1) product(tm + 128, s_q, 2, &sh.s_full[1]);
+            for (int n = 0; n < tiles; ++n) {
+                wait(&sh.ds_full, n & 1);
                 tc::fence_after_sync();
-                if (n + 1 < n_k) dprob(n + 1);
-                if (!ok) break;
+                if (n + 1 < tiles) product(tm + 256, s_do, 2 * n + 3, &sh.dp_full);
+                const uint64_t k = desc_mn(tile(2 * n), 0);
 #pragma unroll
                 for (int ks = 0; ks < kTile / 16; ++ks)
-                    tc::umma_f16_ts(tmem + 384, tmem + (n & 1) * 128 + (ks >> 2) * 64 + (ks & 3) * 8, desc_mn(tile(2 * n), ks), idesc_o, n > 0 || ks > 0);
-                tc::umma_commit(bar_addr(&sh.empty[(2 * n) % C::kRing]));
-                if (n + 2 < n_k) scores(n + 2);
+                    tc::umma_f16_ts_if(leader && ok, tm + 384, tm + (n & 1) * 128 + (ks >> 2) * 64 + (ks & 3) * 8, k + step_mn(ks), idesc_o, n > 0 || ks > 0);
+                tc::umma_commit_if(leader, bar_addr(&sh.empty[(2 * n) % C::kRing]));
+                if (n + 2 < tiles) product(tm + (n & 1) * 128, s_q, 2 * n + 4, &sh.s_full[n & 1]);
             }
-            if (!ok) *abort_flag = 1;
-            tc::umma_commit(bar_addr(&sh.drain));
+            if (leader && !ok) *abort_flag = 1;
+            tc::umma_commit_if(leader, bar_addr(&sh.drain));
             tc::mbar_wait(bar_addr(&sh.drain), 0);
         }
     } else {

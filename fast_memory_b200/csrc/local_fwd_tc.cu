@@ -3,17 +3,19 @@
 // A CTA owns two query tiles of 128 rows - row = (token, head of the group), so that a tile reads its KV head's keys once for
 // the whole group - and streams the key tiles that either of them sees:
 //     S [128 x 128] = Q K^T        A = Q, B = K, both K-major in shared memory (TMA, 128-byte swizzle); fp32 in TMEM
-//     P = 2^(s - m)                thread = row: 128 scores in registers, running maximum m and sum l, no shuffles;
-//                                  P goes back to TMEM over S as packed 16-bit: the A operand of the second product
+//     P = 2^(s - m)                two threads a row: 64 scores in registers, sum l, no shuffles; P goes back to TMEM over S as
+//                                  packed 16-bit: the A operand of the second product
 //     O [128 x d] += P V           B = V, the same tile layout read MN-major; fp32 in TMEM (S0 S1 O0 O1 = 512 columns)
-// The two tiles take turns: while one's 128 threads do a softmax, the tensor core works for the other.  m is only moved when a
-// row's maximum has grown by more than 2^8 (the sums are fp32 and P is a floating-point number: a late reference costs no
-// accuracy), so O is rescaled in TMEM a few times a row instead of once a tile.
+// The two tiles take turns: while one's 256 threads do a softmax, the tensor core works for the other.  The reference m is the
+// maximum of the row's first tile and is renewed only when a tile's sum of p exceeds 2^12: the sums are fp32 and P is a
+// floating-point number (fp16 reaches 2^16), so a reference that is too small costs no accuracy.  Most tiles then need no maximum
+// at all (600 of 2300 cycles of a tile's softmax), and O is rescaled in TMEM next to never.
 // l sums the unrounded p; P is rounded to the element type because the second product takes 16-bit operands.
 //
-//   warps 0-3, 4-7   softmax and epilogue of tile 0, 1 (a warp reaches its own quarter of the TMEM lanes)
-//   warp 8           one thread issues all products
-//   warp 9           TMA: query tiles, then K and V tiles through one ring; a paged tile is one box a page, its addresses looked
+//   warps 0-7, 8-15  softmax and epilogue of tile 0, 1; two threads a row, 64 columns each (a warp reaches its own quarter of
+//                    the TMEM lanes)
+//   warp 16          issues all products
+//   warp 17          TMA: query tiles, then K and V tiles through one ring; a paged tile is one box a page, its addresses looked
 //                    up by the lanes side by side.  Rows behind the document's last key are zeroed in the V tile: they would
 //                    meet P = 0, and 0 * NaN is NaN
 // A hidden key INSIDE the document can still hold a NaN value.  It shows as a result that is not finite; such rows are computed
@@ -29,14 +31,13 @@ namespace {
 
 using namespace ltc;
 
-constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kLoadWarp = 9;        // warps 10 and 11 complete the third warpgroup: registers are split by warpgroup
-constexpr float kLazy = 8.f;                        // how far (log2) a row maximum may outgrow the reference before O is rescaled
+constexpr int kThreads = 640;
+constexpr int kMmaWarp = 16, kLoadWarp = 17;        // warps 18 and 19 complete the fifth warpgroup: registers are split by warpgroup
+constexpr float kMostSum = 4096.f;                  // sum of a tile's p from which a row's reference is renewed
 
 template <int D> struct Cfg {
     static constexpr uint32_t kTileBytes = uint32_t(D / 64) * kBlock;
     static constexpr int kRing = D == 128 ? 5 : 8;  // K and V tiles in flight or in use
-    static constexpr uint32_t kSmem = (2 + kRing) * kTileBytes + 1024;
 };
 
 struct Block {
@@ -60,7 +61,10 @@ template <int D> struct Shared {
     uint32_t tmem_slot;
     int abort;
     Block b;
+    float half[2][2][kTile];                        // per query tile, half and row: what the two threads of a row tell each other
+    unsigned again[2][4];                           // rows whose result is not finite
 };
+template <int D> constexpr uint32_t smem_bytes() { return (2 + Cfg<D>::kRing) * Cfg<D>::kTileBytes + uint32_t(sizeof(Shared<D>)); }
 
 __device__ __forceinline__ void make_block(const LocalParams &p, Block &b, int doc, int index, int h, int part, int parts)
 {
@@ -89,10 +93,10 @@ __device__ __forceinline__ void make_block(const LocalParams &p, Block &b, int d
 }
 
 // Column c of the tile is a visible key if it lies in [a, b) or below pre.
-__device__ __forceinline__ void mask_scores(uint32_t (&s)[4][32], int a, int b, int pre)
+__device__ __forceinline__ void mask_scores(uint32_t (&s)[2][32], int a, int b, int pre)
 {
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
             const int j = x * 32 + c;
@@ -100,35 +104,83 @@ __device__ __forceinline__ void mask_scores(uint32_t (&s)[4][32], int a, int b, 
         }
 }
 
-// Scores in log2 units after scale, cap and distance; what is left to multiply is 1.
-__device__ __forceinline__ void shape_scores(const LocalParams &p, uint32_t (&s)[4][32], float slope2, float fp)
+// Scores in log2 units after scale, cap and distance (fp: the row's position less the first column's); what is left to multiply
+// is 1.
+__device__ __forceinline__ void shape_scores(const LocalParams &p, uint32_t (&s)[2][32], float slope2, float fp)
 {
     if (p.cap > 0.f) {
-        // cap tanh(x) = cap - 2 cap / (1 + e^2x): e^2x = inf gives cap, 0 gives -cap
-        const float k = 2.f * kLog2e * p.scale / p.cap, c2 = p.cap * kLog2e;
+        float big[2] = {0.f, 0.f};
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int c = 0; c < 32; c += 2)
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-                const float e = fast_exp2(__uint_as_float(s[x][c]) * k);
-                float r;
-                asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-                s[x][c] = __float_as_uint(fmaf(-2.f * c2, r, c2));
-            }
+            for (int x = 0; x < 2; ++x) big[x] = max3(big[x], fabsf(__uint_as_float(s[x][c])), fabsf(__uint_as_float(s[x][c + 1])));
+        const float k = p.scale / p.cap, c2 = p.cap * kLog2e;
+        if (__all_sync(0xffffffffu, fmaxf(big[0], big[1]) * fabsf(k) <= kTanhRange)) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int c = 0; c < 32; c += 2) {
+                    const float2 t = split(mul2(tanh_small(mul2(pair(s[x][c], s[x][c + 1]), pair(k, k))), pair(c2, c2)));
+                    s[x][c] = __float_as_uint(t.x);
+                    s[x][c + 1] = __float_as_uint(t.y);
+                }
+        } else {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int c = 0; c < 32; ++c) s[x][c] = __float_as_uint(c2 * tanh_any(__uint_as_float(s[x][c]) * k));
+        }
     } else {
-        const float k = p.scale * kLog2e;
+        const f32x2 scale = pair(p.scale * kLog2e, p.scale * kLog2e);
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int c = 0; c < 32; ++c) s[x][c] = __float_as_uint(__uint_as_float(s[x][c]) * k);
+            for (int c = 0; c < 32; c += 2) {
+                const float2 t = split(mul2(pair(s[x][c], s[x][c + 1]), scale));
+                s[x][c] = __float_as_uint(t.x);
+                s[x][c + 1] = __float_as_uint(t.y);
+            }
     }
-    if (slope2 != 0.f) {
+    if (p.slopes) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int c = 0; c < 32; ++c)
                 s[x][c] = __float_as_uint(fmaf(-slope2, fabsf(fp - float(x * 32 + c)), __uint_as_float(s[x][c])));
     }
+}
+
+__device__ __forceinline__ float row_max(const uint32_t (&x)[2][32])
+{
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int c = 0; c < 32; c += 4)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            mx[y] = max3(mx[y], __uint_as_float(x[y][c]), __uint_as_float(x[y][c + 1]));
+            mx[y + 2] = max3(mx[y + 2], __uint_as_float(x[y][c + 2]), __uint_as_float(x[y][c + 3]));
+        }
+    return max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+}
+
+// P = 2^(s mul - sub) of 32 columns as packed 16-bit into TMEM; adds the unrounded p to sum.
+template <typename T, bool MIX> __device__ __forceinline__ void exp_scores(const uint32_t (&x)[32], float mul, float sub, uint32_t t_p, f32x2 (&sum)[2])
+{
+    const f32x2 m2 = pair(mul, mul), n2 = pair(-sub, -sub);
+    uint32_t pk[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const f32x2 e = exp2_pair<MIX>(fma2(pair(x[2 * i], x[2 * i + 1]), m2, n2), i);
+        sum[i & 1] = add2(sum[i & 1], e);
+        const float2 v = split(e);
+        pk[i] = pack2<T>(v.x, v.y);
+    }
+    tc::tmem_st_x16(t_p, pk);
+}
+__device__ __forceinline__ float total(const f32x2 (&sum)[2])
+{
+    const float2 v = split(add2(sum[0], sum[1]));
+    return v.x + v.y;
 }
 
 template <typename T, int D> __device__ __forceinline__ void redo_rows(const LocalParams &p, const Block &b, unsigned rows, int token0, int row0)
@@ -145,12 +197,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, uint32_t idesc_s, uint32_t idesc_o, float *part_o, float *part_lse)
 {
-    extern __shared__ unsigned char smem_dyn[];
-    __shared__ __align__(16) Shared<D> sh;
+    extern __shared__ __align__(1024) unsigned char smem_dyn[];
     using C = Cfg<D>;
+    Shared<D> &sh = *reinterpret_cast<Shared<D> *>(smem_dyn + (2 + C::kRing) * C::kTileBytes);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t base = (tc::smem_addr(smem_dyn) + 1023u) & ~1023u;
-    unsigned char *base_ptr = smem_dyn + (base - tc::smem_addr(smem_dyn));
+    const uint32_t base = tc::smem_addr(smem_dyn);
     const uint32_t ring0 = base + 2 * C::kTileBytes;
     volatile int *abort_flag = &sh.abort;
 
@@ -168,7 +219,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         for (int s = 0; s < 2; ++s) {
             tc::mbar_init(bar_addr(&sh.q_full[s]), 1);
             tc::mbar_init(bar_addr(&sh.s_full[s]), 1);
-            tc::mbar_init(bar_addr(&sh.p_full[s]), 4);
+            tc::mbar_init(bar_addr(&sh.p_full[s]), 8);
             tc::mbar_init(bar_addr(&sh.o_done[s]), 1);
         }
         for (int i = 0; i < C::kRing; ++i) {
@@ -183,6 +234,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         tc::prefetch_tensormap(&tm_k);
         tc::prefetch_tensormap(&tm_v);
     }
+    if (tid < 8) sh.again[tid >> 2][tid & 3] = 0;
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -190,9 +242,9 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
     const uint32_t tmem = sh.tmem_slot;
     const int n0 = b.n0, n1 = b.n1;
 
-    // 384 threads x 168 registers at launch = 256 x 216 + 128 x 72
-    if (warp >= 8) {
-        tc::set_registers_down<72>();
+    // 640 threads x 96 registers at launch = 512 x 104 + 128 x 64
+    if (warp >= 16) {
+        tc::set_registers_down<64>();
         if (warp == kLoadWarp) {
             // ---- loads ----------------------------------------------------------------------------------------------------
             if (n1 > n0) {
@@ -241,7 +293,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                             for (int i = rows * 8 + lane; i < kTile * 8; i += 32)
     #pragma unroll
                                 for (int c = 0; c < D / 64; ++c)
-                                    *reinterpret_cast<uint4 *>(base_ptr + (dst - base) + c * kBlock + i * 16) = make_uint4(0, 0, 0, 0);
+                                    *reinterpret_cast<uint4 *>(smem_dyn + (dst - base) + c * kBlock + i * 16) = make_uint4(0, 0, 0, 0);
                             tc::fence_proxy_async_smem();
                             __syncwarp();
                             if (lane == 0) tc::mbar_arrive(bar_addr(&sh.full[slot]));
@@ -257,145 +309,170 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 }
             }
         } else if (warp == kMmaWarp) {
-            // ---- products -------------------------------------------------------------------------------------------------
-            if (lane == 0 && n1 > n0) {
-                bool ok = true;
-                int done[2] = {0, 0};                                              // key tiles of each query tile so far
-                auto ring_wait = [&](int i) { ok = ok && tc::mbar_wait_or_abort(bar_addr(&sh.full[i % C::kRing]), (i / C::kRing) & 1, abort_flag); };
-                auto scores = [&](int s, int n) {                                  // S of query tile s and key tile n
-                    const uint32_t q = base + s * C::kTileBytes, k = ring0 + ((2 * (n - n0)) % C::kRing) * C::kTileBytes;
-    #pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks) tc::umma_f16(tmem + s * 128, desc_k(q, ks), desc_k(k, ks), idesc_s, ks > 0);
-                    tc::umma_commit(bar_addr(&sh.s_full[s]));
+            // ---- products ---------------------------------------------------------------------------------------------
+            const uint32_t tm = uniform(int(tmem));
+            const int m0 = uniform(n0), m1 = uniform(n1), n_pre = uniform(b.n_pre), first = uniform(b.lo0);
+            const int on[2] = {uniform(b.t0[0] < b.t1[0]), uniform(b.t0[1] < b.t1[1])};
+            const int lo[2] = {uniform(b.lo[0]), uniform(b.lo[1])}, hi[2] = {uniform(b.hi[0]), uniform(b.hi[1])};
+            auto active = [&](int s, int n) { const int kt = first + n - n_pre; return on[s] && (n < n_pre || (kt >= lo[s] && kt < hi[s])); };
+            if (m1 > m0) {
+                const bool leader = tc::elect_one();
+                bool ok = true;                                                // (what the leader's waits said; the others follow the same path)
+                int done[2] = {0, 0};                                          // key tiles of each query tile so far
+                auto wait = [&](uint64_t *bar, int parity) { ok = ok && tc::mbar_wait_or_abort(bar_addr(bar), parity, abort_flag); };
+                auto ring_wait = [&](int i) { wait(&sh.full[i % C::kRing], (i / C::kRing) & 1); };
+                auto commit = [&](uint64_t *bar) { tc::umma_commit_if(leader, bar_addr(bar)); };
+                auto scores = [&](int s, int n) {                              // S of query tile s and key tile n
+                    const uint64_t q = desc_k(base + s * C::kTileBytes, 0), k = desc_k(ring0 + ((2 * (n - m0)) % C::kRing) * C::kTileBytes, 0);
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) tc::umma_f16_if(leader && ok, tm + s * 128, q + step_k(ks), k + step_k(ks), idesc_s, ks > 0);
+                    commit(&sh.s_full[s]);
                 };
                 ring_wait(0);
                 for (int s = 0; s < 2; ++s)
-                    if (b.t0[s] < b.t1[s]) ok = ok && tc::mbar_wait_or_abort(bar_addr(&sh.q_full[s]), 0, abort_flag);
-                if (ok) {
-                    for (int s = 0; s < 2; ++s)
-                        if (b.active(s, n0)) scores(s, n0);
-                    tc::umma_commit(bar_addr(&sh.empty[0]));
-                }
-                for (int n = n0; n < n1 && ok; ++n) {
-                    const int vi = 2 * (n - n0) + 1;
-                    const uint32_t v = ring0 + (vi % C::kRing) * C::kTileBytes;
-                    ring_wait(vi);
-                    for (int s = 0; s < 2 && ok; ++s) {
-                        if (b.active(s, n)) {
-                            ok = tc::mbar_wait_or_abort(bar_addr(&sh.p_full[s]), done[s] & 1, abort_flag);
-                            if (!ok) break;
+                    if (on[s]) wait(&sh.q_full[s], 0);
+                for (int s = 0; s < 2; ++s)
+                    if (active(s, m0)) scores(s, m0);
+                commit(&sh.empty[0]);
+                for (int n = m0; n < m1; ++n) {
+                    const int vi = 2 * (n - m0) + 1;
+                    const uint64_t v = desc_mn(ring0 + (vi % C::kRing) * C::kTileBytes, 0);
+                    ring_wait(vi);                                             // both tiles are there long before P is
+                    if (n + 1 < m1) ring_wait(vi + 1);
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        if (active(s, n)) {
+                            wait(&sh.p_full[s], done[s] & 1);
                             tc::fence_after_sync();
-    #pragma unroll
+#pragma unroll
                             for (int ks = 0; ks < kTile / 16; ++ks)
-                                tc::umma_f16_ts(tmem + 256 + s * 128, tmem + s * 128 + ks * 8, desc_mn(v, ks), idesc_o, done[s] > 0 || ks > 0);
-                            tc::umma_commit(bar_addr(&sh.o_done[s]));
+                                tc::umma_f16_ts_if(leader && ok, tm + 256 + s * 128, tm + s * 128 + (ks >> 2) * 64 + (ks & 3) * 8, v + step_mn(ks), idesc_o,
+                                                   done[s] > 0 || ks > 0);
                             ++done[s];
+                            commit(&sh.o_done[s]);
                         }
-                        if (s == 1) tc::umma_commit(bar_addr(&sh.empty[vi % C::kRing]));
-                        if (n + 1 < n1) {
-                            if (s == 0) ring_wait(vi + 1);
-                            if (ok && b.active(s, n + 1)) scores(s, n + 1);
-                            if (s == 1) tc::umma_commit(bar_addr(&sh.empty[(vi + 1) % C::kRing]));
-                        }
+                        if (n + 1 < m1 && active(s, n + 1)) scores(s, n + 1);
                     }
+                    commit(&sh.empty[vi % C::kRing]);
+                    if (n + 1 < m1) commit(&sh.empty[(vi + 1) % C::kRing]);
                 }
-                if (!ok) *abort_flag = 1;
-                tc::umma_commit(bar_addr(&sh.drain));
+                if (leader && !ok) *abort_flag = 1;
+                commit(&sh.drain);
                 tc::mbar_wait(bar_addr(&sh.drain), 0);
             }
         }
     } else {
-        tc::set_registers_up<216>();
+        tc::set_registers_up<104>();
         // ---- softmax and epilogue ---------------------------------------------------------------------------------------
-        const int s = warp >> 2, row = tid & 127;
+        const int s = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane, bar_id = 1 + s;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t t_s = tmem + s * 128 + lanes, t_o = tmem + 256 + s * 128 + lanes;
+        const uint32_t t_s = tmem + s * 128 + half * 64 + lanes, t_o = tmem + 256 + s * 128 + half * (D / 2) + lanes;
         const int token = b.t0[s] + row / p.G, head = b.h * p.G + row % p.G;
         const bool valid = row < b.tokens * p.G && token < b.t1[s];
-        const int pos = b.D.nk - b.D.nq + token;
-        const int2 run = local_run(p, pos, b.D.nk);
-        const int pos_lo = b.D.nk - b.D.nq + b.t0[s], pos_hi = b.D.nk - b.D.nq + b.t1[s] - 1;
-        const int safe_lo = p.window ? pos_hi - p.window + 1 : 0;              // keys in [safe_lo, safe_hi) are seen by every row
-        const int safe_hi = local_run(p, pos_lo, b.D.nk).y;
-        const float slope2 = p.slopes && valid ? p.slopes[head] * kLog2e : 0.f;
+        const int shift = b.D.nk - b.D.nq, pos = shift + token;
+        const int safe_lo = p.window ? shift + b.t1[s] - p.window : 0;         // keys in [safe_lo, safe_hi) are seen by every row
+        const int safe_hi = local_run(p, shift + b.t0[s], b.D.nk).y;
         const bool shaped = p.cap > 0.f || p.slopes || !(p.scale > 0.f);
         const float mul = shaped ? 1.f : p.scale * kLog2e;
         float m = -INFINITY, l = 0.f;
         int done = 0;
-        bool ok = true;
+        bool ok = true, fresh = true;                                          // fresh: some row has no reference yet
         for (int n = n0; n < n1; ++n) {
             if (!b.active(s, n)) continue;
             const int j0 = b.key_tile(n) * kTile;
             ok = tc::mbar_wait_or_abort(bar_addr(&sh.s_full[s]), done & 1, abort_flag);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            ok = tc::named_barrier_and(bar_id, 256, ok);
+            if (!ok) break;
             tc::fence_after_sync();
-            uint32_t x[4][32];
+            uint32_t x[2][32];
+            f32x2 sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+            const bool masked = !(j0 + kTile <= b.D.prefix || (j0 >= safe_lo && j0 + kTile <= safe_hi));
+            tc::tmem_ld_x32(t_s, x[0]);
+            tc::tmem_ld_wait(x[0]);
+            tc::tmem_ld_x32(t_s + 32, x[1]);
+            if (!fresh && !masked && !shaped) {
+                // the usual tile: half of the scores arrive under the exponentials of the other half
+                exp_scores<T, true>(x[0], mul, m, t_s, sums);
+                tc::tmem_ld_wait(x[1]);
+                exp_scores<T, true>(x[1], mul, m, t_s + 16, sums);
+            } else {
+                tc::tmem_ld_wait(x[1]);
+                if (shaped) shape_scores(p, x, p.slopes && valid ? p.slopes[head] * kLog2e : 0.f, float(pos - j0 - half * 64));
+                if (masked) {
+                    const int2 run = local_run(p, pos, b.D.nk);
+                    mask_scores(x, run.x - j0 - half * 64, run.y - j0 - half * 64, b.D.prefix - j0 - half * 64);
+                }
+                if (fresh) {
+                    sh.half[s][half][row] = row_max(x) * mul;
+                    tc::named_barrier(bar_id, 256);
+                    if (m == -INFINITY) m = fmaxf(sh.half[s][0][row], sh.half[s][1][row]);
+                }
+                // hidden scores need exact zeros, which the polynomial does not give
+                if (!masked && __all_sync(0xffffffffu, m > -INFINITY)) {
+                    exp_scores<T, true>(x[0], mul, m, t_s, sums);
+                    exp_scores<T, true>(x[1], mul, m, t_s + 16, sums);
+                } else {
+                    const float sub = m == -INFINITY ? 0.f : m;
+                    exp_scores<T, false>(x[0], mul, sub, t_s, sums);
+                    exp_scores<T, false>(x[1], mul, sub, t_s + 16, sums);
+                }
+            }
+            float sum = total(sums);
+            // Rows that have outgrown their reference get a new one; rows that have none yet ask the next tile for it.
+            if (tc::named_barrier_or(bar_id, 256, valid && (sum > kMostSum || m == -INFINITY))) {
+                if (tc::named_barrier_or(bar_id, 256, sum > kMostSum)) {
+                    sh.half[s][half][row] = sum > kMostSum ? 1.f : 0.f;
+                    tc::named_barrier(bar_id, 256);
+                    const bool grow = sh.half[s][0][row] + sh.half[s][1][row] > 0.f;
+                    tc::named_barrier(bar_id, 256);
+                    sh.half[s][half][row] = row_max(x) * mul;
+                    tc::named_barrier(bar_id, 256);
+                    const float top = fmaxf(sh.half[s][0][row], sh.half[s][1][row]), f = grow ? fast_exp2(m - top) : 1.f;
+                    if (done > 0) {
+                        ok = tc::mbar_wait_or_abort(bar_addr(&sh.o_done[s]), (done - 1) & 1, abort_flag);
+                        ok = tc::named_barrier_and(bar_id, 256, ok);
+                        if (!ok) break;
+                        tc::fence_after_sync();
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tc::tmem_ld_x32(t_s + c * 32, x[c]);
+                        for (int c = 0; c < D / 32; ++c) {
+                            uint32_t o[16];
+                            tc::tmem_ld_x16(t_o + c * 16, o);
+                            tc::tmem_ld_wait16(o);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tc::tmem_ld_wait(x[c]);
-            if (shaped) shape_scores(p, x, slope2, float(pos - j0));
-            if (!(j0 + kTile <= b.D.prefix || (j0 >= safe_lo && j0 + kTile <= safe_hi))) mask_scores(x, run.x - j0, run.y - j0, b.D.prefix - j0);
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-#pragma unroll
-                for (int y = 0; y < 4; ++y) mx[y] = fmaxf(mx[y], __uint_as_float(x[y][c]));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * mul;
-            if (done == 0) m = top;
-            else {
-                const bool grow = top > m + kLazy || (m == -INFINITY && top > m);
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float f = grow ? fast_exp2(m - top) : 1.f;           // 0 where nothing was seen before
-                    ok = tc::mbar_wait_or_abort(bar_addr(&sh.o_done[s]), (done - 1) & 1, abort_flag);
-                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                    tc::fence_after_sync();
-                    if (grow) { m = top; l *= f; }
-#pragma unroll
-                    for (int c = 0; c < D / 16; ++c) {
-                        uint32_t o[16];
-                        tc::tmem_ld_x16(t_o + c * 16, o);
-                        tc::tmem_ld_wait16(o);
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tc::tmem_st_x16(t_o + c * 16, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tc::tmem_st_x16(t_o + c * 16, o);
+                        }
                     }
+                    if (grow) { m = top; l *= f; }
+                    const float sub = m == -INFINITY ? 0.f : m;
+                    sums[0] = sums[1] = pair(0.f, 0.f);
+                    exp_scores<T, false>(x[0], mul, sub, t_s, sums);
+                    exp_scores<T, false>(x[1], mul, sub, t_s + 16, sums);
+                    sum = total(sums);
                 }
-            }
-            const float sub = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t pk[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float a = fast_exp2(fmaf(__uint_as_float(x[c][2 * i]), mul, -sub)), d = fast_exp2(fmaf(__uint_as_float(x[c][2 * i + 1]), mul, -sub));
-                    sum[(2 * i) & 3] += a;
-                    sum[(2 * i + 1) & 3] += d;
-                    pk[i] = pack2<T>(a, d);
-                }
-                tc::tmem_st_x16(t_s + c * 16, pk);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                fresh = tc::named_barrier_or(bar_id, 256, valid && m == -INFINITY);
+            } else fresh = false;
+            l += sum;
             tc::tmem_st_wait();
             tc::fence_before_sync();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(bar_addr(&sh.p_full[s]));
             ++done;
         }
-        if (ok && done > 0) {
-            ok = tc::mbar_wait_or_abort(bar_addr(&sh.o_done[s]), (done - 1) & 1, abort_flag);
-            ok = __all_sync(0xffffffffu, ok);
-        }
+        if (ok && done > 0) ok = tc::mbar_wait_or_abort(bar_addr(&sh.o_done[s]), (done - 1) & 1, abort_flag);
+        sh.half[s][half][row] = l;
+        ok = tc::named_barrier_and(bar_id, 256, ok && !*abort_flag);           // also: both halves' sums are there
         if (!ok) *abort_flag = 1;
         tc::fence_after_sync();
+        l += sh.half[s][half ^ 1][row];
         const int64_t out_row = int64_t(head) * p.S + b.D.q0 + token;
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
         const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
         bool fine = ok && l < INFINITY && l >= 0.f;
         if (ok && b.t0[s] < b.t1[s]) {
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = 0; c < D / 64; ++c) {
+                const int col = half * (D / 2) + c * 32;
                 uint32_t o[32];
                 if (done) {
                     tc::tmem_ld_x32(t_o + c * 32, o);
@@ -414,7 +491,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 fine = fine && worst == 0.f;
                 if (valid) {
                     if (gridDim.y == 1) {
-                        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(p.o) + out_row * D + c * 32);
+                        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(p.o) + out_row * D + col);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             dst[i] = make_uint4(pack2<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1])),
@@ -422,20 +499,22 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                                                 pack2<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5])),
                                                 pack2<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7])));
                     } else {
-                        uint4 *dst = reinterpret_cast<uint4 *>(part_o + (int64_t(blockIdx.y) * p.Hq * p.S + out_row) * D + c * 32);
+                        uint4 *dst = reinterpret_cast<uint4 *>(part_o + (int64_t(blockIdx.y) * p.Hq * p.S + out_row) * D + col);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                 }
             }
         }
+        if (valid && !fine) atomicOr(&sh.again[s][row >> 5], 1u << lane);
+        if (valid && half == 0 && gridDim.y == 1) p.lse[out_row] = lse;
+        tc::named_barrier(bar_id, 256);                                        // every part of a row has been written and judged
+        const unsigned again = sh.again[s][row >> 5];
+        const bool redo = again >> lane & 1u;
         if (gridDim.y == 1) {
-            if (valid) p.lse[out_row] = lse;
-            const unsigned again = __ballot_sync(0xffffffffu, valid && !fine);
-            __syncwarp();
-            if (again) redo_rows<T, D>(p, b, again, b.t0[s], row & ~31);
-        } else if (valid) {
-            part_lse[int64_t(blockIdx.y) * p.Hq * p.S + out_row] = fine ? lse : __int_as_float(0x7fc00000);
+            if (again && half == 0) redo_rows<T, D>(p, b, again, b.t0[s], row & ~31);
+        } else if (valid && half == 0) {
+            part_lse[int64_t(blockIdx.y) * p.Hq * p.S + out_row] = redo ? __int_as_float(0x7fc00000) : lse;
         }
         tc::fence_before_sync();
     }
@@ -465,7 +544,6 @@ Shape shape_of(const LocalParams &p)
 
 template <typename T, int D> int launch(const LocalParams &p, int dtype, void *ws, cudaStream_t st)
 {
-    using C = Cfg<D>;
     const Shape sh = shape_of(p);
     CUtensorMap tm_q, tm_k, tm_v;
     if (int rc = local_query_map(&tm_q, p, p.q, p.q_sh, p.q_st, dtype)) return rc;
@@ -473,8 +551,8 @@ template <typename T, int D> int launch(const LocalParams &p, int dtype, void *w
     if (int rc = local_key_map(&tm_v, p, p.v, p.v_sh, p.v_st, dtype)) return rc;
     float *part_lse = static_cast<float *>(ws), *part_o = part_lse + (size_t(sh.parts) * p.Hq * p.S + 31) / 32 * 32;
     const bool bf16 = dtype == FM_BF16;
-    FM_CUDA_OK(func_attr_cached((const void *)local_fwd_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::kSmem));
-    local_fwd_kernel<T, D><<<dim3(unsigned(sh.blocks), unsigned(sh.parts)), kThreads, C::kSmem, st>>>(
+    FM_CUDA_OK(func_attr_cached((const void *)local_fwd_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>()));
+    local_fwd_kernel<T, D><<<dim3(unsigned(sh.blocks), unsigned(sh.parts)), kThreads, smem_bytes<D>(), st>>>(
         p, tm_q, tm_k, tm_v, tc::instr_desc_f16(bf16, ltc::kTile, ltc::kTile), tc::instr_desc_f16(bf16, ltc::kTile, D, false, true), part_o, part_lse);
     FM_LAUNCHED("local_fwd_kernel");
     return sh.parts > 1 ? local_combine(p, dtype, part_o, part_lse, sh.parts, st) : FM_OK;

@@ -21,6 +21,106 @@ __device__ __forceinline__ uint64_t desc_k(uint32_t tile, int ks) { return tc::s
 // MN-major operand of a tile (the contraction runs over its ROWS): K step ks = rows 16 ks ..
 __device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int ks) { return tc::smem_desc_mn_sw128(tile + uint32_t(ks) * 2048u, kBlock); }
 
+// and what a K step adds to the descriptor of step 0
+__host__ __device__ constexpr uint32_t step_k(int ks) { return (uint32_t(ks >> 2) * kBlock + uint32_t(ks & 3) * 32u) >> 4; }
+__host__ __device__ constexpr uint32_t step_mn(int ks) { return uint32_t(ks) * 2048u >> 4; }
+
+// ---- two fp32 numbers an instruction ------------------------------------------------------------------------------------
+// The softmax of a tile is issue-bound unless its arithmetic goes two scores at a time, and bound by the special-function unit
+// (16 exponentials a cycle and SM: 1024 cycles a tile, as long as two of its products) unless some of its exponentials go
+// to the FMA pipe.
+typedef uint64_t f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b)
+{
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 pair(uint32_t a, uint32_t b) { return pair(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ float2 split(f32x2 x)
+{
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c)
+{
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b)
+{
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+__device__ __forceinline__ f32x2 exp2_sfu(f32x2 x)
+{
+    const float2 v = split(x);
+    return pair(fast_exp2(v.x), fast_exp2(v.y));
+}
+
+// 2^x on the FMA pipe, x <= 120: x = n + f with n the nearest whole number (the sum with 1.5 2^23 holds it in its low bits),
+// 2^f by the degree-5 polynomial of least relative error on [-1/2, 1/2] (7e-8; 2.4e-7 with fp32 rounding), n added to the
+// exponent.  x is cut at -126: no exact zeros come out of this one.
+__device__ __forceinline__ f32x2 exp2_fma(f32x2 x)
+{
+    const float2 v = split(x);
+    const f32x2 y = pair(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+    const f32x2 t = add2(y, pair(12582912.f, 12582912.f));
+    const f32x2 f = add2(y, mul2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f)));
+    f32x2 q = fma2(f, pair(1.32917648e-3f, 1.32917648e-3f), pair(9.67562478e-3f, 9.67562478e-3f));
+    q = fma2(q, f, pair(5.55065386e-2f, 5.55065386e-2f));
+    q = fma2(q, f, pair(2.40221202e-1f, 2.40221202e-1f));
+    q = fma2(q, f, pair(6.93147004e-1f, 6.93147004e-1f));
+    q = fma2(q, f, pair(1.f, 1.f));
+    const float2 a = split(q), b = split(t);
+    return pair(__float_as_uint(a.x) + (__float_as_uint(b.x) << 23), __float_as_uint(a.y) + (__float_as_uint(b.y) << 23));
+}
+
+// Exponential of score pair i of a row; MIX: three of eight go to the FMA pipe.
+template <bool MIX> __device__ __forceinline__ f32x2 exp2_pair(f32x2 x, int i)
+{
+    if (MIX && (i & 7) >= 5) return exp2_fma(x);
+    return exp2_sfu(x);
+}
+
+// tanh of a pair, |x| <= 0.7: x + x^3 p(x^2), p of degree 4 with the least error on that range (5e-8 in fp32).
+constexpr float kTanhRange = 0.7f;
+__device__ __forceinline__ f32x2 tanh_small(f32x2 x)
+{
+    const f32x2 u = mul2(x, x);
+    f32x2 q = fma2(u, pair(-5.13866311e-3f, -5.13866311e-3f), pair(2.00919714e-2f, 2.00919714e-2f));
+    q = fma2(q, u, pair(-5.35588600e-2f, -5.35588600e-2f));
+    q = fma2(q, u, pair(1.33291110e-1f, 1.33291110e-1f));
+    q = fma2(q, u, pair(-3.33331913e-1f, -3.33331913e-1f));
+    return fma2(mul2(x, u), q, x);
+}
+// tanh x = 1 - 2 / (1 + e^2x): e^2x = inf gives 1, 0 gives -1
+__device__ __forceinline__ float tanh_any(float x)
+{
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(x * (2.f * kLog2e))));
+    return fmaf(-2.f, r, 1.f);
+}
+
+// A value that is the same in every lane, so that the compiler can see it.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // Blocks of `per` rows, document by document (`KEYS`: of keys, else of queries): which document and which block of it is
 // block number `b`?  Called by one whole warp; .x = document (n_docs: the tail), .y = block; .x = -1: there is no such block.
 template <bool KEYS> __device__ __forceinline__ int2 find_block(const LocalParams &p, int per, int b)

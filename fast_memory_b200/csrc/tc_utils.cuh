@@ -122,6 +122,41 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols)     
 __device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one()
+{
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
+
+// Products issued by a whole converged warp, `go` true in one lane: the instruction alone is predicated, so that descriptors are
+// computed where the compiler can keep them in uniform registers.  (Inside a branch of one thread every descriptor that changes
+// costs moves into uniform registers: ~105 cycles for an instruction with two of them instead of 64.)
+__device__ __forceinline__ void umma_f16_if(bool go, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate)
+{
+    asm volatile("{\n\t.reg .pred p, g;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "setp.ne.b32 g, %6, 0;\n\t"
+                 "@g tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+                 ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(0u), "r"(go ? 1u : 0u) : "memory");
+}
+// the same with A in TMEM: lane = row of A, a 32-bit column holds two consecutive 16-bit elements along K
+__device__ __forceinline__ void umma_f16_ts_if(bool go, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate)
+{
+    asm volatile("{\n\t.reg .pred p, g;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "setp.ne.b32 g, %6, 0;\n\t"
+                 "@g tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+                 ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1u : 0u), "r"(0u), "r"(go ? 1u : 0u) : "memory");
+}
+__device__ __forceinline__ void umma_commit_if(bool go, uint32_t bar)
+{
+    asm volatile("{\n\t.reg .pred g;\n\t"
+                 "setp.ne.b32 g, %1, 0;\n\t"
+                 "@g tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(go ? 1u : 0u) : "memory");
+}
+
 // D[tmem] (+)= A[smem] * B[smem]^T, one thread issues
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, bool accumulate)
 {
@@ -130,15 +165,6 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
                  "setp.ne.b32 p, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
                  ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc), "r"(0u) : "memory");
-}
-// D[tmem] (+)= A[tmem] * B[smem]^T: lane = row of A, a 32-bit column holds two consecutive 16-bit elements along K
-__device__ __forceinline__ void umma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, bool accumulate)
-{
-    uint32_t acc = accumulate ? 1u : 0u;
-    asm volatile("{\n\t.reg .pred p;\n\t"
-                 "setp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-                 ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(acc), "r"(0u) : "memory");
 }
 // arrives on the mbarrier once every MMA issued so far by this thread has completed
 __device__ __forceinline__ void umma_commit(uint32_t bar)
@@ -223,6 +249,17 @@ __device__ __forceinline__ bool named_barrier_and(int id, int count, bool pred)
     asm volatile("{\n\t.reg .pred p, q;\n\t"
                  "setp.ne.b32 p, %3, 0;\n\t"
                  "barrier.cta.red.and.pred q, %1, %2, p;\n\t"
+                 "selp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(out) : "r"(id), "r"(count), "r"(pred ? 1u : 0u) : "memory");
+    return out != 0;
+}
+// The same with OR.
+__device__ __forceinline__ bool named_barrier_or(int id, int count, bool pred)
+{
+    uint32_t out;
+    asm volatile("{\n\t.reg .pred p, q;\n\t"
+                 "setp.ne.b32 p, %3, 0;\n\t"
+                 "barrier.cta.red.or.pred q, %1, %2, p;\n\t"
                  "selp.u32 %0, 1, 0, q;\n\t}"
                  : "=r"(out) : "r"(id), "r"(count), "r"(pred ? 1u : 0u) : "memory");
     return out != 0;

@@ -47,7 +47,7 @@ def _int32(values: Optional[Prefix], dev: torch.device, name: str, count: Option
             raise TypeError(f"{name} must be a 1-d int32 or int64 tensor")
         if values.device != dev:
             raise ValueError(f"{name} is on {values.device}, the tensors are on {dev}")
-        t = values.to(torch.int32).contiguous()
+        t = values if values.dtype is torch.int32 and values.is_contiguous() else values.to(torch.int32).contiguous()
     else:
         t = torch.tensor([int(x) for x in values], dtype=torch.int32, device=dev)
     if count is not None and t.numel() != count:
@@ -98,9 +98,12 @@ def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.devic
     return dev
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(dev: torch.device):
     """Kernels launch on the tensors' device whatever the current one is."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _doc_args(q, k, v, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, prefix):
@@ -111,15 +114,26 @@ def _doc_args(q, k, v, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, pr
         0, 0, 0, 0)
 
 
+def _stream(dev: torch.device) -> int:
+    """Handle of the current stream of ``dev`` (the raw form: a tenth of the time of ``torch.cuda.current_stream``)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _scratch(nbytes: int, dev: torch.device) -> Optional[torch.Tensor]:
+    """A workspace for one call, or none: a captured graph keeps its own, and no other graph or stream writes it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
 def _forward(args: L.LocalAttnArgs, q: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     dev = q.device
-    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
+    o = q.new_empty(q.shape)
+    lse = q.new_empty(q.shape[:2], dtype=torch.float32)
     lib, ref = L.lib(), ctypes.byref(args)
     with _on(dev):
-        # a workspace of its own: a captured graph keeps it, and no other graph or stream writes it
-        ws = torch.empty(lib.fm_local_attn_workspace_bytes(ref), dtype=torch.uint8, device=dev)
-        L.check(lib.fm_local_attn_fwd(ref, o.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), L.stream_ptr(dev)), "fm_local_attn_fwd")
+        nbytes = lib.fm_local_attn_workspace_bytes(ref)
+        ws = _scratch(nbytes, dev)
+        status = lib.fm_local_attn_fwd(ref, o.data_ptr(), lse.data_ptr(), L.ptr(ws), nbytes, _stream(dev))
+    L.check(status, "fm_local_attn_fwd")
     return o, lse
 
 
@@ -133,14 +147,15 @@ def _local_bwd(q, k, v, out, lse, d_out, d_lse, sm_scale, causal, window, softca
     out, lse = out.contiguous(), lse.contiguous()
     d_lse = None if d_lse is None else d_lse.contiguous()
     dev = q.device
-    dq, dk, dv = (torch.empty(t.shape, dtype=q.dtype, device=dev) for t in (q, k, v))
+    dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
     args = _doc_args(q, k, v, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, prefix)
     lib, ref = L.lib(), ctypes.byref(args)
     with _on(dev):
-        ws = torch.empty(lib.fm_local_attn_bwd_workspace_bytes(ref), dtype=torch.uint8, device=dev)
-        L.check(lib.fm_local_attn_bwd(ref, out.data_ptr(), lse.data_ptr(), d_out.data_ptr(), d_out.stride(0), d_out.stride(1),
-                                      L.ptr(d_lse), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), ws.numel(),
-                                      L.stream_ptr(dev)), "fm_local_attn_bwd")
+        nbytes = lib.fm_local_attn_bwd_workspace_bytes(ref)
+        ws = _scratch(nbytes, dev)
+        status = lib.fm_local_attn_bwd(ref, out.data_ptr(), lse.data_ptr(), d_out.data_ptr(), d_out.stride(0), d_out.stride(1),
+                                       L.ptr(d_lse), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), L.ptr(ws), nbytes, _stream(dev))
+    L.check(status, "fm_local_attn_bwd")
     return dq, dk, dv
 
 

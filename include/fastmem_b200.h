@@ -189,7 +189,7 @@ typedef struct {
     int64_t page_table_width, n_pages;
     int32_t page_size, n_seqs;            /* n_seqs: rows of page_table                               */
 } fm_local_attn_args;
-size_t fm_local_attn_workspace_bytes(const fm_local_attn_args *args);
+size_t fm_local_attn_workspace_bytes(const fm_local_attn_args *args);        /* 0: none is needed, pass NULL */
 int fm_local_attn_fwd(const fm_local_attn_args *args, void *o, float *lse, void *workspace, size_t workspace_bytes, fm_stream_t stream);
 
 /* Gradients of fm_local_attn_fwd (documents, not pages): o [n_q_heads, n_q_rows, d] contiguous and lse are the result the
