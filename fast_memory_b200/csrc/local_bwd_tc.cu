@@ -85,14 +85,15 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
 
     if (warp == 0) {
         const int nb = gridDim.x / p.H, h = blockIdx.x / nb;
-        const int2 at = find_block<true>(p, kTile, blockIdx.x % nb);
+        Doc doc;
+        const int index = find_block<true>(p, kTile, blockIdx.x % nb, doc);
         if (lane == 0) {
             sh.h = h;
             sh.n_q = 0;
             sh.j0 = -1;
-            if (at.x >= 0) {
-                sh.D = local_doc<true>(p, at.x);
-                sh.j0 = at.y * kTile;
+            if (index >= 0) {
+                sh.D = doc;
+                sh.j0 = index * kTile;
                 const int last = min(sh.j0 + kTile, sh.D.nk) - 1;
                 int2 run = make_int2(local_query_run(p, sh.D, sh.j0).x, local_query_run(p, sh.D, last).y);
                 if (sh.j0 < sh.D.prefix) run = make_int2(0, sh.D.nq);
@@ -453,14 +454,14 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
 
     if (warp == 0) {
         const int nb = gridDim.x / p.H, h = blockIdx.x / nb;
-        const int2 at = find_block<false>(p, tokens, nb - 1 - int(blockIdx.x % nb));       // (the most keys first)
+        Doc doc;
+        const int index = find_block<false>(p, tokens, nb - 1 - int(blockIdx.x % nb), doc);   // (the most keys first)
         if (lane == 0) {
             sh.h = h;
             sh.t0 = sh.t1 = sh.n_pre = sh.lo = sh.n_k = 0;
-            if (at.x >= 0) {
-                sh.D = local_doc(p, at.x);
-                const Doc &D = sh.D;
-                sh.t0 = at.y * tokens;
+            if (index >= 0) {
+                const Doc &D = sh.D = doc;
+                sh.t0 = index * tokens;
                 sh.t1 = min(sh.t0 + tokens, D.nq);
                 const int lo = local_run(p, D.nk - D.nq + sh.t0, D.nk).x, hi = local_run(p, D.nk - D.nq + sh.t1 - 1, D.nk).y;
                 sh.n_pre = (D.prefix + kTile - 1) / kTile;

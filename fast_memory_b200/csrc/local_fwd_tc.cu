@@ -1,21 +1,26 @@
 // Local attention forward on the 5th-generation tensor cores, 16-bit types, head dim 64 or 128.
 //
 // A CTA owns two query tiles of 128 rows - row = (token, head of the group), so that a tile reads its KV head's keys once for
-// the whole group - and streams the key tiles that either of them sees:
-//     S [128 x 128] = Q K^T        A = Q, B = K, both K-major in shared memory (TMA, 128-byte swizzle); fp32 in TMEM
-//     P = 2^(s - m)                two threads a row: 64 scores in registers, sum l, no shuffles; P goes back to TMEM over S as
+// the whole group - and streams the key tiles that either of them sees, in steps of 64 keys:
+//     S [128 x 64] = Q K^T         A = Q, B = K, both K-major in shared memory (TMA, 128-byte swizzle); fp32 in TMEM
+//     P = 2^(s - m)                thread = row: 64 scores in registers, sum l, no shuffles; P goes back to TMEM over S as
 //                                  packed 16-bit: the A operand of the second product
-//     O [128 x d] += P V           B = V, the same tile layout read MN-major; fp32 in TMEM (S0 S1 O0 O1 = 512 columns)
-// The two tiles take turns: while one's 256 threads do a softmax, the tensor core works for the other.  The reference m is the
-// maximum of the row's first tile and is renewed only when a tile's sum of p exceeds 2^12: the sums are fp32 and P is a
-// floating-point number (fp16 reaches 2^16), so a reference that is too small costs no accuracy.  Most tiles then need no maximum
-// at all (600 of 2300 cycles of a tile's softmax), and O is rescaled in TMEM next to never.
+//     O [128 x d] += P V           B = V, the same tile layout read MN-major; fp32 in TMEM
+// TMEM: two buffers of S for each tile and O of each, 512 columns.  S of step k + 1 is under way while step k is in the softmax,
+// so that neither waits for the other: the special-function unit (16 exponentials a cycle: 1024 cycles for 128 keys of a tile)
+// and the tensor core (1280 cycles; a product with N = 64 and both operands in shared memory takes 48 cycles, not 32) are
+// both busy.  With steps of 128 keys TMEM holds one buffer of S, and a tile's softmax (2000 cycles) and products (1500 with their
+// hand-over) take turns.
+// The reference m is the maximum of the row's first step and is renewed only when a step's sum of p exceeds 2^12: the sums are
+// fp32 and P is a floating-point number (fp16 reaches 2^16), so a reference that is too small costs no accuracy.  Most steps then
+// need no maximum at all, and O is rescaled in TMEM next to never.
 // l sums the unrounded p; P is rounded to the element type because the second product takes 16-bit operands.
 //
-//   warps 0-7, 8-15  softmax and epilogue of tile 0, 1; two threads a row, 64 columns each (a warp reaches its own quarter of
-//                    the TMEM lanes)
-//   warp 16          issues all products
-//   warp 17          TMA: query tiles, then K and V tiles through one ring; a paged tile is one box a page, its addresses looked
+//   warps 0-3, 4-7   softmax and epilogue of tile 0, 1 (a warp reaches its own quarter of the TMEM lanes).  Two threads a row
+//                    would keep the special-function unit 15 % busier, but the barrier and the bookkeeping that they need
+//                    in every step cost more than that
+//   warps 8, 9       issue the products of tile 0, 1
+//   warp 10          TMA: query tiles, then K and V tiles through one ring; a paged tile is one box a page, its addresses looked
 //                    up by the lanes side by side.  Rows behind the document's last key are zeroed in the V tile: they would
 //                    meet P = 0, and 0 * NaN is NaN
 // A hidden key INSIDE the document can still hold a NaN value.  It shows as a result that is not finite; such rows are computed
@@ -31,9 +36,10 @@ namespace {
 
 using namespace ltc;
 
-constexpr int kThreads = 640;
-constexpr int kMmaWarp = 16, kLoadWarp = 17;        // warps 18 and 19 complete the fifth warpgroup: registers are split by warpgroup
-constexpr float kMostSum = 4096.f;                  // sum of a tile's p from which a row's reference is renewed
+constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 10;         // warp 11 completes the third warpgroup: registers are split by warpgroup
+constexpr int kStep = 64;                           // keys of a step: half a key tile
+constexpr float kMostSum = 4096.f;                  // sum of a step's p from which a row's reference is renewed
 
 template <int D> struct Cfg {
     static constexpr uint32_t kTileBytes = uint32_t(D / 64) * kBlock;
@@ -44,35 +50,44 @@ struct Block {
     Doc D;
     int h, tokens;                                  // KV head; tokens of a query tile
     int t0[2], t1[2];                               // tokens of each tile in the document, [t0, t1)
-    int lo[2], hi[2];                               // key tiles of each tile behind the prefix's, [lo, hi)
+    int lo[2], hi[2];                               // steps (of 64 keys) of each tile behind the prefix's, [lo, hi)
+    int pre_steps;                                  // steps of the prefix (seen by both)
     int n_pre, lo0;                                 // key tiles of the prefix; first one behind them that any tile sees
-    int n0, n1;                                     // this CTA's part of the list
+    int n0, n1;                                     // this CTA's part of the list of key tiles
     __device__ __forceinline__ int key_tile(int n) const { return n < n_pre ? n : lo0 + n - n_pre; }
-    __device__ __forceinline__ bool active(int s, int n) const
+};
+
+// Which steps a query tile takes part in, as registers of one role.
+struct Steps {
+    int on, pre, lo, hi, n_pre, lo0;
+    __device__ __forceinline__ Steps(const Block &b, int s)
+        : on(uniform(b.t0[s] < b.t1[s])), pre(uniform(b.pre_steps)), lo(uniform(b.lo[s])), hi(uniform(b.hi[s])), n_pre(uniform(b.n_pre)), lo0(uniform(b.lo0)) {}
+    // step u (0, 1) of tile n of the list, as its number among the document's steps
+    __device__ __forceinline__ int step(int n, int u) const { return 2 * (n < n_pre ? n : lo0 + n - n_pre) + u; }
+    __device__ __forceinline__ bool active(int n, int u) const
     {
-        const int kt = key_tile(n);
-        return t0[s] < t1[s] && (n < n_pre || (kt >= lo[s] && kt < hi[s]));
+        const int e = step(n, u);
+        return on && (e < pre || (e >= lo && e < hi));
     }
 };
 
 template <int D> struct Shared {
     uint64_t q_full[2], full[Cfg<D>::kRing], empty[Cfg<D>::kRing], tail;
-    uint64_t s_full[2], p_full[2], o_done[2], drain;
+    uint64_t s_full[2][2], p_full[2][2], o_done[2][2], drain[2];
     uint32_t tmem_slot;
     int abort;
     Block b;
-    float half[2][2][kTile];                        // per query tile, half and row: what the two threads of a row tell each other
-    unsigned again[2][4];                           // rows whose result is not finite
 };
 template <int D> constexpr uint32_t smem_bytes() { return (2 + Cfg<D>::kRing) * Cfg<D>::kTileBytes + uint32_t(sizeof(Shared<D>)); }
 
-__device__ __forceinline__ void make_block(const LocalParams &p, Block &b, int doc, int index, int h, int part, int parts)
+__device__ __forceinline__ void make_block(const LocalParams &p, Block &b, const Doc &doc, int index, int h, int part, int parts)
 {
-    b.D = local_doc(p, doc);
+    b.D = doc;
     b.h = h;
     b.tokens = kTile / p.G;
     const int shift = b.D.nk - b.D.nq;
     b.n_pre = (b.D.prefix + kTile - 1) / kTile;
+    b.pre_steps = (b.D.prefix + kStep - 1) / kStep;
     int first = 1 << 30, last = 0;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -81,96 +96,73 @@ __device__ __forceinline__ void make_block(const LocalParams &p, Block &b, int d
         b.lo[s] = b.hi[s] = 0;
         if (b.t0[s] < b.t1[s]) {
             const int lo = local_run(p, shift + b.t0[s], b.D.nk).x, hi = local_run(p, shift + b.t1[s] - 1, b.D.nk).y;
-            b.lo[s] = max(lo / kTile, b.n_pre);
-            b.hi[s] = hi > lo ? max((hi + kTile - 1) / kTile, b.lo[s]) : b.lo[s];
-            if (b.hi[s] > b.lo[s]) { first = min(first, b.lo[s]); last = max(last, b.hi[s]); }
+            b.lo[s] = max(lo / kStep, b.pre_steps);
+            b.hi[s] = hi > lo ? max((hi + kStep - 1) / kStep, b.lo[s]) : b.lo[s];
+            if (b.hi[s] > b.lo[s]) { first = min(first, b.lo[s] / 2); last = max(last, (b.hi[s] + 1) / 2); }
         }
     }
+    first = max(first, b.n_pre);                    // (a step that shares its tile with the prefix's last one is in that tile)
     b.lo0 = first;
     const int n = b.n_pre + max(last - first, 0);
     b.n0 = int(int64_t(n) * part / parts);
     b.n1 = int(int64_t(n) * (part + 1) / parts);
 }
 
-// Column c of the tile is a visible key if it lies in [a, b) or below pre.
-__device__ __forceinline__ void mask_scores(uint32_t (&s)[2][32], int a, int b, int pre)
+// Column c is a visible key if it lies in [a, b) or below pre.
+__device__ __forceinline__ void mask_scores(uint32_t (&s)[32], int a, int b, int pre)
 {
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-            const int j = x * 32 + c;
-            if (!((j >= a && j < b) || j < pre)) s[x][c] = 0xff800000u;
-        }
+    for (int c = 0; c < 32; ++c)
+        if (!((c >= a && c < b) || c < pre)) s[c] = 0xff800000u;
 }
 
 // Scores in log2 units after scale, cap and distance (fp: the row's position less the first column's); what is left to multiply
 // is 1.
-__device__ __forceinline__ void shape_scores(const LocalParams &p, uint32_t (&s)[2][32], float slope2, float fp)
+__device__ __forceinline__ void shape_scores(const LocalParams &p, uint32_t (&s)[32], float slope2, float fp)
 {
     if (p.cap > 0.f) {
         float big[2] = {0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < 32; c += 2)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) big[x] = max3(big[x], fabsf(__uint_as_float(s[x][c])), fabsf(__uint_as_float(s[x][c + 1])));
+        for (int c = 0; c < 32; c += 2) big[c >> 1 & 1] = max3(big[c >> 1 & 1], fabsf(__uint_as_float(s[c])), fabsf(__uint_as_float(s[c + 1])));
         const float k = p.scale / p.cap, c2 = p.cap * kLog2e;
         if (__all_sync(0xffffffffu, fmaxf(big[0], big[1]) * fabsf(k) <= kTanhRange)) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int c = 0; c < 32; c += 2) {
-                    const float2 t = split(mul2(tanh_small(mul2(pair(s[x][c], s[x][c + 1]), pair(k, k))), pair(c2, c2)));
-                    s[x][c] = __float_as_uint(t.x);
-                    s[x][c + 1] = __float_as_uint(t.y);
-                }
+            for (int c = 0; c < 32; c += 2) {
+                const float2 t = split(mul2(tanh_small(mul2(pair(s[c], s[c + 1]), pair(k, k))), pair(c2, c2)));
+                s[c] = __float_as_uint(t.x);
+                s[c + 1] = __float_as_uint(t.y);
+            }
         } else {
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int c = 0; c < 32; ++c) s[x][c] = __float_as_uint(c2 * tanh_any(__uint_as_float(s[x][c]) * k));
+            for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(c2 * tanh_any(__uint_as_float(s[c]) * k));
         }
     } else {
-        const f32x2 scale = pair(p.scale * kLog2e, p.scale * kLog2e);
+        const float k = p.scale * kLog2e;
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-                const float2 t = split(mul2(pair(s[x][c], s[x][c + 1]), scale));
-                s[x][c] = __float_as_uint(t.x);
-                s[x][c + 1] = __float_as_uint(t.y);
-            }
+        for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(__uint_as_float(s[c]) * k);
     }
     if (p.slopes) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-                s[x][c] = __float_as_uint(fmaf(-slope2, fabsf(fp - float(x * 32 + c)), __uint_as_float(s[x][c])));
+        for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(fmaf(-slope2, fabsf(fp - float(c)), __uint_as_float(s[c])));
     }
 }
 
-__device__ __forceinline__ float row_max(const uint32_t (&x)[2][32])
+__device__ __forceinline__ float row_max(const uint32_t (&x)[32])
 {
     float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-    for (int c = 0; c < 32; c += 4)
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            mx[y] = max3(mx[y], __uint_as_float(x[y][c]), __uint_as_float(x[y][c + 1]));
-            mx[y + 2] = max3(mx[y + 2], __uint_as_float(x[y][c + 2]), __uint_as_float(x[y][c + 3]));
-        }
+    for (int c = 0; c < 32; c += 2) mx[c >> 1 & 3] = max3(mx[c >> 1 & 3], __uint_as_float(x[c]), __uint_as_float(x[c + 1]));
     return max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
 }
 
 // P = 2^(s mul - sub) of 32 columns as packed 16-bit into TMEM; adds the unrounded p to sum.
-template <typename T, bool MIX> __device__ __forceinline__ void exp_scores(const uint32_t (&x)[32], float mul, float sub, uint32_t t_p, f32x2 (&sum)[2])
+template <typename T> __device__ __forceinline__ void exp_scores(const uint32_t (&x)[32], float mul, float sub, uint32_t t_p, f32x2 (&sum)[2])
 {
     const f32x2 m2 = pair(mul, mul), n2 = pair(-sub, -sub);
     uint32_t pk[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const f32x2 e = exp2_pair<MIX>(fma2(pair(x[2 * i], x[2 * i + 1]), m2, n2), i);
+        const f32x2 e = exp2_pair(fma2(pair(x[2 * i], x[2 * i + 1]), m2, n2));
         sum[i & 1] = add2(sum[i & 1], e);
         const float2 v = split(e);
         pk[i] = pack2<T>(v.x, v.y);
@@ -207,34 +199,36 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
 
     if (warp == 0) {
         // the last blocks of a document have the most keys (causal): they go first
-        const int nb = gridDim.x / p.H, h = blockIdx.x / nb, parts = gridDim.y;
-        const int2 at = find_block<false>(p, 2 * (kTile / p.G), nb - 1 - int(blockIdx.x % nb));
+        const int nb = gridDim.x / p.H, h = blockIdx.x / nb;
+        Doc doc;
+        const int index = find_block<false>(p, 2 * (kTile / p.G), nb - 1 - int(blockIdx.x % nb), doc);
         if (lane == 0) {
-            if (at.x >= 0) make_block(p, sh.b, at.x, at.y, h, blockIdx.y, parts);
-            else { sh.b.t0[0] = sh.b.t1[0] = sh.b.t0[1] = sh.b.t1[1] = 0; sh.b.n0 = sh.b.n1 = 0; }
+            if (index >= 0) make_block(p, sh.b, doc, index, h, blockIdx.y, gridDim.y);
+            else { sh.b = Block{}; }
         }
     }
     if (warp == kMmaWarp) tc::tmem_alloc(tc::smem_addr(&sh.tmem_slot), 512);
     if (warp == kLoadWarp && lane == 0) {
         for (int s = 0; s < 2; ++s) {
             tc::mbar_init(bar_addr(&sh.q_full[s]), 1);
-            tc::mbar_init(bar_addr(&sh.s_full[s]), 1);
-            tc::mbar_init(bar_addr(&sh.p_full[s]), 8);
-            tc::mbar_init(bar_addr(&sh.o_done[s]), 1);
+            tc::mbar_init(bar_addr(&sh.drain[s]), 1);
+            for (int u = 0; u < 2; ++u) {
+                tc::mbar_init(bar_addr(&sh.s_full[s][u]), 1);
+                tc::mbar_init(bar_addr(&sh.p_full[s][u]), 4);
+                tc::mbar_init(bar_addr(&sh.o_done[s][u]), 1);
+            }
         }
         for (int i = 0; i < C::kRing; ++i) {
             tc::mbar_init(bar_addr(&sh.full[i]), 1);
-            tc::mbar_init(bar_addr(&sh.empty[i]), 1);
+            tc::mbar_init(bar_addr(&sh.empty[i]), 2);                          // both product warps let go of it
         }
         tc::mbar_init(bar_addr(&sh.tail), 1);
-        tc::mbar_init(bar_addr(&sh.drain), 1);
         tc::mbar_fence_init();
         sh.abort = 0;
         tc::prefetch_tensormap(&tm_q);
         tc::prefetch_tensormap(&tm_k);
         tc::prefetch_tensormap(&tm_v);
     }
-    if (tid < 8) sh.again[tid >> 2][tid & 3] = 0;
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -242,9 +236,9 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
     const uint32_t tmem = sh.tmem_slot;
     const int n0 = b.n0, n1 = b.n1;
 
-    // 640 threads x 96 registers at launch = 512 x 104 + 128 x 64
-    if (warp >= 16) {
-        tc::set_registers_down<64>();
+    // 384 threads x 168 registers at launch = 256 x 216 + 128 x 72
+    if (warp >= 8) {
+        tc::set_registers_down<72>();
         if (warp == kLoadWarp) {
             // ---- loads ----------------------------------------------------------------------------------------------------
             if (n1 > n0) {
@@ -260,9 +254,19 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 const int box_rows = min(page, kTile);
                 int issued = 0;
                 bool ok = true;
+                // lane x * (d / 64) + c loads column block c of the tile's box x; its page is looked up a tile ahead
+                const int box = lane / (D / 64), col = lane % (D / 64);
+                auto look_up = [&](int n) {
+                    const int j = b.key_tile(n) * kTile + box * box_rows;
+                    if (!p.table || n >= n1 || box >= boxes || j >= b.D.nk) return 0;
+                    return min(max(p.table[int64_t(b.D.seq) * p.table_ld + (j >> p.page_shift)], 0), p.n_pages - 1);
+                };
+                int page_id = look_up(n0);
                 for (int n = n0; n < n1 && ok; ++n) {
                     const int j0 = b.key_tile(n) * kTile, rows = b.D.nk - j0;      // rows of the tile that are keys of the document
                     const int live = rows >= kTile ? boxes : (rows + box_rows - 1) / box_rows;
+                    const int next_id = look_up(n + 1);
+                    const int y = p.table ? (j0 + box * box_rows) & (page - 1) : b.D.k0 + j0, z = p.table ? page_id * p.H + b.h : b.h;
                     for (int kv = 0; kv < 2 && ok; ++kv, ++issued) {
                         const int slot = issued % C::kRing;
                         if (issued >= C::kRing) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((issued / C::kRing) & 1) ^ 1, abort_flag);
@@ -273,25 +277,13 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                         const uint32_t bar = bar_addr(cut ? &sh.tail : &sh.full[slot]);
                         if (lane == 0) tc::mbar_arrive_expect_tx(bar, uint32_t(live) * box_rows * (D * 2));
                         __syncwarp();
-                        for (int i = lane; i < live * (D / 64); i += 32) {
-                            const int x = i / (D / 64), c = i % (D / 64);
-                            int y, z;
-                            if (p.table) {
-                                const int j = j0 + x * box_rows;
-                                z = min(max(p.table[int64_t(b.D.seq) * p.table_ld + (j >> p.page_shift)], 0), p.n_pages - 1) * p.H + b.h;
-                                y = j & (page - 1);
-                            } else {
-                                y = b.D.k0 + j0;
-                                z = b.h;
-                            }
-                            tc::tma_load_3d(dst + c * kBlock + x * box_rows * 128, kv ? &tm_v : &tm_k, c * 64, y, z, bar);
-                        }
+                        if (box < live) tc::tma_load_3d(dst + col * kBlock + box * box_rows * 128, kv ? &tm_v : &tm_k, col * 64, y, z, bar);
                         if (cut) {                                                 // at most once a CTA: the document's last tile
                             ok = tc::mbar_wait_or_abort(bar, 0, abort_flag);
                             ok = __all_sync(0xffffffffu, ok);
                             if (!ok) break;
                             for (int i = rows * 8 + lane; i < kTile * 8; i += 32)
-    #pragma unroll
+#pragma unroll
                                 for (int c = 0; c < D / 64; ++c)
                                     *reinterpret_cast<uint4 *>(smem_dyn + (dst - base) + c * kBlock + i * 16) = make_uint4(0, 0, 0, 0);
                             tc::fence_proxy_async_smem();
@@ -299,6 +291,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                             if (lane == 0) tc::mbar_arrive(bar_addr(&sh.full[slot]));
                         }
                     }
+                    page_id = next_id;
                 }
                 if (!ok) {
                     // unwind: every copy in flight lands before the CTA's shared memory goes away
@@ -308,65 +301,68 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                         if (b.t0[s] < b.t1[s]) tc::mbar_wait(bar_addr(&sh.q_full[s]), 0);
                 }
             }
-        } else if (warp == kMmaWarp) {
-            // ---- products ---------------------------------------------------------------------------------------------
-            const uint32_t tm = uniform(int(tmem));
-            const int m0 = uniform(n0), m1 = uniform(n1), n_pre = uniform(b.n_pre), first = uniform(b.lo0);
-            const int on[2] = {uniform(b.t0[0] < b.t1[0]), uniform(b.t0[1] < b.t1[1])};
-            const int lo[2] = {uniform(b.lo[0]), uniform(b.lo[1])}, hi[2] = {uniform(b.hi[0]), uniform(b.hi[1])};
-            auto active = [&](int s, int n) { const int kt = first + n - n_pre; return on[s] && (n < n_pre || (kt >= lo[s] && kt < hi[s])); };
-            if (m1 > m0) {
-                const bool leader = tc::elect_one();
-                bool ok = true;                                                // (what the leader's waits said; the others follow the same path)
-                int done[2] = {0, 0};                                          // key tiles of each query tile so far
-                auto wait = [&](uint64_t *bar, int parity) { ok = ok && tc::mbar_wait_or_abort(bar_addr(bar), parity, abort_flag); };
-                auto ring_wait = [&](int i) { wait(&sh.full[i % C::kRing], (i / C::kRing) & 1); };
-                auto commit = [&](uint64_t *bar) { tc::umma_commit_if(leader, bar_addr(bar)); };
-                auto scores = [&](int s, int n) {                              // S of query tile s and key tile n
-                    const uint64_t q = desc_k(base + s * C::kTileBytes, 0), k = desc_k(ring0 + ((2 * (n - m0)) % C::kRing) * C::kTileBytes, 0);
+        } else if (warp < kLoadWarp && n1 > n0) {
+            // ---- products of one query tile: S runs two steps ahead of P V -----------------------------------------------------
+            const int s = warp - kMmaWarp, m0 = uniform(n0), m1 = uniform(n1);
+            const uint32_t t_s = uniform(int(tmem)) + s * 128, t_o = uniform(int(tmem)) + 256 + s * 128;
+            const Steps st(b, s);
+            const bool leader = tc::elect_one();
+            bool ok = true;                                                    // (what the leader's waits said; the others follow the same path)
+            auto wait = [&](uint64_t *bar, int parity) { ok = ok && tc::mbar_wait_or_abort(bar_addr(bar), parity, abort_flag); };
+            auto ring_wait = [&](int i) { wait(&sh.full[i % C::kRing], (i / C::kRing) & 1); };
+            auto commit = [&](uint64_t *bar) { tc::umma_commit_if(leader, bar_addr(bar)); };
+            const uint64_t q = desc_k(base + s * C::kTileBytes, 0);
+            int sn = m0, su = 0, ns = 0, done = 0;                             // the step whose S comes next; steps issued, and multiplied with V
+            // S up to two steps ahead, but no further than the tile behind `n`: the ring has to turn.  A key tile that is passed is let go of.
+            auto scores = [&](int n) {
+                while (ns - done < 2 && sn < m1 && sn <= n + 1) {
+                    const int i = 2 * (sn - m0);
+                    if (su == 0) ring_wait(i);
+                    if (st.active(sn, su)) {
+                        const uint64_t k = desc_k(ring0 + (i % C::kRing) * C::kTileBytes, 0) + uint32_t(su * (kStep * 128) >> 4);
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks) tc::umma_f16_if(leader && ok, tm + s * 128, q + step_k(ks), k + step_k(ks), idesc_s, ks > 0);
-                    commit(&sh.s_full[s]);
-                };
-                ring_wait(0);
-                for (int s = 0; s < 2; ++s)
-                    if (on[s]) wait(&sh.q_full[s], 0);
-                for (int s = 0; s < 2; ++s)
-                    if (active(s, m0)) scores(s, m0);
-                commit(&sh.empty[0]);
-                for (int n = m0; n < m1; ++n) {
-                    const int vi = 2 * (n - m0) + 1;
-                    const uint64_t v = desc_mn(ring0 + (vi % C::kRing) * C::kTileBytes, 0);
-                    ring_wait(vi);                                             // both tiles are there long before P is
-                    if (n + 1 < m1) ring_wait(vi + 1);
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        if (active(s, n)) {
-                            wait(&sh.p_full[s], done[s] & 1);
-                            tc::fence_after_sync();
-#pragma unroll
-                            for (int ks = 0; ks < kTile / 16; ++ks)
-                                tc::umma_f16_ts_if(leader && ok, tm + 256 + s * 128, tm + s * 128 + (ks >> 2) * 64 + (ks & 3) * 8, v + step_mn(ks), idesc_o,
-                                                   done[s] > 0 || ks > 0);
-                            ++done[s];
-                            commit(&sh.o_done[s]);
-                        }
-                        if (n + 1 < m1 && active(s, n + 1)) scores(s, n + 1);
+                        for (int ks = 0; ks < D / 16; ++ks) tc::umma_f16_if(leader && ok, t_s + (ns & 1) * kStep, q + step_k(ks), k + step_k(ks), idesc_s, ks > 0);
+                        commit(&sh.s_full[s][ns & 1]);
+                        ++ns;
                     }
-                    commit(&sh.empty[vi % C::kRing]);
-                    if (n + 1 < m1) commit(&sh.empty[(vi + 1) % C::kRing]);
+                    if (su == 1) commit(&sh.empty[i % C::kRing]);
+                    sn += su;
+                    su ^= 1;
                 }
-                if (leader && !ok) *abort_flag = 1;
-                commit(&sh.drain);
-                tc::mbar_wait(bar_addr(&sh.drain), 0);
+            };
+            if (st.on) wait(&sh.q_full[s], 0);
+            for (int n = m0; n < m1; ++n) {
+                const int i = 2 * (n - m0) + 1;
+                scores(n);
+                ring_wait(i);
+                const uint64_t v = desc_mn(ring0 + (i % C::kRing) * C::kTileBytes, 0);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (st.active(n, u)) {
+                        const int buf = done & 1;
+                        wait(&sh.p_full[s][buf], (done >> 1) & 1);
+                        tc::fence_after_sync();
+#pragma unroll
+                        for (int ks = 0; ks < kStep / 16; ++ks)
+                            tc::umma_f16_ts_if(leader && ok, t_o, t_s + buf * kStep + ks * 8, v + step_mn(u * (kStep / 16) + ks), idesc_o,
+                                               done > 0 || ks > 0);
+                        commit(&sh.o_done[s][buf]);
+                        ++done;
+                    }
+                    if (u == 1) commit(&sh.empty[i % C::kRing]);
+                    scores(n);
+                }
             }
+            if (leader && !ok) *abort_flag = 1;
+            commit(&sh.drain[s]);
+            tc::mbar_wait(bar_addr(&sh.drain[s]), 0);
         }
     } else {
-        tc::set_registers_up<104>();
+        tc::set_registers_up<216>();
         // ---- softmax and epilogue ---------------------------------------------------------------------------------------
-        const int s = warp >> 3, half = (warp >> 2) & 1, row = (warp & 3) * 32 + lane, bar_id = 1 + s;
+        const int s = warp >> 2, row = tid & 127;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t t_s = tmem + s * 128 + half * 64 + lanes, t_o = tmem + 256 + s * 128 + half * (D / 2) + lanes;
+        const uint32_t t_s = tmem + s * 128 + lanes, t_o = tmem + 256 + s * 128 + lanes;
         const int token = b.t0[s] + row / p.G, head = b.h * p.G + row % p.G;
         const bool valid = row < b.tokens * p.G && token < b.t1[s];
         const int shift = b.D.nk - b.D.nq, pos = shift + token;
@@ -374,67 +370,59 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         const int safe_hi = local_run(p, shift + b.t0[s], b.D.nk).y;
         const bool shaped = p.cap > 0.f || p.slopes || !(p.scale > 0.f);
         const float mul = shaped ? 1.f : p.scale * kLog2e;
+        const Steps st(b, s);
         float m = -INFINITY, l = 0.f;
         int done = 0;
-        bool ok = true, fresh = true;                                          // fresh: some row has no reference yet
-        for (int n = n0; n < n1; ++n) {
-            if (!b.active(s, n)) continue;
-            const int j0 = b.key_tile(n) * kTile;
-            ok = tc::mbar_wait_or_abort(bar_addr(&sh.s_full[s]), done & 1, abort_flag);
-            ok = tc::named_barrier_and(bar_id, 256, ok);
-            if (!ok) break;
-            tc::fence_after_sync();
-            uint32_t x[2][32];
-            f32x2 sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-            const bool masked = !(j0 + kTile <= b.D.prefix || (j0 >= safe_lo && j0 + kTile <= safe_hi));
-            tc::tmem_ld_x32(t_s, x[0]);
-            tc::tmem_ld_wait(x[0]);
-            tc::tmem_ld_x32(t_s + 32, x[1]);
-            if (!fresh && !masked && !shaped) {
-                // the usual tile: half of the scores arrive under the exponentials of the other half
-                exp_scores<T, true>(x[0], mul, m, t_s, sums);
-                tc::tmem_ld_wait(x[1]);
-                exp_scores<T, true>(x[1], mul, m, t_s + 16, sums);
-            } else {
-                tc::tmem_ld_wait(x[1]);
-                if (shaped) shape_scores(p, x, p.slopes && valid ? p.slopes[head] * kLog2e : 0.f, float(pos - j0 - half * 64));
-                if (masked) {
-                    const int2 run = local_run(p, pos, b.D.nk);
-                    mask_scores(x, run.x - j0 - half * 64, run.y - j0 - half * 64, b.D.prefix - j0 - half * 64);
-                }
-                if (fresh) {
-                    sh.half[s][half][row] = row_max(x) * mul;
-                    tc::named_barrier(bar_id, 256);
-                    if (m == -INFINITY) m = fmaxf(sh.half[s][0][row], sh.half[s][1][row]);
-                }
-                // hidden scores need exact zeros, which the polynomial does not give
-                if (!masked && __all_sync(0xffffffffu, m > -INFINITY)) {
-                    exp_scores<T, true>(x[0], mul, m, t_s, sums);
-                    exp_scores<T, true>(x[1], mul, m, t_s + 16, sums);
+        bool ok = true, fresh = true;                                          // fresh: a row of the warp has no reference yet
+        for (int n = n0; n < n1 && ok; ++n)
+#pragma unroll 1
+            for (int u = 0; u < 2; ++u) {
+                if (!st.active(n, u)) continue;
+                const int j0 = st.step(n, u) * kStep, buf = done & 1;
+                const uint32_t t_p = t_s + buf * kStep;                        // S of this step, then P
+                ok = tc::mbar_wait_or_abort(bar_addr(&sh.s_full[s][buf]), (done >> 1) & 1, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                tc::fence_after_sync();
+                uint32_t x[2][32];
+                f32x2 sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+                tc::tmem_ld_x32(t_p, x[0]);
+                tc::tmem_ld_wait(x[0]);
+                tc::tmem_ld_x32(t_p + 32, x[1]);
+                const bool masked = !(j0 + kStep <= b.D.prefix || (j0 >= safe_lo && j0 + kStep <= safe_hi));
+                if (!fresh && !masked && !shaped) {
+                    // the usual step: half of the scores arrive under the exponentials of the others
+                    exp_scores<T>(x[0], mul, m, t_p, sums);
+                    tc::tmem_ld_wait(x[1]);
+                    exp_scores<T>(x[1], mul, m, t_p + 16, sums);
                 } else {
+                    tc::tmem_ld_wait(x[1]);
+                    if (shaped) {
+                        const float slope2 = p.slopes && valid ? p.slopes[head] * kLog2e : 0.f;
+                        shape_scores(p, x[0], slope2, float(pos - j0));
+                        shape_scores(p, x[1], slope2, float(pos - j0 - 32));
+                    }
+                    if (masked) {
+                        const int2 run = local_run(p, pos, b.D.nk);
+                        mask_scores(x[0], run.x - j0, run.y - j0, b.D.prefix - j0);
+                        mask_scores(x[1], run.x - j0 - 32, run.y - j0 - 32, b.D.prefix - j0 - 32);
+                    }
+                    if (fresh && m == -INFINITY) m = fmaxf(row_max(x[0]), row_max(x[1])) * mul;
+                    fresh = __any_sync(0xffffffffu, m == -INFINITY);
                     const float sub = m == -INFINITY ? 0.f : m;
-                    exp_scores<T, false>(x[0], mul, sub, t_s, sums);
-                    exp_scores<T, false>(x[1], mul, sub, t_s + 16, sums);
+                    exp_scores<T>(x[0], mul, sub, t_p, sums);
+                    exp_scores<T>(x[1], mul, sub, t_p + 16, sums);
                 }
-            }
-            float sum = total(sums);
-            // Rows that have outgrown their reference get a new one; rows that have none yet ask the next tile for it.
-            if (tc::named_barrier_or(bar_id, 256, valid && (sum > kMostSum || m == -INFINITY))) {
-                if (tc::named_barrier_or(bar_id, 256, sum > kMostSum)) {
-                    sh.half[s][half][row] = sum > kMostSum ? 1.f : 0.f;
-                    tc::named_barrier(bar_id, 256);
-                    const bool grow = sh.half[s][0][row] + sh.half[s][1][row] > 0.f;
-                    tc::named_barrier(bar_id, 256);
-                    sh.half[s][half][row] = row_max(x) * mul;
-                    tc::named_barrier(bar_id, 256);
-                    const float top = fmaxf(sh.half[s][0][row], sh.half[s][1][row]), f = grow ? fast_exp2(m - top) : 1.f;
+                float sum = total(sums);
+                const bool grow = sum > kMostSum;
+                if (__any_sync(0xffffffffu, grow)) {                           // rows that have outgrown their reference get a new one
+                    const float top = fmaxf(row_max(x[0]), row_max(x[1])) * mul, f = grow ? fast_exp2(m - top) : 1.f;
                     if (done > 0) {
-                        ok = tc::mbar_wait_or_abort(bar_addr(&sh.o_done[s]), (done - 1) & 1, abort_flag);
-                        ok = tc::named_barrier_and(bar_id, 256, ok);
-                        if (!ok) break;
+                        // every product into O has finished: the next one waits for this step's P
+                        ok = tc::mbar_wait_or_abort(bar_addr(&sh.o_done[s][buf ^ 1]), ((done - 1) >> 1) & 1, abort_flag);
+                        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                         tc::fence_after_sync();
 #pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
+                        for (int c = 0; c < D / 16; ++c) {
                             uint32_t o[16];
                             tc::tmem_ld_x16(t_o + c * 16, o);
                             tc::tmem_ld_wait16(o);
@@ -446,33 +434,29 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                     if (grow) { m = top; l *= f; }
                     const float sub = m == -INFINITY ? 0.f : m;
                     sums[0] = sums[1] = pair(0.f, 0.f);
-                    exp_scores<T, false>(x[0], mul, sub, t_s, sums);
-                    exp_scores<T, false>(x[1], mul, sub, t_s + 16, sums);
+                    exp_scores<T>(x[0], mul, sub, t_p, sums);
+                    exp_scores<T>(x[1], mul, sub, t_p + 16, sums);
                     sum = total(sums);
                 }
-                fresh = tc::named_barrier_or(bar_id, 256, valid && m == -INFINITY);
-            } else fresh = false;
-            l += sum;
-            tc::tmem_st_wait();
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(bar_addr(&sh.p_full[s]));
-            ++done;
-        }
-        if (ok && done > 0) ok = tc::mbar_wait_or_abort(bar_addr(&sh.o_done[s]), (done - 1) & 1, abort_flag);
-        sh.half[s][half][row] = l;
-        ok = tc::named_barrier_and(bar_id, 256, ok && !*abort_flag);           // also: both halves' sums are there
+                l += sum;
+                tc::tmem_st_wait();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(bar_addr(&sh.p_full[s][buf]));
+                ++done;
+            }
+        if (ok && done > 0) ok = tc::mbar_wait_or_abort(bar_addr(&sh.o_done[s][(done - 1) & 1]), ((done - 1) >> 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok && !*abort_flag);
         if (!ok) *abort_flag = 1;
         tc::fence_after_sync();
-        l += sh.half[s][half ^ 1][row];
         const int64_t out_row = int64_t(head) * p.S + b.D.q0 + token;
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
         const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
         bool fine = ok && l < INFINITY && l >= 0.f;
         if (ok && b.t0[s] < b.t1[s]) {
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
-                const int col = half * (D / 2) + c * 32;
+            for (int c = 0; c < D / 32; ++c) {
+                const int col = c * 32;
                 uint32_t o[32];
                 if (done) {
                     tc::tmem_ld_x32(t_o + c * 32, o);
@@ -506,15 +490,13 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 }
             }
         }
-        if (valid && !fine) atomicOr(&sh.again[s][row >> 5], 1u << lane);
-        if (valid && half == 0 && gridDim.y == 1) p.lse[out_row] = lse;
-        tc::named_barrier(bar_id, 256);                                        // every part of a row has been written and judged
-        const unsigned again = sh.again[s][row >> 5];
-        const bool redo = again >> lane & 1u;
+        const unsigned again = __ballot_sync(0xffffffffu, valid && !fine);
         if (gridDim.y == 1) {
-            if (again && half == 0) redo_rows<T, D>(p, b, again, b.t0[s], row & ~31);
-        } else if (valid && half == 0) {
-            part_lse[int64_t(blockIdx.y) * p.Hq * p.S + out_row] = redo ? __int_as_float(0x7fc00000) : lse;
+            if (valid) p.lse[out_row] = lse;
+            __syncwarp();
+            if (again) redo_rows<T, D>(p, b, again, b.t0[s], row & ~31);
+        } else if (valid) {
+            part_lse[int64_t(blockIdx.y) * p.Hq * p.S + out_row] = fine ? lse : __int_as_float(0x7fc00000);
         }
         tc::fence_before_sync();
     }
@@ -553,7 +535,7 @@ template <typename T, int D> int launch(const LocalParams &p, int dtype, void *w
     const bool bf16 = dtype == FM_BF16;
     FM_CUDA_OK(func_attr_cached((const void *)local_fwd_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>()));
     local_fwd_kernel<T, D><<<dim3(unsigned(sh.blocks), unsigned(sh.parts)), kThreads, smem_bytes<D>(), st>>>(
-        p, tm_q, tm_k, tm_v, tc::instr_desc_f16(bf16, ltc::kTile, ltc::kTile), tc::instr_desc_f16(bf16, ltc::kTile, D, false, true), part_o, part_lse);
+        p, tm_q, tm_k, tm_v, tc::instr_desc_f16(bf16, ltc::kTile, kStep), tc::instr_desc_f16(bf16, ltc::kTile, D, false, true), part_o, part_lse);
     FM_LAUNCHED("local_fwd_kernel");
     return sh.parts > 1 ? local_combine(p, dtype, part_o, part_lse, sh.parts, st) : FM_OK;
 }

@@ -136,16 +136,19 @@ template <typename T, int D> struct Rows {
     }
 };
 
-// Which block: document in .x (-1: none), block in .y; by the whole CTA
-template <bool KEYS> __device__ __forceinline__ int2 cta_block(const LocalParams &p, int b)
+// ltc::find_block for the whole CTA
+template <bool KEYS> __device__ __forceinline__ int cta_block(const LocalParams &p, int b, Doc &doc)
 {
-    __shared__ int2 at;
+    __shared__ Doc found;
+    __shared__ int index;
     if (threadIdx.x < 32) {
-        const int2 x = ltc::find_block<KEYS>(p, kB, b);
-        if (threadIdx.x == 0) at = x;
+        Doc d;
+        const int i = ltc::find_block<KEYS>(p, kB, b, d);
+        if (threadIdx.x == 0) { found = d; index = i; }
     }
     __syncthreads();
-    return at;
+    doc = found;
+    return index;
 }
 
 template <typename T, int D> constexpr int fwd_smem() { return (2 * Lay<D>::kTileF + kB * kLdP) * 4; }
@@ -158,11 +161,11 @@ __global__ void __launch_bounds__(kT) local_simt_fwd_kernel(const __grid_constan
     __shared__ int bad[kB];
     constexpr int W = Lay<D>::W, M = Lay<D>::M;
     const int nb = gridDim.x / p.Hq, head = blockIdx.x / nb, h = head / p.G;
-    const int2 at = cta_block<false>(p, nb - 1 - int(blockIdx.x % nb));
-    if (at.x < 0) return;
-    const Doc doc = local_doc(p, at.x);
+    Doc doc;
+    const int index = cta_block<false>(p, nb - 1 - int(blockIdx.x % nb), doc);
+    if (index < 0) return;
     const Rows<T, D> rows{p, doc, h};
-    const int t0 = at.y * kB, t1 = min(t0 + kB, doc.nq), shift = doc.nk - doc.nq;
+    const int t0 = index * kB, t1 = min(t0 + kB, doc.nq), shift = doc.nk - doc.nq;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const float slope = p.slopes ? p.slopes[head] : 0.f;
     const T *qb = static_cast<const T *>(p.q) + int64_t(head) * p.q_sh;
@@ -268,11 +271,11 @@ __global__ void __launch_bounds__(kT) local_simt_dq_kernel(const __grid_constant
     __shared__ int bad[kB];
     constexpr int W = Lay<D>::W, M = Lay<D>::M;
     const int nb = gridDim.x / p.Hq, head = blockIdx.x / nb, h = head / p.G;
-    const int2 at = cta_block<false>(p, nb - 1 - int(blockIdx.x % nb));
-    if (at.x < 0) return;
-    const Doc doc = local_doc(p, at.x);
+    Doc doc;
+    const int index = cta_block<false>(p, nb - 1 - int(blockIdx.x % nb), doc);
+    if (index < 0) return;
     const Rows<T, D> rows{p, doc, h};
-    const int t0 = at.y * kB, t1 = min(t0 + kB, doc.nq), shift = doc.nk - doc.nq;
+    const int t0 = index * kB, t1 = min(t0 + kB, doc.nq), shift = doc.nk - doc.nq;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const float slope = p.slopes ? p.slopes[head] : 0.f;
     const T *qb = static_cast<const T *>(p.q) + int64_t(head) * p.q_sh, *db = static_cast<const T *>(g.dout) + int64_t(head) * g.do_sh;
@@ -351,11 +354,11 @@ __global__ void __launch_bounds__(kT) local_simt_dkv_kernel(const __grid_constan
     __shared__ int bad[kB];
     constexpr int W = Lay<D>::W, M = Lay<D>::M;
     const int nb = gridDim.x / p.H, h = blockIdx.x / nb;
-    const int2 at = cta_block<true>(p, blockIdx.x % nb);
-    if (at.x < 0) return;
-    const Doc doc = local_doc<true>(p, at.x);
+    Doc doc;
+    const int index = cta_block<true>(p, blockIdx.x % nb, doc);
+    if (index < 0) return;
     const Rows<T, D> rows{p, doc, h};
-    const int j0 = at.y * kB, j1 = min(j0 + kB, doc.nk), shift = doc.nk - doc.nq;
+    const int j0 = index * kB, j1 = min(j0 + kB, doc.nk), shift = doc.nk - doc.nq;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     load_tile<T, D>(K, [&](int r) { return rows.key(p.k, p.k_sh, p.k_st, j0 + r); });
     load_tile<T, D>(V, [&](int r) { return rows.key(p.v, p.v_sh, p.v_st, j0 + r); });

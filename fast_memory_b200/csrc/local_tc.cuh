@@ -26,9 +26,9 @@ __host__ __device__ constexpr uint32_t step_k(int ks) { return (uint32_t(ks >> 2
 __host__ __device__ constexpr uint32_t step_mn(int ks) { return uint32_t(ks) * 2048u >> 4; }
 
 // ---- two fp32 numbers an instruction ------------------------------------------------------------------------------------
-// The softmax of a tile is issue-bound unless its arithmetic goes two scores at a time, and bound by the special-function unit
-// (16 exponentials a cycle and SM: 1024 cycles a tile, as long as two of its products) unless some of its exponentials go
-// to the FMA pipe.
+// A pair takes the FMA pipe as long as two single operations, but one issue slot.  (Moving part of the exponentials from the
+// special-function unit, 16 a cycle and SM, to a polynomial on the FMA pipe was measured and made every kernel here slower: a
+// pair costs 27 cycles of a scheduler's pipe that way, 16 on the special-function unit.)
 typedef uint64_t f32x2;
 __device__ __forceinline__ f32x2 pair(float a, float b)
 {
@@ -68,35 +68,10 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return r;
 }
 
-__device__ __forceinline__ f32x2 exp2_sfu(f32x2 x)
+__device__ __forceinline__ f32x2 exp2_pair(f32x2 x)
 {
     const float2 v = split(x);
     return pair(fast_exp2(v.x), fast_exp2(v.y));
-}
-
-// 2^x on the FMA pipe, x <= 120: x = n + f with n the nearest whole number (the sum with 1.5 2^23 holds it in its low bits),
-// 2^f by the degree-5 polynomial of least relative error on [-1/2, 1/2] (7e-8; 2.4e-7 with fp32 rounding), n added to the
-// exponent.  x is cut at -126: no exact zeros come out of this one.
-__device__ __forceinline__ f32x2 exp2_fma(f32x2 x)
-{
-    const float2 v = split(x);
-    const f32x2 y = pair(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
-    const f32x2 t = add2(y, pair(12582912.f, 12582912.f));
-    const f32x2 f = add2(y, mul2(add2(t, pair(-12582912.f, -12582912.f)), pair(-1.f, -1.f)));
-    f32x2 q = fma2(f, pair(1.32917648e-3f, 1.32917648e-3f), pair(9.67562478e-3f, 9.67562478e-3f));
-    q = fma2(q, f, pair(5.55065386e-2f, 5.55065386e-2f));
-    q = fma2(q, f, pair(2.40221202e-1f, 2.40221202e-1f));
-    q = fma2(q, f, pair(6.93147004e-1f, 6.93147004e-1f));
-    q = fma2(q, f, pair(1.f, 1.f));
-    const float2 a = split(q), b = split(t);
-    return pair(__float_as_uint(a.x) + (__float_as_uint(b.x) << 23), __float_as_uint(a.y) + (__float_as_uint(b.y) << 23));
-}
-
-// Exponential of score pair i of a row; MIX: three of eight go to the FMA pipe.
-template <bool MIX> __device__ __forceinline__ f32x2 exp2_pair(f32x2 x, int i)
-{
-    if (MIX && (i & 7) >= 5) return exp2_fma(x);
-    return exp2_sfu(x);
 }
 
 // tanh of a pair, |x| <= 0.7: x + x^3 p(x^2), p of degree 4 with the least error on that range (5e-8 in fp32).
@@ -121,19 +96,17 @@ __device__ __forceinline__ float tanh_any(float x)
 // A value that is the same in every lane, so that the compiler can see it.
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
-// Blocks of `per` rows, document by document (`KEYS`: of keys, else of queries): which document and which block of it is
-// block number `b`?  Called by one whole warp; .x = document (n_docs: the tail), .y = block; .x = -1: there is no such block.
-template <bool KEYS> __device__ __forceinline__ int2 find_block(const LocalParams &p, int per, int b)
+// Blocks of `per` rows, document by document (`KEYS`: of keys, else of queries): the document of block number `b` and which of its
+// blocks that is (-1: there is no such block).  Called by one whole warp; every lane gets the answer.
+template <bool KEYS> __device__ __forceinline__ int find_block(const LocalParams &p, int per, int b, Doc &doc)
 {
     const int lane = threadIdx.x & 31;
     int before = 0;
     for (int t0 = 0; t0 <= p.n_docs; t0 += 32) {
         const int t = t0 + lane;
-        int n = 0;
-        if (t <= p.n_docs) {
-            const Doc D = local_doc<KEYS>(p, t);
-            n = ((KEYS ? D.nk : D.nq) + per - 1) / per;
-        }
+        Doc D = {};
+        if (t <= p.n_docs) D = local_doc<KEYS>(p, t);
+        const int n = ((KEYS ? D.nk : D.nq) + per - 1) / per;
         int s = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -142,14 +115,19 @@ template <bool KEYS> __device__ __forceinline__ int2 find_block(const LocalParam
         }
         const int total = __shfl_sync(0xffffffffu, s, 31);
         if (b < before + total) {
-            const unsigned m = __ballot_sync(0xffffffffu, b < before + s);
-            const int l = __ffs(m) - 1;
-            const int first = before + __shfl_sync(0xffffffffu, s - n, l);
-            return make_int2(t0 + l, b - first);
+            const int l = __ffs(__ballot_sync(0xffffffffu, b < before + s)) - 1;
+            doc.q0 = __shfl_sync(0xffffffffu, D.q0, l);
+            doc.nq = __shfl_sync(0xffffffffu, D.nq, l);
+            doc.k0 = __shfl_sync(0xffffffffu, D.k0, l);
+            doc.nk = __shfl_sync(0xffffffffu, D.nk, l);
+            doc.prefix = __shfl_sync(0xffffffffu, D.prefix, l);
+            doc.seq = __shfl_sync(0xffffffffu, D.seq, l);
+            return b - before - __shfl_sync(0xffffffffu, s - n, l);
         }
         before += total;
     }
-    return make_int2(-1, 0);
+    doc = Doc{};
+    return -1;
 }
 
 }  // namespace ltc
