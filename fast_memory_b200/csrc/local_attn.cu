@@ -55,17 +55,27 @@ __global__ void __launch_bounds__(kRowThreads) local_combine_kernel(const __grid
     if (lane == 0) p.lse[row] = total > 0.f ? m + logf(total) : -INFINITY;
 }
 
-// delta[row] = dO . O - d_lse
+// delta[row] = dO . O - d_lse.  16 bytes a lane, as many lanes a row as that takes; bound by HBM.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads) local_delta_kernel(LocalParams p, BwdParams g, const T *o, const float *d_lse, float *delta)
 {
-    const int64_t w = (int64_t(blockIdx.x) * kRowThreads + threadIdx.x) >> 5;
-    if (w >= int64_t(p.Hq) * p.S) return;
-    RowRegs<T, D> a, b;
-    a.load(o + w * D);
-    b.load(static_cast<const T *>(g.dout) + (w / p.S) * g.do_sh + (w % p.S) * g.do_st);
-    const float x = a.dot(b);
-    if ((threadIdx.x & 31) == 0) delta[w] = x - (d_lse ? d_lse[w] : 0.f);
+    constexpr int E = 16 / sizeof(T), L = D / E < 32 ? D / E : 32;             // elements a load, lanes a row
+    const int64_t w = (int64_t(blockIdx.x) * kRowThreads + threadIdx.x) / L;
+    const int lane = threadIdx.x % L;
+    float x = 0.f;
+    if (w < int64_t(p.Hq) * p.S) {
+        const T *a = o + w * D, *b = static_cast<const T *>(g.dout) + (w / p.S) * g.do_sh + (w % p.S) * g.do_st;
+#pragma unroll
+        for (int c = lane * E; c < D; c += L * E) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(a + c), v = *reinterpret_cast<const uint4 *>(b + c);
+            const T *s = reinterpret_cast<const T *>(&u), *t = reinterpret_cast<const T *>(&v);
+#pragma unroll
+            for (int i = 0; i < E; ++i) x = fmaf(Elem<T>::to_f32(s[i]), Elem<T>::to_f32(t[i]), x);
+        }
+    }
+#pragma unroll
+    for (int i = L / 2; i; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
+    if (lane == 0 && w < int64_t(p.Hq) * p.S) delta[w] = x - (d_lse ? d_lse[w] : 0.f);
 }
 
 template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) local_rows_dq_kernel(LocalParams p, BwdParams g)
@@ -247,7 +257,8 @@ int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *l
     if (p.S > 0) {
         const int rc = with_type(a->dtype, p.d, [&](auto t, auto dim) -> int {
             using T = decltype(t);
-            local_delta_kernel<T, decltype(dim)::value><<<row_grid(int64_t(p.Hq) * p.S), kRowThreads, 0, st>>>(p, g, static_cast<const T *>(o), d_lse, delta);
+            constexpr int lanes = decltype(dim)::value * sizeof(T) / 16;
+            local_delta_kernel<T, decltype(dim)::value><<<unsigned(ceil_div(int64_t(p.Hq) * p.S * std::min(lanes, 32), kRowThreads)), kRowThreads, 0, st>>>(p, g, static_cast<const T *>(o), d_lse, delta);
             FM_LAUNCHED("local_delta_kernel");
             return FM_OK;
         });

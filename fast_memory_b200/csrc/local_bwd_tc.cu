@@ -21,6 +21,8 @@
 // are all rows of a CTA whose pipeline wait gave up.
 #include "local_tc.cuh"
 
+#include <type_traits>
+
 namespace fm {
 
 namespace {
@@ -33,19 +35,6 @@ constexpr int kMmaWarp = 8, kLoadWarp = 9, kStatWarp = 10;
 template <int D> struct Bytes {
     static constexpr uint32_t kTileB = uint32_t(D / 64) * kBlock;
 };
-
-// ---- one pair's exponent ------------------------------------------------------------------------------------------------
-// From the product: x = score in log2 units, dcap = derivative of the cap.
-__device__ __forceinline__ float shape_one(const LocalParams &p, float qk, float k1, float c2, float &dcap)
-{
-    // cap: t = tanh(s / cap) = 1 - 2 / (1 + e^2x), k1 = 2 scale / cap log2 e, c2 = cap log2 e
-    const float e = fast_exp2(qk * k1);
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    const float t = fmaf(-2.f, r, 1.f);
-    dcap = fmaf(-t, t, 1.f);
-    return t * c2;
-}
 
 // ======================================================= dK, dV ============================================================
 template <int D> struct DkvCfg {
@@ -62,16 +51,16 @@ template <int DIM> struct DkvShared {
     int abort;
     int h, j0, q_lo, n_q;                                        // head, first key, first query tile, query tiles
     Doc D;
-    alignas(16) float lse2[2][kTile], delta[2][kTile];
-    alignas(16) float slope2[kTile];
-    alignas(16) int token[kTile];                                // of a column, from the tile's first
+    alignas(16) float lse2[2][kTile], delta[2][kTile];           // both negated
+    alignas(16) float slope2[kTile], place[kTile];               // negated slope; token of a column, from the tile's first
+    alignas(16) int token[kTile];
 };
 
-template <typename T, int DIM>
+template <typename T, int DIM, bool CAP, bool SLOPES>
 __global__ void __launch_bounds__(kThreads, 1)
 local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ BwdParams g, const __grid_constant__ CUtensorMap tm_q,
                  const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                 uint32_t idesc_s, uint32_t idesc_o)
+                 const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv, uint32_t idesc_s, uint32_t idesc_o)
 {
     extern __shared__ unsigned char smem_dyn[];
     __shared__ __align__(16) DkvShared<DIM> sh;
@@ -128,6 +117,7 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
     }
     if (tid < kTile) {
         sh.token[tid] = tid / p.G;
+        sh.place[tid] = float(tid / p.G);
         sh.slope2[tid] = 0.f;
     }
     // rows that no load writes: a group that does not divide the tile
@@ -203,9 +193,9 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                         lse = g.lse[int64_t(head) * p.S + D.q0 + token];
                         delta = g.delta[int64_t(head) * p.S + D.q0 + token];
                     }
-                    sh.lse2[buf][r] = lse == -INFINITY ? INFINITY : lse * kLog2e;          // no such row, or one that sees nothing: P = 0
-                    sh.delta[buf][r] = delta;
-                    if (i == 0 && p.slopes && r < rows) sh.slope2[r] = p.slopes[head] * kLog2e;
+                    sh.lse2[buf][r] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;          // no such row, or one that sees nothing: P = 0
+                    sh.delta[buf][r] = -delta;
+                    if (i == 0 && p.slopes && r < rows) sh.slope2[r] = -p.slopes[head] * kLog2e;
                 }
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(bar_addr(&sh.stat_full[buf]));
@@ -263,16 +253,19 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
             if (valid) run = local_query_run(p, D, j);
             all = make_int2(local_query_run(p, D, last).x, local_query_run(p, D, max(j0, min(D.prefix, last))).y);
         }
-        const float scale2 = p.scale * kLog2e, k1 = p.cap > 0.f ? 2.f * kLog2e * p.scale / p.cap : 0.f, c2 = p.cap * kLog2e;
+        const f32x2 scale2 = pair(p.scale * kLog2e, p.scale * kLog2e), c2 = pair(p.cap * kLog2e, p.cap * kLog2e);
+        const f32x2 minus = pair(-1.f, -1.f), one = pair(1.f, 1.f);
+        const float kc = p.cap > 0.f ? p.scale / p.cap : 0.f;
         bool ok = true;
         for (int i = 0; i < n_q; ++i) {
             const int buf = i & 1, t0 = (q_lo + i) * tokens;
+            const f32x2 dist0 = pair(float(D.nk - D.nq + t0 - j), float(D.nk - D.nq + t0 - j));
             const bool masked = !(all.x <= t0 && min(t0 + tokens, D.nq) <= all.y);
             ok = tc::mbar_wait_or_abort(bar_addr(&sh.stat_full[buf]), (i >> 1) & 1, abort_flag) &&
                  tc::mbar_wait_or_abort(bar_addr(&sh.s_full), i & 1, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after_sync();
-            float pr[64];
+            f32x2 pr[32];                                        // P, times the derivative of the cap
             unsigned seen[2] = {0xffffffffu, 0xffffffffu};
             if (masked) {
 #pragma unroll
@@ -286,49 +279,37 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                     seen[x] = m;
                 }
             }
+            auto weights = [&](auto with_mask) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                uint32_t s[32];
-                tc::tmem_ld_x32(t_s + x * 32, s);
-                tc::tmem_ld_wait(s);
-                const float *lse2 = &sh.lse2[buf][half * 64 + x * 32];
-                if (p.cap > 0.f || p.slopes) {
-                    const float dist0 = float(D.nk - D.nq + t0 - j);
-                    uint32_t pk[16];
+                for (int x = 0; x < 2; ++x) {
+                    uint32_t s[32], pk[16];
+                    tc::tmem_ld_x32(t_s + x * 32, s);
+                    tc::tmem_ld_wait(s);
+                    const int col0 = half * 64 + x * 32;
+                    const ulonglong2 *lse2 = reinterpret_cast<const ulonglong2 *>(&sh.lse2[buf][col0]);
+                    f32x2 t[16];
+                    if constexpr (CAP) cap_scores(t, s, kc, valid);
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        float w[2], dcap[2] = {1.f, 1.f};
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const int col = half * 64 + x * 32 + c + y;
-                            float b = __uint_as_float(s[c + y]);
-                            b = p.cap > 0.f ? shape_one(p, b, k1, c2, dcap[y]) : b * scale2;
-                            b = fmaf(-sh.slope2[col], fabsf(dist0 + float(sh.token[col])), b);
-                            w[y] = (seen[x] >> (c + y) & 1u) ? fast_exp2(b - lse2[c + y]) : 0.f;
-                            pr[x * 32 + c + y] = w[y] * dcap[y];
+                    for (int c = 0; c < 16; ++c) {
+                        const f32x2 n = (c & 1) ? lse2[c >> 1].y : lse2[c >> 1].x;
+                        f32x2 e = CAP ? fma2(t[c], c2, n) : fma2(pair(s[2 * c], s[2 * c + 1]), scale2, n);
+                        if constexpr (SLOPES) {
+                            const float2 d = split(add2(dist0, *reinterpret_cast<const f32x2 *>(&sh.place[col0 + 2 * c])));
+                            e = fma2(*reinterpret_cast<const f32x2 *>(&sh.slope2[col0 + 2 * c]), pair(fabsf(d.x), fabsf(d.y)), e);
                         }
-                        pk[c >> 1] = pack2<T>(w[0], w[1]);
+                        float2 w = split(exp2_pair(e));
+                        if constexpr (decltype(with_mask)::value) {
+                            w.x = (seen[x] >> (2 * c) & 1u) ? w.x : 0.f;
+                            w.y = (seen[x] >> (2 * c + 1) & 1u) ? w.y : 0.f;
+                        }
+                        pk[c] = pack2<T>(w.x, w.y);
+                        pr[x * 16 + c] = CAP ? mul2(pair(w.x, w.y), fma2(mul2(t[c], minus), t[c], one)) : pair(w.x, w.y);
                     }
-                    tc::tmem_st_x16(t_s + x * 16, pk);
-                } else {
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
-                        const float4 L = *reinterpret_cast<const float4 *>(lse2 + c);
-                        pr[x * 32 + c] = fast_exp2(fmaf(__uint_as_float(s[c]), scale2, -L.x));
-                        pr[x * 32 + c + 1] = fast_exp2(fmaf(__uint_as_float(s[c + 1]), scale2, -L.y));
-                        pr[x * 32 + c + 2] = fast_exp2(fmaf(__uint_as_float(s[c + 2]), scale2, -L.z));
-                        pr[x * 32 + c + 3] = fast_exp2(fmaf(__uint_as_float(s[c + 3]), scale2, -L.w));
-                    }
-                    if (masked) {
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) pr[x * 32 + c] = (seen[x] >> c & 1u) ? pr[x * 32 + c] : 0.f;
-                    }
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) pk[c] = pack2<T>(pr[x * 32 + 2 * c], pr[x * 32 + 2 * c + 1]);
                     tc::tmem_st_x16(t_s + x * 16, pk);
                 }
-            }
+            };
+            if (masked) weights(std::true_type{});
+            else weights(std::false_type{});
             tc::tmem_st_wait();
             tc::fence_before_sync();
             __syncwarp();
@@ -336,28 +317,28 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
             ok = tc::mbar_wait_or_abort(bar_addr(&sh.dp_full), i & 1, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after_sync();
+            auto gradients = [&](auto with_mask) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                uint32_t s[32], pk[16];
-                tc::tmem_ld_x32(t_dp + x * 32, s);
-                tc::tmem_ld_wait(s);
-                const float *delta = &sh.delta[buf][half * 64 + x * 32];
+                for (int x = 0; x < 2; ++x) {
+                    uint32_t s[32], pk[16];
+                    tc::tmem_ld_x32(t_dp + x * 32, s);
+                    tc::tmem_ld_wait(s);
+                    const ulonglong2 *delta = reinterpret_cast<const ulonglong2 *>(&sh.delta[buf][half * 64 + x * 32]);
 #pragma unroll
-                for (int c = 0; c < 32; c += 4) {
-                    const float4 dl = *reinterpret_cast<const float4 *>(delta + c);
-                    s[c] = __float_as_uint(pr[x * 32 + c] * (__uint_as_float(s[c]) - dl.x));
-                    s[c + 1] = __float_as_uint(pr[x * 32 + c + 1] * (__uint_as_float(s[c + 1]) - dl.y));
-                    s[c + 2] = __float_as_uint(pr[x * 32 + c + 2] * (__uint_as_float(s[c + 2]) - dl.z));
-                    s[c + 3] = __float_as_uint(pr[x * 32 + c + 3] * (__uint_as_float(s[c + 3]) - dl.w));
+                    for (int c = 0; c < 16; ++c) {
+                        const f32x2 n = (c & 1) ? delta[c >> 1].y : delta[c >> 1].x;
+                        float2 w = split(mul2(pr[x * 16 + c], add2(pair(s[2 * c], s[2 * c + 1]), n)));
+                        if constexpr (decltype(with_mask)::value) {          // P = 0 is not enough: dP may be NaN there
+                            w.x = (seen[x] >> (2 * c) & 1u) ? w.x : 0.f;
+                            w.y = (seen[x] >> (2 * c + 1) & 1u) ? w.y : 0.f;
+                        }
+                        pk[c] = pack2<T>(w.x, w.y);
+                    }
+                    tc::tmem_st_x16(t_dp + x * 16, pk);
                 }
-                if (masked) {
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) s[c] = (seen[x] >> c & 1u) ? s[c] : 0u;
-                }
-#pragma unroll
-                for (int c = 0; c < 16; ++c) pk[c] = pack2<T>(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
-                tc::tmem_st_x16(t_dp + x * 16, pk);
-            }
+            };
+            if (masked) gradients(std::true_type{});
+            else gradients(std::false_type{});
             tc::tmem_st_wait();
             tc::fence_before_sync();
             __syncwarp();
@@ -370,14 +351,15 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
             ok = tc::mbar_wait_or_abort(bar_addr(&sh.drain), 0, abort_flag);
             ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
         }
-        ok = __all_sync(0xffffffffu, ok);
+        ok = tc::named_barrier_and(1, 256, ok);                                // all warps go on together
         if (!ok) *abort_flag = 1;
         tc::fence_after_sync();
-        // first warpgroup: dV, second: dK
+        // first warpgroup: dV, second: dK; a whole tile goes out through the shared memory of K or V, which no product reads any more
         bool fine = ok;
         const float f = half ? p.scale : 1.f;
-        T *out = static_cast<T *>(half ? g.dk : g.dv) + (int64_t(h) * p.N + D.k0 + j) * DIM;
+        const bool whole = ok && j0 >= 0 && j0 + kTile <= D.nk;
         if (ok && j0 >= 0) {
+            T *out = valid ? static_cast<T *>(half ? g.dk : g.dv) + (int64_t(h) * p.N + D.k0 + j) * DIM : nullptr;
 #pragma unroll
             for (int c = 0; c < DIM / 32; ++c) {
                 uint32_t o[32];
@@ -388,27 +370,23 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0;
                 }
-                float worst = 0.f;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float x = __uint_as_float(o[i]) * f;
-                    o[i] = __float_as_uint(x);
-                    worst = fmaf(x, 0.f, worst);
-                }
-                fine = fine && worst == 0.f;
-                if (valid) {
-                    uint4 *dst = reinterpret_cast<uint4 *>(out + c * 32);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        dst[i] = make_uint4(pack2<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1])),
-                                            pack2<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3])),
-                                            pack2<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5])),
-                                            pack2<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7])));
-                }
+                const bool good = put_row<T>(o, f, whole ? base_ptr + half * C::kTileB : nullptr, out, row, c * 32);
+                fine = fine && good;
             }
         }
-        unsigned again = __ballot_sync(0xffffffffu, valid && !fine);
-        tc::named_barrier(1, 256);                                             // a row's dV and dK have been written before either is redone
+        if (whole) tc::fence_proxy_async_smem();
+        const bool any = tc::named_barrier_or(1, 256, valid && !fine);         // (both warpgroups redo a row together)
+        if (whole && row == 0) {
+            for (int c = 0; c < DIM / 64; ++c) tc::tma_store_3d(half ? &tm_dk : &tm_dv, c * 64, D.k0 + j0, h, base + half * C::kTileB + c * kBlock);
+            tc::tma_store_commit();
+            if (any) tc::tma_store_wait_all();
+            else tc::tma_store_wait_read();
+        }
+        unsigned again = 0;
+        if (any) {
+            tc::named_barrier(1, 256);
+            again = __ballot_sync(0xffffffffu, valid && !fine);
+        }
         while (again) {
             const int r = (row & ~31) + __ffs(again) - 1;
             again &= again - 1;
@@ -436,11 +414,11 @@ template <int DIM> struct DqShared {
     Doc D;
 };
 
-template <typename T, int DIM>
+template <typename T, int DIM, bool CAP, bool SLOPES>
 __global__ void __launch_bounds__(kThreads, 1)
 local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ BwdParams g, const __grid_constant__ CUtensorMap tm_q,
                 const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                uint32_t idesc_s, uint32_t idesc_o)
+                const __grid_constant__ CUtensorMap tm_dq, uint32_t idesc_s, uint32_t idesc_o)
 {
     extern __shared__ unsigned char smem_dyn[];
     __shared__ __align__(16) DqShared<DIM> sh;
@@ -590,7 +568,10 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
         const int2 run = valid ? local_run(p, pos, D.nk) : make_int2(0, 0);
         const int pre = valid ? D.prefix : 0;
         const int safe_lo = p.window ? shift + t1 - p.window : 0, safe_hi = n_k > 0 ? local_run(p, shift + t0, D.nk).y : 0;
-        const float scale2 = p.scale * kLog2e, k1 = p.cap > 0.f ? 2.f * kLog2e * p.scale / p.cap : 0.f, c2 = p.cap * kLog2e;
+        const f32x2 scale2 = pair(p.scale * kLog2e, p.scale * kLog2e), c2 = pair(p.cap * kLog2e, p.cap * kLog2e);
+        const f32x2 minus = pair(-1.f, -1.f), one = pair(1.f, 1.f);
+        const f32x2 nlse = pair(-lse2, -lse2), ndelta = pair(-delta, -delta), nslope = pair(-slope2, -slope2);
+        const float kc = p.cap > 0.f ? p.scale / p.cap : 0.f;
         bool ok = true;
         for (int n = 0; n < n_k; ++n) {
             const int j0 = key_tile(n) * kTile, b = n & 1, col0 = j0 + half * 64;
@@ -599,46 +580,50 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
             ok = tc::mbar_wait_or_abort(bar_addr(&sh.s_full[b]), (n >> 1) & 1, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after_sync();
-            float pr[64];
+            f32x2 pr[32];                                        // P, times the derivative of the cap
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 uint32_t s[32];
                 tc::tmem_ld_x32(t_s + x * 32, s);
                 tc::tmem_ld_wait(s);
-                if (p.cap > 0.f || p.slopes) {
-                    const float dist0 = float(pos - col0);
+                f32x2 t[16];
+                if constexpr (CAP) cap_scores(t, s, kc, valid);
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        float dcap = 1.f, y = __uint_as_float(s[c]);
-                        y = p.cap > 0.f ? shape_one(p, y, k1, c2, dcap) : y * scale2;
-                        y = fmaf(-slope2, fabsf(dist0 - float(x * 32 + c)), y);
-                        pr[x * 32 + c] = fast_exp2(y - lse2) * dcap;
+                for (int c = 0; c < 16; ++c) {
+                    f32x2 e = CAP ? fma2(t[c], c2, nlse) : fma2(pair(s[2 * c], s[2 * c + 1]), scale2, nlse);
+                    if constexpr (SLOPES) {
+                        const float d = float(pos - col0 - x * 32 - 2 * c);
+                        e = fma2(nslope, pair(fabsf(d), fabsf(d - 1.f)), e);
                     }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) pr[x * 32 + c] = fast_exp2(fmaf(__uint_as_float(s[c]), scale2, -lse2));
+                    e = exp2_pair(e);
+                    pr[x * 16 + c] = CAP ? mul2(e, fma2(mul2(t[c], minus), t[c], one)) : e;
                 }
             }
             ok = tc::mbar_wait_or_abort(bar_addr(&sh.dp_full), n & 1, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after_sync();
+            auto gradients = [&](auto with_mask) {
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                uint32_t s[32], pk[16];
-                tc::tmem_ld_x32(t_dp + x * 32, s);
-                tc::tmem_ld_wait(s);
-#pragma unroll
-                for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(pr[x * 32 + c] * (__uint_as_float(s[c]) - delta));
-                if (masked) {
+                for (int x = 0; x < 2; ++x) {
+                    uint32_t s[32], pk[16];
+                    tc::tmem_ld_x32(t_dp + x * 32, s);
+                    tc::tmem_ld_wait(s);
                     const int a = run.x - col0 - x * 32, e = run.y - col0 - x * 32, q = pre - col0 - x * 32;
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (!((c >= a && c < e) || c < q)) s[c] = 0u;
+                    for (int c = 0; c < 16; ++c) {
+                        float2 w = split(mul2(pr[x * 16 + c], add2(pair(s[2 * c], s[2 * c + 1]), ndelta)));
+                        if constexpr (decltype(with_mask)::value) {
+                            const int i = 2 * c;
+                            if (!((i >= a && i < e) || i < q)) w.x = 0.f;
+                            if (!((i + 1 >= a && i + 1 < e) || i + 1 < q)) w.y = 0.f;
+                        }
+                        pk[c] = pack2<T>(w.x, w.y);
+                    }
+                    tc::tmem_st_x16(t_s + x * 16, pk);
                 }
-#pragma unroll
-                for (int c = 0; c < 16; ++c) pk[c] = pack2<T>(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1]));
-                tc::tmem_st_x16(t_s + x * 16, pk);
-            }
+            };
+            if (masked) gradients(std::true_type{});
+            else gradients(std::false_type{});
             tc::tmem_st_wait();
             tc::fence_before_sync();
             __syncwarp();
@@ -648,12 +633,14 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
             ok = tc::mbar_wait_or_abort(bar_addr(&sh.drain), 0, abort_flag);
             ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
         }
-        ok = __all_sync(0xffffffffu, ok);
+        ok = tc::named_barrier_and(1, 256, ok);                                // all warps go on together
         if (!ok) *abort_flag = 1;
         tc::fence_after_sync();
         bool fine = ok;
+        const bool whole = ok && t1 - t0 == tokens;
         // each warpgroup writes its half of the columns
         if (ok && t0 < t1) {
+            T *out = valid ? static_cast<T *>(g.dq) + out_row * DIM : nullptr;
 #pragma unroll
             for (int c = 0; c < DIM / 64; ++c) {
                 const int col = half * (DIM / 2) + c * 32;
@@ -665,27 +652,23 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0;
                 }
-                float worst = 0.f;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float x = __uint_as_float(o[i]) * p.scale;
-                    o[i] = __float_as_uint(x);
-                    worst = fmaf(x, 0.f, worst);
-                }
-                fine = fine && worst == 0.f;
-                if (valid) {
-                    uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(g.dq) + out_row * DIM + col);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        dst[i] = make_uint4(pack2<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1])),
-                                            pack2<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3])),
-                                            pack2<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5])),
-                                            pack2<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7])));
-                }
+                const bool good = put_row<T>(o, p.scale, whole ? base_ptr : nullptr, out, row, col);
+                fine = fine && good;
             }
         }
-        unsigned again = __ballot_sync(0xffffffffu, valid && !fine);
-        tc::named_barrier(1, 256);
+        if (whole) tc::fence_proxy_async_smem();
+        const bool any = tc::named_barrier_or(1, 256, valid && !fine);
+        if (whole && tid == 0) {
+            for (int c = 0; c < DIM / 64; ++c) tc::tma_store_4d(&tm_dq, c * 64, 0, D.q0 + t0, h, s_q + c * kBlock);
+            tc::tma_store_commit();
+            if (any) tc::tma_store_wait_all();
+            else tc::tma_store_wait_read();
+        }
+        unsigned again = 0;
+        if (any) {
+            tc::named_barrier(1, 256);
+            again = __ballot_sync(0xffffffffu, valid && !fine);
+        }
         while (again) {
             const int r = (row & ~31) + __ffs(again) - 1;
             again &= again - 1;
@@ -700,22 +683,31 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
 template <typename T, int DIM> int launch(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st)
 {
     const int tokens = kTile / p.G, docs = p.n_docs + (p.cu_q ? 1 : 0);
-    CUtensorMap tm_q, tm_do, tm_k, tm_v;
+    CUtensorMap tm_q, tm_do, tm_k, tm_v, tm_dq, tm_dk, tm_dv;
     if (int rc = local_query_map(&tm_q, p, p.q, p.q_sh, p.q_st, dtype)) return rc;
     if (int rc = local_query_map(&tm_do, p, g.dout, g.do_sh, g.do_st, dtype)) return rc;
     if (int rc = local_key_map(&tm_k, p, p.k, p.k_sh, p.k_st, dtype)) return rc;
     if (int rc = local_key_map(&tm_v, p, p.v, p.v_sh, p.v_st, dtype)) return rc;
+    if (int rc = local_query_map(&tm_dq, p, g.dq, int64_t(p.S) * DIM, DIM, dtype)) return rc;
+    if (int rc = local_key_map(&tm_dk, p, g.dk, int64_t(p.N) * DIM, DIM, dtype)) return rc;
+    if (int rc = local_key_map(&tm_dv, p, g.dv, int64_t(p.N) * DIM, DIM, dtype)) return rc;
     const bool bf16 = dtype == FM_BF16;
     const uint32_t idesc_s = tc::instr_desc_f16(bf16, kTile, kTile), idesc_o = tc::instr_desc_f16(bf16, kTile, DIM, false, true);
     const int64_t q_blocks = std::min<int64_t>(p.S, (int64_t(p.S) + int64_t(docs) * (tokens - 1)) / tokens) * p.H;
     const int64_t k_blocks = std::min<int64_t>(p.N, (int64_t(p.N) + int64_t(docs) * (kTile - 1)) / kTile) * p.H;
-    FM_CUDA_OK(func_attr_cached((const void *)local_dq_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DqCfg<DIM>::kSmem));
-    FM_CUDA_OK(func_attr_cached((const void *)local_dkv_kernel<T, DIM>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DkvCfg<DIM>::kSmem));
-    local_dkv_kernel<T, DIM><<<unsigned(k_blocks), kThreads, DkvCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, idesc_s, idesc_o);
-    FM_LAUNCHED("local_dkv_kernel");
-    local_dq_kernel<T, DIM><<<unsigned(q_blocks), kThreads, DqCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, idesc_s, idesc_o);
-    FM_LAUNCHED("local_dq_kernel");
-    return FM_OK;
+    auto launch_mode = [&](auto cap, auto slopes) -> int {
+        auto *dkv = local_dkv_kernel<T, DIM, decltype(cap)::value, decltype(slopes)::value>;
+        auto *dq = local_dq_kernel<T, DIM, decltype(cap)::value, decltype(slopes)::value>;
+        FM_CUDA_OK(func_attr_cached((const void *)dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DkvCfg<DIM>::kSmem));
+        FM_CUDA_OK(func_attr_cached((const void *)dq, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DqCfg<DIM>::kSmem));
+        dkv<<<unsigned(k_blocks), kThreads, DkvCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, tm_dk, tm_dv, idesc_s, idesc_o);
+        FM_LAUNCHED("local_dkv_kernel");
+        dq<<<unsigned(q_blocks), kThreads, DqCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, tm_dq, idesc_s, idesc_o);
+        FM_LAUNCHED("local_dq_kernel");
+        return FM_OK;
+    };
+    if (p.cap > 0.f) return p.slopes ? launch_mode(std::true_type{}, std::true_type{}) : launch_mode(std::true_type{}, std::false_type{});
+    return p.slopes ? launch_mode(std::false_type{}, std::true_type{}) : launch_mode(std::false_type{}, std::false_type{});
 }
 
 }  // namespace

@@ -30,6 +30,8 @@
 // rows and their LSE in the workspace, and local_combine joins them.
 #include "local_tc.cuh"
 
+#include <type_traits>
+
 namespace fm {
 
 namespace {
@@ -108,42 +110,29 @@ __device__ __forceinline__ void make_block(const LocalParams &p, Block &b, const
     b.n1 = int(int64_t(n) * (part + 1) / parts);
 }
 
-// Column c is a visible key if it lies in [a, b) or below pre.
-__device__ __forceinline__ void mask_scores(uint32_t (&s)[32], int a, int b, int pre)
+// Column c is a visible key if it lies in [a, b) or below pre; the others become `hidden`.
+__device__ __forceinline__ void mask_scores(uint32_t (&s)[32], int a, int b, int pre, uint32_t hidden)
 {
 #pragma unroll
     for (int c = 0; c < 32; ++c)
-        if (!((c >= a && c < b) || c < pre)) s[c] = 0xff800000u;
+        if (!((c >= a && c < b) || c < pre)) s[c] = hidden;
 }
 
 // Scores in log2 units after scale, cap and distance (fp: the row's position less the first column's); what is left to multiply
 // is 1.
-__device__ __forceinline__ void shape_scores(const LocalParams &p, uint32_t (&s)[32], float slope2, float fp)
+template <bool CAP, bool SLOPES>
+__device__ __forceinline__ void shape_scores(const LocalParams &p, uint32_t (&s)[32], float slope2, float fp, bool valid)
 {
-    if (p.cap > 0.f) {
-        float big[2] = {0.f, 0.f};
+    const float c2 = CAP ? p.cap * kLog2e : p.scale * kLog2e;
+    f32x2 t[16];
+    if constexpr (CAP) cap_scores(t, s, p.scale / p.cap, valid);
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) big[c >> 1 & 1] = max3(big[c >> 1 & 1], fabsf(__uint_as_float(s[c])), fabsf(__uint_as_float(s[c + 1])));
-        const float k = p.scale / p.cap, c2 = p.cap * kLog2e;
-        if (__all_sync(0xffffffffu, fmaxf(big[0], big[1]) * fabsf(k) <= kTanhRange)) {
-#pragma unroll
-            for (int c = 0; c < 32; c += 2) {
-                const float2 t = split(mul2(tanh_small(mul2(pair(s[c], s[c + 1]), pair(k, k))), pair(c2, c2)));
-                s[c] = __float_as_uint(t.x);
-                s[c + 1] = __float_as_uint(t.y);
-            }
-        } else {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(c2 * tanh_any(__uint_as_float(s[c]) * k));
-        }
-    } else {
-        const float k = p.scale * kLog2e;
-#pragma unroll
-        for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(__uint_as_float(s[c]) * k);
-    }
-    if (p.slopes) {
-#pragma unroll
-        for (int c = 0; c < 32; ++c) s[c] = __float_as_uint(fmaf(-slope2, fabsf(fp - float(c)), __uint_as_float(s[c])));
+    for (int c = 0; c < 16; ++c) {
+        f32x2 e = mul2(CAP ? t[c] : pair(s[2 * c], s[2 * c + 1]), pair(c2, c2));
+        if constexpr (SLOPES) e = fma2(pair(-slope2, -slope2), pair(fabsf(fp - float(2 * c)), fabsf(fp - float(2 * c + 1))), e);
+        const float2 v = split(e);
+        s[2 * c] = __float_as_uint(v.x);
+        s[2 * c + 1] = __float_as_uint(v.y);
     }
 }
 
@@ -184,10 +173,10 @@ template <typename T, int D> __device__ __forceinline__ void redo_rows(const Loc
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool CAP, bool SLOPES>
 __global__ void __launch_bounds__(kThreads, 1)
 local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                 const __grid_constant__ CUtensorMap tm_v, uint32_t idesc_s, uint32_t idesc_o, float *part_o, float *part_lse)
+                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, uint32_t idesc_s, uint32_t idesc_o, float *part_o, float *part_lse)
 {
     extern __shared__ __align__(1024) unsigned char smem_dyn[];
     using C = Cfg<D>;
@@ -368,8 +357,9 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         const int shift = b.D.nk - b.D.nq, pos = shift + token;
         const int safe_lo = p.window ? shift + b.t1[s] - p.window : 0;         // keys in [safe_lo, safe_hi) are seen by every row
         const int safe_hi = local_run(p, shift + b.t0[s], b.D.nk).y;
-        const bool shaped = p.cap > 0.f || p.slopes || !(p.scale > 0.f);
-        const float mul = shaped ? 1.f : p.scale * kLog2e;
+        constexpr bool shaped = CAP || SLOPES;
+        const float mul = shaped ? 1.f : p.scale * kLog2e;                     // positive
+        const float slope2 = p.slopes && valid ? p.slopes[head] * kLog2e : 0.f;
         const Steps st(b, s);
         float m = -INFINITY, l = 0.f;
         int done = 0;
@@ -389,23 +379,26 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 tc::tmem_ld_wait(x[0]);
                 tc::tmem_ld_x32(t_p + 32, x[1]);
                 const bool masked = !(j0 + kStep <= b.D.prefix || (j0 >= safe_lo && j0 + kStep <= safe_hi));
-                if (!fresh && !masked && !shaped) {
+                if (!fresh && !masked) {
                     // the usual step: half of the scores arrive under the exponentials of the others
+                    if constexpr (shaped) shape_scores<CAP, SLOPES>(p, x[0], slope2, float(pos - j0), valid);
                     exp_scores<T>(x[0], mul, m, t_p, sums);
                     tc::tmem_ld_wait(x[1]);
+                    if constexpr (shaped) shape_scores<CAP, SLOPES>(p, x[1], slope2, float(pos - j0 - 32), valid);
                     exp_scores<T>(x[1], mul, m, t_p + 16, sums);
                 } else {
                     tc::tmem_ld_wait(x[1]);
-                    if (shaped) {
-                        const float slope2 = p.slopes && valid ? p.slopes[head] * kLog2e : 0.f;
-                        shape_scores(p, x[0], slope2, float(pos - j0));
-                        shape_scores(p, x[1], slope2, float(pos - j0 - 32));
+                    const int2 run = local_run(p, pos, b.D.nk);
+                    auto mask = [&](uint32_t hidden) {
+                        mask_scores(x[0], run.x - j0, run.y - j0, b.D.prefix - j0, hidden);
+                        mask_scores(x[1], run.x - j0 - 32, run.y - j0 - 32, b.D.prefix - j0 - 32, hidden);
+                    };
+                    if constexpr (shaped) {
+                        if (masked) mask(0u);                                  // what is hidden must not choose the formula
+                        shape_scores<CAP, SLOPES>(p, x[0], slope2, float(pos - j0), valid);
+                        shape_scores<CAP, SLOPES>(p, x[1], slope2, float(pos - j0 - 32), valid);
                     }
-                    if (masked) {
-                        const int2 run = local_run(p, pos, b.D.nk);
-                        mask_scores(x[0], run.x - j0, run.y - j0, b.D.prefix - j0);
-                        mask_scores(x[1], run.x - j0 - 32, run.y - j0 - 32, b.D.prefix - j0 - 32);
-                    }
+                    if (masked) mask(0xff800000u);
                     if (fresh && m == -INFINITY) m = fmaxf(row_max(x[0]), row_max(x[1])) * mul;
                     fresh = __any_sync(0xffffffffu, m == -INFINITY);
                     const float sub = m == -INFINITY ? 0.f : m;
@@ -446,17 +439,19 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 ++done;
             }
         if (ok && done > 0) ok = tc::mbar_wait_or_abort(bar_addr(&sh.o_done[s][(done - 1) & 1]), ((done - 1) >> 1) & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok && !*abort_flag);
+        ok = tc::named_barrier_and(1 + s, 128, ok && !*abort_flag);            // the tile's warps go on together
         if (!ok) *abort_flag = 1;
         tc::fence_after_sync();
         const int64_t out_row = int64_t(head) * p.S + b.D.q0 + token;
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
         const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
         bool fine = ok && l < INFINITY && l >= 0.f;
+        // a whole tile goes out through the query tile's shared memory, which no product reads any more
+        const bool whole = ok && gridDim.y == 1 && b.t1[s] - b.t0[s] == b.tokens && b.tokens > 0;
         if (ok && b.t0[s] < b.t1[s]) {
+            unsigned char *tile = smem_dyn + s * C::kTileBytes;
 #pragma unroll
             for (int c = 0; c < D / 32; ++c) {
-                const int col = c * 32;
                 uint32_t o[32];
                 if (done) {
                     tc::tmem_ld_x32(t_o + c * 32, o);
@@ -465,36 +460,42 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0;
                 }
-                float worst = 0.f;
+                if (gridDim.y == 1) {
+                    T *dst = valid ? static_cast<T *>(p.o) + out_row * D : nullptr;
+                    const bool good = put_row<T>(o, inv, whole ? tile : nullptr, dst, row, c * 32);
+                    fine = fine && good;
+                } else {
+                    float worst = 0.f;
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float f = __uint_as_float(o[i]) * inv;
-                    o[i] = __float_as_uint(f);
-                    worst = fmaf(f, 0.f, worst);                               // NaN as soon as one is not finite
-                }
-                fine = fine && worst == 0.f;
-                if (valid) {
-                    if (gridDim.y == 1) {
-                        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<T *>(p.o) + out_row * D + col);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            dst[i] = make_uint4(pack2<T>(__uint_as_float(o[8 * i]), __uint_as_float(o[8 * i + 1])),
-                                                pack2<T>(__uint_as_float(o[8 * i + 2]), __uint_as_float(o[8 * i + 3])),
-                                                pack2<T>(__uint_as_float(o[8 * i + 4]), __uint_as_float(o[8 * i + 5])),
-                                                pack2<T>(__uint_as_float(o[8 * i + 6]), __uint_as_float(o[8 * i + 7])));
-                    } else {
-                        uint4 *dst = reinterpret_cast<uint4 *>(part_o + (int64_t(blockIdx.y) * p.Hq * p.S + out_row) * D + col);
+                    for (int i = 0; i < 32; ++i) {
+                        const float f = __uint_as_float(o[i]) * inv;
+                        o[i] = __float_as_uint(f);
+                        worst = fmaf(f, 0.f, worst);
+                    }
+                    fine = fine && worst == 0.f;
+                    if (valid) {
+                        uint4 *dst = reinterpret_cast<uint4 *>(part_o + (int64_t(blockIdx.y) * p.Hq * p.S + out_row) * D + c * 32);
 #pragma unroll
                         for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                     }
                 }
             }
         }
-        const unsigned again = __ballot_sync(0xffffffffu, valid && !fine);
         if (gridDim.y == 1) {
             if (valid) p.lse[out_row] = lse;
-            __syncwarp();
-            if (again) redo_rows<T, D>(p, b, again, b.t0[s], row & ~31);
+            if (whole) tc::fence_proxy_async_smem();
+            const bool any = tc::named_barrier_or(1 + s, 128, valid && !fine);
+            if (whole && row == 0) {                                           // (the same thread waits for its stores)
+                for (int c = 0; c < D / 64; ++c) tc::tma_store_4d(&tm_o, c * 64, 0, b.D.q0 + b.t0[s], b.h, base + s * C::kTileBytes + c * kBlock);
+                tc::tma_store_commit();
+                if (any) tc::tma_store_wait_all();
+                else tc::tma_store_wait_read();
+            }
+            if (any) {
+                tc::named_barrier(1 + s, 128);                                 // every row of the tile has been written
+                const unsigned again = __ballot_sync(0xffffffffu, valid && !fine);
+                if (again) redo_rows<T, D>(p, b, again, b.t0[s], row & ~31);
+            }
         } else if (valid) {
             part_lse[int64_t(blockIdx.y) * p.Hq * p.S + out_row] = fine ? lse : __int_as_float(0x7fc00000);
         }
@@ -527,16 +528,25 @@ Shape shape_of(const LocalParams &p)
 template <typename T, int D> int launch(const LocalParams &p, int dtype, void *ws, cudaStream_t st)
 {
     const Shape sh = shape_of(p);
-    CUtensorMap tm_q, tm_k, tm_v;
+    CUtensorMap tm_q, tm_k, tm_v, tm_o;
     if (int rc = local_query_map(&tm_q, p, p.q, p.q_sh, p.q_st, dtype)) return rc;
     if (int rc = local_key_map(&tm_k, p, p.k, p.k_sh, p.k_st, dtype)) return rc;
     if (int rc = local_key_map(&tm_v, p, p.v, p.v_sh, p.v_st, dtype)) return rc;
+    if (int rc = local_query_map(&tm_o, p, p.o, int64_t(p.S) * D, D, dtype)) return rc;
     float *part_lse = static_cast<float *>(ws), *part_o = part_lse + (size_t(sh.parts) * p.Hq * p.S + 31) / 32 * 32;
     const bool bf16 = dtype == FM_BF16;
-    FM_CUDA_OK(func_attr_cached((const void *)local_fwd_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>()));
-    local_fwd_kernel<T, D><<<dim3(unsigned(sh.blocks), unsigned(sh.parts)), kThreads, smem_bytes<D>(), st>>>(
-        p, tm_q, tm_k, tm_v, tc::instr_desc_f16(bf16, ltc::kTile, kStep), tc::instr_desc_f16(bf16, ltc::kTile, D, false, true), part_o, part_lse);
-    FM_LAUNCHED("local_fwd_kernel");
+    auto launch_mode = [&](auto cap, auto slopes) -> int {
+        auto *kernel = local_fwd_kernel<T, D, decltype(cap)::value, decltype(slopes)::value>;
+        FM_CUDA_OK(func_attr_cached((const void *)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<D>()));
+        kernel<<<dim3(unsigned(sh.blocks), unsigned(sh.parts)), kThreads, smem_bytes<D>(), st>>>(
+            p, tm_q, tm_k, tm_v, tm_o, tc::instr_desc_f16(bf16, ltc::kTile, kStep), tc::instr_desc_f16(bf16, ltc::kTile, D, false, true), part_o, part_lse);
+        FM_LAUNCHED("local_fwd_kernel");
+        return FM_OK;
+    };
+    const bool slopes = p.slopes || !(p.scale > 0.f);            // the plain form needs scores that grow with the products
+    const int rc = p.cap > 0.f ? (slopes ? launch_mode(std::true_type{}, std::true_type{}) : launch_mode(std::true_type{}, std::false_type{}))
+                               : (slopes ? launch_mode(std::false_type{}, std::true_type{}) : launch_mode(std::false_type{}, std::false_type{}));
+    if (rc) return rc;
     return sh.parts > 1 ? local_combine(p, dtype, part_o, part_lse, sh.parts, st) : FM_OK;
 }
 

@@ -93,6 +93,47 @@ __device__ __forceinline__ float tanh_any(float x)
     return fmaf(-2.f, r, 1.f);
 }
 
+// t = tanh(s k).  One formula for the warp: the short one if |s k| allows it in every lane that holds a row (what the others hold
+// must not choose).
+__device__ __forceinline__ void cap_scores(f32x2 (&t)[16], const uint32_t (&s)[32], float k, bool valid)
+{
+    float big[2] = {0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 32; c += 2) big[c >> 1 & 1] = max3(big[c >> 1 & 1], fabsf(__uint_as_float(s[c])), fabsf(__uint_as_float(s[c + 1])));
+    if (__all_sync(0xffffffffu, !valid || fmaxf(big[0], big[1]) * fabsf(k) <= kTanhRange)) {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) t[c] = tanh_small(mul2(pair(s[2 * c], s[2 * c + 1]), pair(k, k)));
+    } else {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) t[c] = pair(tanh_any(__uint_as_float(s[2 * c]) * k), tanh_any(__uint_as_float(s[2 * c + 1]) * k));
+    }
+}
+
+// 32 accumulator columns of a row, scaled and rounded, into a tile in shared memory (128-byte swizzle; dst: the tile, generic
+// address) or straight to the row.  Returns false if one of them is not finite.  A thread's row written straight costs 32
+// lines an instruction; through shared memory and a TMA store it costs four.
+template <typename T> __device__ __forceinline__ bool put_row(const uint32_t (&o)[32], float f, unsigned char *tile, T *row_ptr, int row, int col)
+{
+    uint4 v[4];
+    uint32_t *w = reinterpret_cast<uint32_t *>(v);
+    float worst = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float a = __uint_as_float(o[2 * i]) * f, b = __uint_as_float(o[2 * i + 1]) * f;
+        worst = fmaf(a, 0.f, fmaf(b, 0.f, worst));                             // NaN as soon as one is not finite
+        w[i] = pack2<T>(a, b);
+    }
+    if (tile) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4 *>(tile + (col >> 6) * kBlock + row * 128 + ((((col & 63) >> 3) + i) ^ (row & 7)) * 16) = v[i];
+    } else if (row_ptr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4 *>(row_ptr + col)[i] = v[i];
+    }
+    return worst == 0.f;
+}
+
 // A value that is the same in every lane, so that the compiler can see it.
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
