@@ -110,12 +110,14 @@ __device__ __forceinline__ void make_block(const LocalParams &p, Block &b, const
     b.n1 = int(int64_t(n) * (part + 1) / parts);
 }
 
+// Bits [0, x) of a word, for any x.
+__device__ __forceinline__ uint32_t bits_below(int x) { return x <= 0 ? 0u : x >= 32 ? 0xffffffffu : (1u << x) - 1u; }
 // Column c is a visible key if it lies in [a, b) or below pre; the others become `hidden`.
 __device__ __forceinline__ void mask_scores(uint32_t (&s)[32], int a, int b, int pre, uint32_t hidden)
 {
+    const uint32_t seen = (bits_below(b) & ~bits_below(a)) | bits_below(pre);
 #pragma unroll
-    for (int c = 0; c < 32; ++c)
-        if (!((c >= a && c < b) || c < pre)) s[c] = hidden;
+    for (int c = 0; c < 32; ++c) s[c] = (seen & (1u << c)) ? s[c] : hidden;
 }
 
 // Scores in log2 units after scale, cap and distance (fp: the row's position less the first column's); what is left to multiply
@@ -186,43 +188,48 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
     const uint32_t ring0 = base + 2 * C::kTileBytes;
     volatile int *abort_flag = &sh.abort;
 
-    if (warp == 0) {
+    const Block &b = sh.b;
+    // The loading warp makes the barriers and the block and starts loading at once; everybody meets when it has filled the ring.
+    auto meet = [&] {
+        tc::fence_before_sync();
+        tc::named_barrier(3, kThreads);
+        tc::fence_after_sync();
+    };
+    if (warp == kLoadWarp) {
+        if (lane == 0) {
+            tc::prefetch_tensormap(&tm_q);
+            tc::prefetch_tensormap(&tm_k);
+            tc::prefetch_tensormap(&tm_v);
+            for (int s = 0; s < 2; ++s) {
+                tc::mbar_init(bar_addr(&sh.q_full[s]), 1);
+                tc::mbar_init(bar_addr(&sh.drain[s]), 1);
+                for (int u = 0; u < 2; ++u) {
+                    tc::mbar_init(bar_addr(&sh.s_full[s][u]), 1);
+                    tc::mbar_init(bar_addr(&sh.p_full[s][u]), 4);
+                    tc::mbar_init(bar_addr(&sh.o_done[s][u]), 1);
+                }
+            }
+            for (int i = 0; i < C::kRing; ++i) {
+                tc::mbar_init(bar_addr(&sh.full[i]), 1);
+                tc::mbar_init(bar_addr(&sh.empty[i]), 2);                          // both product warps let go of it
+            }
+            tc::mbar_init(bar_addr(&sh.tail), 1);
+            tc::mbar_fence_init();
+            sh.abort = 0;
+        }
         // the last blocks of a document have the most keys (causal): they go first
-        const int nb = gridDim.x / p.H, h = blockIdx.x / nb;
+        const int nb = gridDim.x / p.H;
         Doc doc;
         const int index = find_block<false>(p, 2 * (kTile / p.G), nb - 1 - int(blockIdx.x % nb), doc);
         if (lane == 0) {
-            if (index >= 0) make_block(p, sh.b, doc, index, h, blockIdx.y, gridDim.y);
-            else { sh.b = Block{}; }
+            if (index >= 0) make_block(p, sh.b, doc, index, blockIdx.x / nb, blockIdx.y, gridDim.y);
+            else sh.b = Block{};
         }
+        __syncwarp();
+    } else {
+        if (warp == kMmaWarp) tc::tmem_alloc(tc::smem_addr(&sh.tmem_slot), 512);
+        meet();
     }
-    if (warp == kMmaWarp) tc::tmem_alloc(tc::smem_addr(&sh.tmem_slot), 512);
-    if (warp == kLoadWarp && lane == 0) {
-        for (int s = 0; s < 2; ++s) {
-            tc::mbar_init(bar_addr(&sh.q_full[s]), 1);
-            tc::mbar_init(bar_addr(&sh.drain[s]), 1);
-            for (int u = 0; u < 2; ++u) {
-                tc::mbar_init(bar_addr(&sh.s_full[s][u]), 1);
-                tc::mbar_init(bar_addr(&sh.p_full[s][u]), 4);
-                tc::mbar_init(bar_addr(&sh.o_done[s][u]), 1);
-            }
-        }
-        for (int i = 0; i < C::kRing; ++i) {
-            tc::mbar_init(bar_addr(&sh.full[i]), 1);
-            tc::mbar_init(bar_addr(&sh.empty[i]), 2);                          // both product warps let go of it
-        }
-        tc::mbar_init(bar_addr(&sh.tail), 1);
-        tc::mbar_fence_init();
-        sh.abort = 0;
-        tc::prefetch_tensormap(&tm_q);
-        tc::prefetch_tensormap(&tm_k);
-        tc::prefetch_tensormap(&tm_v);
-    }
-    tc::fence_before_sync();
-    __syncthreads();
-    tc::fence_after_sync();
-    const Block &b = sh.b;
-    const uint32_t tmem = sh.tmem_slot;
     const int n0 = b.n0, n1 = b.n1;
 
     // 384 threads x 168 registers at launch = 256 x 216 + 128 x 72
@@ -230,6 +237,8 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         tc::set_registers_down<72>();
         if (warp == kLoadWarp) {
             // ---- loads ----------------------------------------------------------------------------------------------------
+            int issued = 0;
+            bool ok = true, met = false;
             if (n1 > n0) {
                 if (lane < 2 && b.t0[lane] < b.t1[lane]) {
                     const int s = lane;
@@ -241,8 +250,6 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 const int page = p.table ? 1 << p.page_shift : kTile;
                 const int boxes = page >= kTile ? 1 : kTile / page;
                 const int box_rows = min(page, kTile);
-                int issued = 0;
-                bool ok = true;
                 // lane x * (d / 64) + c loads column block c of the tile's box x; its page is looked up a tile ahead
                 const int box = lane / (D / 64), col = lane % (D / 64);
                 auto look_up = [&](int n) {
@@ -256,13 +263,17 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                     const int live = rows >= kTile ? boxes : (rows + box_rows - 1) / box_rows;
                     const int next_id = look_up(n + 1);
                     const int y = p.table ? (j0 + box * box_rows) & (page - 1) : b.D.k0 + j0, z = p.table ? page_id * p.H + b.h : b.h;
-                    for (int kv = 0; kv < 2 && ok; ++kv, ++issued) {
+                    for (int kv = 0; kv < 2; ++kv) {
                         const int slot = issued % C::kRing;
+                        const bool cut = kv == 1 && rows < kTile;                  // a V tile whose last rows must be zeroed
+                        if (!met && (issued >= C::kRing || cut)) {
+                            meet();
+                            met = true;
+                        }
                         if (issued >= C::kRing) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((issued / C::kRing) & 1) ^ 1, abort_flag);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         const uint32_t dst = ring0 + slot * C::kTileBytes;
-                        const bool cut = kv == 1 && rows < kTile;                  // a V tile whose last rows must be zeroed
                         const uint32_t bar = bar_addr(cut ? &sh.tail : &sh.full[slot]);
                         if (lane == 0) tc::mbar_arrive_expect_tx(bar, uint32_t(live) * box_rows * (D * 2));
                         __syncwarp();
@@ -279,21 +290,23 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                             __syncwarp();
                             if (lane == 0) tc::mbar_arrive(bar_addr(&sh.full[slot]));
                         }
+                        ++issued;
                     }
                     page_id = next_id;
                 }
-                if (!ok) {
-                    // unwind: every copy in flight lands before the CTA's shared memory goes away
-                    if (lane == 0) *abort_flag = 1;
-                    for (int i = max(issued - C::kRing, 0); i < issued; ++i) tc::mbar_wait(bar_addr(&sh.full[i % C::kRing]), (i / C::kRing) & 1);
-                    for (int s = 0; s < 2; ++s)
-                        if (b.t0[s] < b.t1[s]) tc::mbar_wait(bar_addr(&sh.q_full[s]), 0);
-                }
+            }
+            if (!met) meet();
+            if (!ok) {
+                // unwind: every copy in flight lands before the CTA's shared memory goes away
+                if (lane == 0) *abort_flag = 1;
+                for (int i = max(issued - C::kRing, 0); i < issued; ++i) tc::mbar_wait(bar_addr(&sh.full[i % C::kRing]), (i / C::kRing) & 1);
+                for (int s = 0; s < 2; ++s)
+                    if (b.t0[s] < b.t1[s]) tc::mbar_wait(bar_addr(&sh.q_full[s]), 0);
             }
         } else if (warp < kLoadWarp && n1 > n0) {
             // ---- products of one query tile: S runs two steps ahead of P V -----------------------------------------------------
             const int s = warp - kMmaWarp, m0 = uniform(n0), m1 = uniform(n1);
-            const uint32_t t_s = uniform(int(tmem)) + s * 128, t_o = uniform(int(tmem)) + 256 + s * 128;
+            const uint32_t t_s = uniform(int(sh.tmem_slot)) + s * 128, t_o = t_s + 256;
             const Steps st(b, s);
             const bool leader = tc::elect_one();
             bool ok = true;                                                    // (what the leader's waits said; the others follow the same path)
@@ -350,8 +363,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         tc::set_registers_up<216>();
         // ---- softmax and epilogue ---------------------------------------------------------------------------------------
         const int s = warp >> 2, row = tid & 127;
-        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
-        const uint32_t t_s = tmem + s * 128 + lanes, t_o = tmem + 256 + s * 128 + lanes;
+        const uint32_t t_s = sh.tmem_slot + s * 128 + (uint32_t((warp & 3) * 32) << 16), t_o = t_s + 256;
         const int token = b.t0[s] + row / p.G, head = b.h * p.G + row % p.G;
         const bool valid = row < b.tokens * p.G && token < b.t1[s];
         const int shift = b.D.nk - b.D.nq, pos = shift + token;
@@ -502,7 +514,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         tc::fence_before_sync();
     }
     __syncthreads();
-    if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
+    if (warp == kMmaWarp) tc::tmem_dealloc(sh.tmem_slot, 512);
 }
 
 // Blocks of query tiles, at most, and the parts that their key tiles are cut into: only where the blocks fill less than half
