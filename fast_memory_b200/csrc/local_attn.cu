@@ -193,6 +193,12 @@ static int local_params(const fm_local_attn_args *a, LocalParams &p)
     return FM_OK;
 }
 
+static size_t forward_workspace(const LocalParams &p, int dtype)
+{
+    if (local_decode_fits(p, dtype)) return local_decode_workspace(p);
+    return local_tc_fits(p, dtype) ? local_tc_fwd_workspace(p) : local_simt_fwd_workspace(p);
+}
+
 }  // namespace fm
 
 extern "C" {
@@ -201,7 +207,7 @@ size_t fm_local_attn_workspace_bytes(const fm_local_attn_args *a)
 {
     fm::LocalParams p;
     if (fm::local_params(a, p) || p.S == 0) return 0;
-    return fm::local_tc_fits(p, a->dtype) ? fm::local_tc_fwd_workspace(p) : fm::local_simt_fwd_workspace(p);
+    return fm::forward_workspace(p, a->dtype);
 }
 
 int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *workspace, size_t workspace_bytes, fm_stream_t stream)
@@ -211,7 +217,7 @@ int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *wo
     if (int rc = local_params(a, p)) return rc;
     if (p.S == 0) return FM_OK;
     FM_REQUIRE(p.q && o && lse && (p.table || p.N == 0 || (p.k && p.v)), "fm_local_attn_fwd: null pointer");
-    const size_t need = local_tc_fits(p, a->dtype) ? local_tc_fwd_workspace(p) : local_simt_fwd_workspace(p);
+    const size_t need = forward_workspace(p, a->dtype);
     if (need && (workspace_bytes < need || !workspace)) {
         set_error("fm_local_attn_fwd: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
         return FM_ERR_WORKSPACE;
@@ -220,6 +226,7 @@ int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *wo
     p.o = o;
     p.lse = lse;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (local_decode_fits(p, a->dtype)) return local_decode_fwd(p, a->dtype, workspace, st);
     if (local_tc_fits(p, a->dtype)) return local_tc_fwd(p, a->dtype, workspace, st);
     return local_simt_fwd(p, a->dtype, workspace, st);
 }

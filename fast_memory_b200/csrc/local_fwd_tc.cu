@@ -575,14 +575,15 @@ int local_query_map(CUtensorMap *map, const LocalParams &p, const void *q, int64
     return make_tensor_map(map, q, dtype, 4, dims, strides, box);
 }
 
-// Keys as (d, row, KV head), or pages as (d, row of the page, page x head): a box is one tile, or the part of it in one page.
-int local_key_map(CUtensorMap *map, const LocalParams &p, const void *k, int64_t sh, int64_t st, int dtype)
+// Keys as (d, row, KV head), or pages as (d, row of the page, page x head): a box is one tile of
+// `rows` keys, or the part of it in one page.
+int local_key_map(CUtensorMap *map, const LocalParams &p, const void *k, int64_t sh, int64_t st, int dtype, int rows)
 {
     auto bytes = [](int64_t stride) { return uint64_t(stride > 0 ? stride * 2 : 16); };
     const int64_t page = int64_t(1) << p.page_shift;
     const uint64_t dims[3] = {uint64_t(p.d), uint64_t(p.table ? page : p.N), uint64_t(p.table ? int64_t(p.n_pages) * p.H : p.H)};
     const uint64_t strides[2] = {p.table ? uint64_t(p.d) * 2 : bytes(st), p.table ? uint64_t(page) * p.d * 2 : bytes(sh)};
-    const uint32_t box[3] = {64, uint32_t(p.table ? std::min<int64_t>(page, ltc::kTile) : ltc::kTile), 1};
+    const uint32_t box[3] = {64, uint32_t(p.table ? std::min<int64_t>(page, rows) : rows), 1};
     return make_tensor_map(map, k, dtype, 3, dims, strides, box);
 }
 

@@ -182,10 +182,15 @@ int local_combine(const LocalParams &p, int dtype, const float *part_o, const fl
 
 // Whether a call goes to the tcgen05 kernels, their launches and tensor maps.
 int local_query_map(CUtensorMap *map, const LocalParams &p, const void *q, int64_t sh, int64_t st, int dtype);
-int local_key_map(CUtensorMap *map, const LocalParams &p, const void *k, int64_t sh, int64_t st, int dtype);
+int local_key_map(CUtensorMap *map, const LocalParams &p, const void *k, int64_t sh, int64_t st, int dtype, int rows = ltc::kTile);
 int local_tc_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st);
 int local_tc_fwd(const LocalParams &p, int dtype, void *ws, cudaStream_t st);
 size_t local_tc_fwd_workspace(const LocalParams &p);
 bool local_tc_fits(const LocalParams &p, int dtype);
+
+// Few queries a document (mma.sync): the same for it.
+bool local_decode_fits(const LocalParams &p, int dtype);
+size_t local_decode_workspace(const LocalParams &p);
+int local_decode_fwd(const LocalParams &p, int dtype, void *ws, cudaStream_t st);
 
 }  // namespace fm
