@@ -193,6 +193,10 @@ static int local_params(const fm_local_attn_args *a, LocalParams &p)
     return FM_OK;
 }
 
+// Workspace of the backward pass: delta, then the parts of dV and dK.
+static size_t delta_bytes(const LocalParams &p) { return align_up(size_t(p.Hq) * size_t(p.S) * sizeof(float), 256); }
+static size_t parts_bytes(const LocalParams &p, int dtype) { return p.S > 0 && local_tc_fits(p, dtype) ? local_tc_bwd_workspace(p) : 0; }
+
 static size_t forward_workspace(const LocalParams &p, int dtype)
 {
     if (local_decode_fits(p, dtype)) return local_decode_workspace(p);
@@ -233,8 +237,8 @@ int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *wo
 
 size_t fm_local_attn_bwd_workspace_bytes(const fm_local_attn_args *a)
 {
-    if (!a || a->n_q_rows < 0 || a->n_q_heads < 0) return 0;
-    return fm::align_up(size_t(a->n_q_heads) * size_t(a->n_q_rows) * sizeof(float), 256) + 256;
+    fm::LocalParams p;
+    return fm::local_params(a, p) ? 0 : fm::delta_bytes(p) + fm::parts_bytes(p, a->dtype);
 }
 
 int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *lse, const void *d_o, int64_t do_stride_head,
@@ -251,10 +255,12 @@ int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *l
     if (p.S == 0 && p.N == 0) return FM_OK;
     FM_REQUIRE(p.S == 0 || (p.q && o && lse && d_o && dq), "fm_local_attn_bwd: null pointer");
     FM_REQUIRE(p.N == 0 || (p.k && p.v && dk && dv), "fm_local_attn_bwd: null pointer");
-    if (workspace_bytes < fm_local_attn_bwd_workspace_bytes(a) || !workspace) {
-        set_error("fm_local_attn_bwd: workspace of %zu bytes, %zu are needed", workspace_bytes, fm_local_attn_bwd_workspace_bytes(a));
+    const size_t need = delta_bytes(p) + parts_bytes(p, a->dtype);
+    if (need && (workspace_bytes < need || !workspace)) {
+        set_error("fm_local_attn_bwd: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
         return FM_ERR_WORKSPACE;
     }
+    FM_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "fm_local_attn_bwd: misaligned buffer");
     FM_REQUIRE((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) % 16 == 0, "fm_local_attn_bwd: misaligned buffer");
     FM_REQUIRE((reinterpret_cast<uintptr_t>(d_o) | reinterpret_cast<uintptr_t>(o) | uintptr_t((do_stride_head | do_stride_row) * elem_bytes(a->dtype))) % 16 == 0,
                "fm_local_attn_bwd: rows must start on 16-byte boundaries");
@@ -271,7 +277,7 @@ int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *l
         });
         if (rc) return rc;
     }
-    if (p.S > 0 && local_tc_fits(p, a->dtype)) return local_tc_bwd(p, g, a->dtype, st);
+    if (p.S > 0 && local_tc_fits(p, a->dtype)) return local_tc_bwd(p, g, a->dtype, reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(p)), st);
     return local_simt_bwd(p, g, a->dtype, st);
 }
 

@@ -60,7 +60,8 @@ template <typename T, int DIM, bool CAP, bool SLOPES>
 __global__ void __launch_bounds__(kThreads, 1)
 local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ BwdParams g, const __grid_constant__ CUtensorMap tm_q,
                  const __grid_constant__ CUtensorMap tm_do, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                 const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv, uint32_t idesc_s, uint32_t idesc_o)
+                 const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv, uint32_t idesc_s, uint32_t idesc_o,
+                 float *parts)
 {
     extern __shared__ unsigned char smem_dyn[];
     __shared__ __align__(16) DkvShared<DIM> sh;
@@ -86,8 +87,10 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 const int last = min(sh.j0 + kTile, sh.D.nk) - 1;
                 int2 run = make_int2(local_query_run(p, sh.D, sh.j0).x, local_query_run(p, sh.D, last).y);
                 if (sh.j0 < sh.D.prefix) run = make_int2(0, sh.D.nq);
-                sh.q_lo = run.x / tokens;
-                sh.n_q = run.y > run.x ? (run.y + tokens - 1) / tokens - sh.q_lo : 0;
+                const int lo = run.x / tokens, n = run.y > run.x ? (run.y + tokens - 1) / tokens - lo : 0;
+                const int from = int(int64_t(n) * blockIdx.y / gridDim.y), to = int(int64_t(n) * (blockIdx.y + 1) / gridDim.y);
+                sh.q_lo = lo + from;                             // this CTA's part of the query tiles
+                sh.n_q = to - from;
             }
         }
     }
@@ -357,8 +360,27 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         // first warpgroup: dV, second: dK; a whole tile goes out through the shared memory of K or V, which no product reads any more
         bool fine = ok;
         const float f = half ? p.scale : 1.f;
-        const bool whole = ok && j0 >= 0 && j0 + kTile <= D.nk;
-        if (ok && j0 >= 0) {
+        const bool whole = ok && j0 >= 0 && j0 + kTile <= D.nk && gridDim.y == 1;
+        if (gridDim.y > 1) {
+            // parts stay fp32, and local_dkv_join looks for what is not finite
+            float *out = parts + ((int64_t(blockIdx.y) * 2 + half) * p.H * p.N + int64_t(h) * p.N + D.k0 + j) * DIM;
+#pragma unroll
+            for (int c = 0; c < DIM / 32; ++c) {
+                uint32_t o[32];
+                if (ok && n_q > 0) {
+                    tc::tmem_ld_x32(tmem + 256 + half * 128 + lanes + c * 32, o);
+                    tc::tmem_ld_wait(o);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = ok ? 0u : 0x7fc00000u;
+                }
+                if (valid) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) reinterpret_cast<uint4 *>(out + c * 32)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                }
+            }
+            fine = true;
+        } else if (ok && j0 >= 0) {
             T *out = valid ? static_cast<T *>(half ? g.dk : g.dv) + (int64_t(h) * p.N + D.k0 + j) * DIM : nullptr;
 #pragma unroll
             for (int c = 0; c < DIM / 32; ++c) {
@@ -396,6 +418,36 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
     }
     __syncthreads();
     if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
+}
+
+// Sums the parts of dV and dK in their order: a warp a key row.
+template <typename T, int DIM>
+__global__ void __launch_bounds__(256) local_dkv_join(const __grid_constant__ LocalParams p, const __grid_constant__ BwdParams g, const float *parts, int n)
+{
+    const int64_t row = (int64_t(blockIdx.x) * 256 + threadIdx.x) >> 5, rows = int64_t(p.H) * p.N;
+    if (row >= rows) return;
+    constexpr int E = DIM / 32;
+    const int c = (threadIdx.x & 31) * E;
+    float dv[E] = {}, dk[E] = {}, worst = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            dv[e] += parts[(int64_t(2 * i) * rows + row) * DIM + c + e];
+            dk[e] += parts[(int64_t(2 * i + 1) * rows + row) * DIM + c + e];
+        }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        dk[e] *= p.scale;
+        worst = fmaf(dv[e], 0.f, fmaf(dk[e], 0.f, worst));
+        static_cast<T *>(g.dv)[row * DIM + c + e] = Elem<T>::from_f32(dv[e]);
+        static_cast<T *>(g.dk)[row * DIM + c + e] = Elem<T>::from_f32(dk[e]);
+    }
+    if (__any_sync(0xffffffffu, worst != 0.f)) {
+        const int r = int(row % p.N);
+        const Doc doc = local_doc<true>(p, p.cu_k ? local_find(p.cu_k, p.n_docs, r) : 0);
+        local_row_dkv<T, DIM>(p, g, doc, int(row / p.N), r - doc.k0);
+    }
 }
 
 // ========================================================= dQ ==============================================================
@@ -680,7 +732,24 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
     if (warp == kMmaWarp) tc::tmem_dealloc(tmem, 512);
 }
 
-template <typename T, int DIM> int launch(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st)
+// Key blocks, at most, and the parts that the query tiles of a block are cut into: only where the blocks fill less than half of the
+// SMs, with at least two query tiles a part.
+struct KeyShape {
+    int64_t blocks;
+    int parts;
+};
+KeyShape key_shape(const LocalParams &p)
+{
+    const int docs = p.n_docs + (p.cu_k ? 1 : 0), tokens = kTile / p.G;
+    KeyShape s{std::min<int64_t>(p.N, (int64_t(p.N) + int64_t(docs) * (kTile - 1)) / kTile) * p.H, 1};
+    int64_t rows = p.S;
+    if (p.window && !p.prefix) rows = std::min<int64_t>(rows, int64_t(p.window) * (p.causal ? 1 : 2) + kTile);
+    if (s.blocks > 0 && s.blocks * 2 <= sm_count())
+        s.parts = int(std::max<int64_t>(1, std::min<int64_t>(sm_count() / s.blocks, ceil_div(rows, tokens) / 2)));
+    return s;
+}
+
+template <typename T, int DIM> int launch(const LocalParams &p, const BwdParams &g, int dtype, float *parts, cudaStream_t st)
 {
     const int tokens = kTile / p.G, docs = p.n_docs + (p.cu_q ? 1 : 0);
     CUtensorMap tm_q, tm_do, tm_k, tm_v, tm_dq, tm_dk, tm_dv;
@@ -694,14 +763,18 @@ template <typename T, int DIM> int launch(const LocalParams &p, const BwdParams 
     const bool bf16 = dtype == FM_BF16;
     const uint32_t idesc_s = tc::instr_desc_f16(bf16, kTile, kTile), idesc_o = tc::instr_desc_f16(bf16, kTile, DIM, false, true);
     const int64_t q_blocks = std::min<int64_t>(p.S, (int64_t(p.S) + int64_t(docs) * (tokens - 1)) / tokens) * p.H;
-    const int64_t k_blocks = std::min<int64_t>(p.N, (int64_t(p.N) + int64_t(docs) * (kTile - 1)) / kTile) * p.H;
+    const KeyShape ks = key_shape(p);
     auto launch_mode = [&](auto cap, auto slopes) -> int {
         auto *dkv = local_dkv_kernel<T, DIM, decltype(cap)::value, decltype(slopes)::value>;
         auto *dq = local_dq_kernel<T, DIM, decltype(cap)::value, decltype(slopes)::value>;
         FM_CUDA_OK(func_attr_cached((const void *)dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DkvCfg<DIM>::kSmem));
         FM_CUDA_OK(func_attr_cached((const void *)dq, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DqCfg<DIM>::kSmem));
-        dkv<<<unsigned(k_blocks), kThreads, DkvCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, tm_dk, tm_dv, idesc_s, idesc_o);
+        dkv<<<dim3(unsigned(ks.blocks), unsigned(ks.parts)), kThreads, DkvCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, tm_dk, tm_dv, idesc_s, idesc_o, parts);
         FM_LAUNCHED("local_dkv_kernel");
+        if (ks.parts > 1) {
+            local_dkv_join<T, DIM><<<unsigned(ceil_div(int64_t(p.H) * p.N * 32, 256)), 256, 0, st>>>(p, g, parts, ks.parts);
+            FM_LAUNCHED("local_dkv_join");
+        }
         dq<<<unsigned(q_blocks), kThreads, DqCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, tm_dq, idesc_s, idesc_o);
         FM_LAUNCHED("local_dq_kernel");
         return FM_OK;
@@ -712,10 +785,16 @@ template <typename T, int DIM> int launch(const LocalParams &p, const BwdParams 
 
 }  // namespace
 
-int local_tc_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st)
+size_t local_tc_bwd_workspace(const LocalParams &p)
 {
-    if (dtype == FM_BF16) return p.d == 128 ? launch<__nv_bfloat16, 128>(p, g, dtype, st) : launch<__nv_bfloat16, 64>(p, g, dtype, st);
-    return p.d == 128 ? launch<__half, 128>(p, g, dtype, st) : launch<__half, 64>(p, g, dtype, st);
+    const KeyShape s = key_shape(p);
+    return s.parts > 1 ? size_t(s.parts) * 2 * p.H * p.N * p.d * sizeof(float) : 0;
+}
+
+int local_tc_bwd(const LocalParams &p, const BwdParams &g, int dtype, float *parts, cudaStream_t st)
+{
+    if (dtype == FM_BF16) return p.d == 128 ? launch<__nv_bfloat16, 128>(p, g, dtype, parts, st) : launch<__nv_bfloat16, 64>(p, g, dtype, parts, st);
+    return p.d == 128 ? launch<__half, 128>(p, g, dtype, parts, st) : launch<__half, 64>(p, g, dtype, parts, st);
 }
 
 }  // namespace fm

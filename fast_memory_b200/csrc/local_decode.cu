@@ -461,15 +461,20 @@ __global__ void __launch_bounds__(32 * kRows) local_decode_join(const __grid_con
     }
     constexpr int N = D / 32;
     float acc[N] = {}, total = 0.f;
-    if (m > -INFINITY)
-        for (int i = 0; i <= cut.more; ++i) {
-            const float w = expf(part_lse[slot(i)] - m);
-            if (w == 0.f) continue;
-            total += w;
-            const float *src = part_o + slot(i) * D + lane * N;
+    for (int i0 = 0; i0 <= cut.more && m > -INFINITY; i0 += 32) {
+        const int n = min(32, cut.more + 1 - i0);
+        const float mine = lane < n ? expf(part_lse[slot(i0 + lane)] - m) : 0.f;
+        total += mine;
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {                                          // (parts that saw nothing are zero)
+            const float w = __shfl_sync(0xffffffffu, mine, i);
+            const float *src = part_o + slot(i0 + i) * D + lane * N;
 #pragma unroll
             for (int c = 0; c < N; ++c) acc[c] = fmaf(w, src[c], acc[c]);
         }
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     const float inv = total > 0.f ? 1.f / total : 0.f;
     const int64_t row = int64_t(head) * p.S + cut.D.q0 + token;
     T *dst = static_cast<T *>(p.o) + row * D + lane * N;

@@ -120,8 +120,8 @@ __device__ __forceinline__ void mask_scores(uint32_t (&s)[32], int a, int b, int
     for (int c = 0; c < 32; ++c) s[c] = (seen & (1u << c)) ? s[c] : hidden;
 }
 
-// Scores in log2 units after scale, cap and distance (fp: the row's position less the first column's); what is left to multiply
-// is 1.
+// Scores after scale, cap and distance (fp: the row's position less the first column's).  What is left to multiply them with to
+// get log2 units (left_over): the cap if it comes last.
 template <bool CAP, bool SLOPES>
 __device__ __forceinline__ void shape_scores(const LocalParams &p, uint32_t (&s)[32], float slope2, float fp, bool valid)
 {
@@ -130,12 +130,16 @@ __device__ __forceinline__ void shape_scores(const LocalParams &p, uint32_t (&s)
     if constexpr (CAP) cap_scores(t, s, p.scale / p.cap, valid);
 #pragma unroll
     for (int c = 0; c < 16; ++c) {
-        f32x2 e = mul2(CAP ? t[c] : pair(s[2 * c], s[2 * c + 1]), pair(c2, c2));
-        if constexpr (SLOPES) e = fma2(pair(-slope2, -slope2), pair(fabsf(fp - float(2 * c)), fabsf(fp - float(2 * c + 1))), e);
+        f32x2 e = CAP ? t[c] : pair(s[2 * c], s[2 * c + 1]);
+        if constexpr (SLOPES) e = fma2(pair(-slope2, -slope2), pair(fabsf(fp - float(2 * c)), fabsf(fp - float(2 * c + 1))), mul2(e, pair(c2, c2)));
         const float2 v = split(e);
         s[2 * c] = __float_as_uint(v.x);
         s[2 * c + 1] = __float_as_uint(v.y);
     }
+}
+template <bool CAP, bool SLOPES> __device__ __forceinline__ float left_over(const LocalParams &p)
+{
+    return SLOPES ? 1.f : (CAP ? p.cap : p.scale) * kLog2e;
 }
 
 __device__ __forceinline__ float row_max(const uint32_t (&x)[32])
@@ -370,7 +374,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         const int safe_lo = p.window ? shift + b.t1[s] - p.window : 0;         // keys in [safe_lo, safe_hi) are seen by every row
         const int safe_hi = local_run(p, shift + b.t0[s], b.D.nk).y;
         constexpr bool shaped = CAP || SLOPES;
-        const float mul = shaped ? 1.f : p.scale * kLog2e;                     // positive
+        const float mul = left_over<CAP, SLOPES>(p);                           // positive
         const float slope2 = p.slopes && valid ? p.slopes[head] * kLog2e : 0.f;
         const Steps st(b, s);
         float m = -INFINITY, l = 0.f;
@@ -555,7 +559,7 @@ template <typename T, int D> int launch(const LocalParams &p, int dtype, void *w
         FM_LAUNCHED("local_fwd_kernel");
         return FM_OK;
     };
-    const bool slopes = p.slopes || !(p.scale > 0.f);            // the plain form needs scores that grow with the products
+    const bool slopes = p.slopes || (!(p.scale > 0.f) && !(p.cap > 0.f));      // the plain form needs scores that grow with the products
     const int rc = p.cap > 0.f ? (slopes ? launch_mode(std::true_type{}, std::true_type{}) : launch_mode(std::true_type{}, std::false_type{}))
                                : (slopes ? launch_mode(std::false_type{}, std::true_type{}) : launch_mode(std::false_type{}, std::false_type{}));
     if (rc) return rc;

@@ -74,9 +74,16 @@ __device__ __forceinline__ f32x2 exp2_pair(f32x2 x)
     return pair(fast_exp2(v.x), fast_exp2(v.y));
 }
 
-// tanh of a pair, |x| <= 0.7: x + x^3 p(x^2), p of degree 4 with the least error on that range (5e-8 in fp32).
-constexpr float kTanhRange = 0.7f;
-__device__ __forceinline__ f32x2 tanh_small(f32x2 x)
+// tanh of a pair: x + x^3 p(x^2), p the polynomial of least relative error on |x| <= 0.35 (degree 2) or 0.7 (degree 4); 1e-7 and
+// 7e-8 in fp32.
+__device__ __forceinline__ f32x2 tanh_035(f32x2 x)
+{
+    const f32x2 u = mul2(x, x);
+    f32x2 q = fma2(u, pair(-4.91485037e-2f, -4.91485037e-2f), pair(1.32998258e-1f, 1.32998258e-1f));
+    q = fma2(q, u, pair(-3.33326638e-1f, -3.33326638e-1f));
+    return fma2(mul2(x, u), q, x);
+}
+__device__ __forceinline__ f32x2 tanh_070(f32x2 x)
 {
     const f32x2 u = mul2(x, x);
     f32x2 q = fma2(u, pair(-5.13866311e-3f, -5.13866311e-3f), pair(2.00919714e-2f, 2.00919714e-2f));
@@ -93,16 +100,20 @@ __device__ __forceinline__ float tanh_any(float x)
     return fmaf(-2.f, r, 1.f);
 }
 
-// t = tanh(s k).  One formula for the warp: the short one if |s k| allows it in every lane that holds a row (what the others hold
-// must not choose).
+// t = tanh(s k).  One formula for the warp: the shortest that |s k| allows in every lane that holds a row (what the others hold
+// must not choose).  Scores are usually small against their cap.
 __device__ __forceinline__ void cap_scores(f32x2 (&t)[16], const uint32_t (&s)[32], float k, bool valid)
 {
     float big[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < 32; c += 2) big[c >> 1 & 1] = max3(big[c >> 1 & 1], fabsf(__uint_as_float(s[c])), fabsf(__uint_as_float(s[c + 1])));
-    if (__all_sync(0xffffffffu, !valid || fmaxf(big[0], big[1]) * fabsf(k) <= kTanhRange)) {
+    const float top = valid ? fmaxf(big[0], big[1]) * fabsf(k) : 0.f;
+    if (__all_sync(0xffffffffu, top <= 0.35f)) {
 #pragma unroll
-        for (int c = 0; c < 16; ++c) t[c] = tanh_small(mul2(pair(s[2 * c], s[2 * c + 1]), pair(k, k)));
+        for (int c = 0; c < 16; ++c) t[c] = tanh_035(mul2(pair(s[2 * c], s[2 * c + 1]), pair(k, k)));
+    } else if (__all_sync(0xffffffffu, top <= 0.7f)) {
+#pragma unroll
+        for (int c = 0; c < 16; ++c) t[c] = tanh_070(mul2(pair(s[2 * c], s[2 * c + 1]), pair(k, k)));
     } else {
 #pragma unroll
         for (int c = 0; c < 16; ++c) t[c] = pair(tanh_any(__uint_as_float(s[2 * c]) * k), tanh_any(__uint_as_float(s[2 * c + 1]) * k));
@@ -183,7 +194,8 @@ int local_combine(const LocalParams &p, int dtype, const float *part_o, const fl
 // Whether a call goes to the tcgen05 kernels, their launches and tensor maps.
 int local_query_map(CUtensorMap *map, const LocalParams &p, const void *q, int64_t sh, int64_t st, int dtype);
 int local_key_map(CUtensorMap *map, const LocalParams &p, const void *k, int64_t sh, int64_t st, int dtype, int rows = ltc::kTile);
-int local_tc_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st);
+int local_tc_bwd(const LocalParams &p, const BwdParams &g, int dtype, float *parts, cudaStream_t st);
+size_t local_tc_bwd_workspace(const LocalParams &p);        // of `parts`
 int local_tc_fwd(const LocalParams &p, int dtype, void *ws, cudaStream_t st);
 size_t local_tc_fwd_workspace(const LocalParams &p);
 bool local_tc_fits(const LocalParams &p, int dtype);
