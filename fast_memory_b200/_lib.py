@@ -7,7 +7,8 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
+import struct
+from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 import torch
 
@@ -40,10 +41,16 @@ class LocalAttnArgs(ctypes.Structure):
                 [("page_table_width", c_int64), ("n_pages", c_int64), ("page_size", c_int32), ("n_seqs", c_int32)])
 
 
+# the same by position, packed natively: a fraction of the time of filling a Structure, for calls that last microseconds
+pack_local_attn_args = struct.Struct("3P8q7i2f7P2q2i").pack
+
+
 class PageCacheArgs(ctypes.Structure):
     """``fm_page_cache``"""
     _fields_ = ([(n, c_void_p) for n in ("k_pages", "v_pages", "page_table", "lengths", "refcounts", "status")] +
                 [("n_pages", c_int64), ("width", c_int64)] + [(n, c_int32) for n in ("dtype", "d", "n_heads", "page_size", "n_seqs")])
+
+pack_page_cache_args = struct.Struct("6P2q5i").pack
 
 
 _SIGNATURES = {
@@ -91,19 +98,19 @@ _SIGNATURES = {
                           c_size_t, c_void_p]),
     "fm_unit_rows": (c_int, [c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p]),
     "fm_table_scores": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int64, c_void_p, c_void_p, c_void_p, c_void_p]),
-    "fm_local_attn_workspace_bytes": (c_size_t, [POINTER(LocalAttnArgs)]),
-    "fm_local_attn_fwd": (c_int, [POINTER(LocalAttnArgs), c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
-    "fm_local_attn_bwd_workspace_bytes": (c_size_t, [POINTER(LocalAttnArgs)]),
-    "fm_local_attn_bwd": (c_int, [POINTER(LocalAttnArgs), c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+    "fm_local_attn_workspace_bytes": (c_size_t, [c_void_p]),
+    "fm_local_attn_fwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "fm_local_attn_bwd_workspace_bytes": (c_size_t, [c_void_p]),
+    "fm_local_attn_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_size_t, c_void_p]),
-    "fm_page_cache_workspace_bytes": (c_size_t, [POINTER(PageCacheArgs), c_int64]),
-    "fm_cache_append": (c_int, [POINTER(PageCacheArgs), c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
+    "fm_page_cache_workspace_bytes": (c_size_t, [c_void_p, c_int64]),
+    "fm_cache_append": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
                                 c_int64, c_void_p, c_size_t, c_void_p]),
-    "fm_cache_fork": (c_int, [POINTER(PageCacheArgs), c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
-    "fm_cache_free": (c_int, [POINTER(PageCacheArgs), c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
-    "fm_cache_compact": (c_int, [POINTER(PageCacheArgs), c_void_p, c_size_t, c_void_p]),
-    "fm_cache_copy_pages": (c_int, [POINTER(PageCacheArgs), c_void_p, c_void_p, c_int64, c_void_p]),
-    "fm_cache_gather": (c_int, [POINTER(PageCacheArgs), c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "fm_cache_fork": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "fm_cache_free": (c_int, [c_void_p, c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "fm_cache_compact": (c_int, [c_void_p, c_void_p, c_size_t, c_void_p]),
+    "fm_cache_copy_pages": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "fm_cache_gather": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "fm_gather_mean": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
 }
 

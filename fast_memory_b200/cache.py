@@ -14,7 +14,6 @@ sets a bit that :meth:`PagedCache.check` raises for.  Calls on one cache belong 
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -53,30 +52,43 @@ class PagedCache:
 
     def _init(self, k_pages, v_pages, page_table, lengths, refcounts, status):
         dev = L.require_cuda(k_pages, v_pages, page_table, lengths, refcounts, status)
-        if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype:
+        shape = k_pages.shape
+        if len(shape) != 4 or v_pages.shape != shape or v_pages.dtype != k_pages.dtype:
             raise ValueError("k_pages and v_pages must be [n_pages, n_heads, page_size, d] with equal shapes and dtypes")
         if status is None:
             status = torch.zeros(1, dtype=torch.int32, device=dev)
-        for t in (page_table, lengths, refcounts, status):
-            if t.dtype != torch.int32:
-                raise TypeError("page_table, lengths, refcounts and status must be int32")
-        if page_table.dim() != 2 or lengths.shape != page_table.shape[:1] or refcounts.shape != k_pages.shape[:1] or status.numel() != 1:
+        i32 = torch.int32
+        if page_table.dtype is not i32 or lengths.dtype is not i32 or refcounts.dtype is not i32 or status.dtype is not i32:
+            raise TypeError("page_table, lengths, refcounts and status must be int32")
+        if page_table.dim() != 2 or lengths.shape != page_table.shape[:1] or refcounts.shape != shape[:1] or status.numel() != 1:
             raise ValueError("page_table [n_seqs, width], lengths [n_seqs], refcounts [n_pages] and status [1] are needed")
-        for t in (k_pages, v_pages, page_table, lengths, refcounts):
-            if not t.is_contiguous():
-                raise ValueError("the tensors of a cache must be contiguous")
+        if not (k_pages.is_contiguous() and v_pages.is_contiguous() and page_table.is_contiguous() and lengths.is_contiguous() and
+                refcounts.is_contiguous()):
+            raise ValueError("the tensors of a cache must be contiguous")
         self.k_pages, self.v_pages, self.page_table, self.lengths, self.refcounts, self.status = \
             k_pages, v_pages, page_table, lengths, refcounts, status
-        self.n_pages, self.n_heads, self.page_size, self.d = k_pages.shape
-        self.n_seqs = page_table.shape[0]
+        self.n_pages, self.n_heads, self.page_size, self.d = shape
+        self.n_seqs, width = page_table.shape
         self.device = dev
-        self._args = L.PageCacheArgs(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), refcounts.data_ptr(),
-                                     status.data_ptr(), self.n_pages, page_table.shape[1], L.dtype_id(k_pages.dtype), self.d, self.n_heads,
-                                     self.page_size, self.n_seqs)
-        self._ref = ctypes.byref(self._args)
+        self._ref = L.pack_page_cache_args(k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lengths.data_ptr(), refcounts.data_ptr(),
+                                           status.data_ptr(), self.n_pages, width, L.dtype_id(k_pages.dtype), self.d, self.n_heads,
+                                           self.page_size, self.n_seqs)
+        self._ws = {}
 
-    def _workspace(self, n: int) -> torch.Tensor:
-        return _scratch(L.lib().fm_page_cache_workspace_bytes(self._ref, n), self.device)
+    def _run(self, call, *args) -> None:
+        """One page operation on the current stream.  Operations on a cache follow one another, so they share a
+        scratch buffer (one a stream); a captured one gets its own, which lives as long as its graph."""
+        dev, lib = self.device, L.lib()
+        with _on(dev):
+            stream = _stream(dev)
+            ws = self._ws.get(stream)
+            if ws is None or torch.cuda.is_current_stream_capturing():
+                ws = _scratch(lib.fm_page_cache_workspace_bytes(self._ref, self.n_seqs), dev)
+                if not torch.cuda.is_current_stream_capturing():
+                    self._ws[stream] = ws
+            status = call(self._ref, *args, ws.data_ptr(), ws.numel(), stream)
+        if status:
+            L.check(status, call.__name__)
 
     def _seqs(self, seqs: Seqs, name: str = "seqs") -> torch.Tensor:
         t = _int32(seqs, self.device, name)
@@ -104,11 +116,8 @@ class PagedCache:
         if (k_new.shape[1] if cu is None else cu.numel() - 1) != seqs.numel():
             raise ValueError("cu_new must have one entry per sequence plus one (left out: one token per sequence)")
         k_new, v_new = _rows(k_new), _rows(v_new)
-        with _on(dev):
-            ws = self._workspace(seqs.numel())
-            L.check(L.lib().fm_cache_append(self._ref, seqs.data_ptr(), seqs.numel(), L.ptr(cu), k_new.data_ptr(), v_new.data_ptr(),
-                                            k_new.shape[1], k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1),
-                                            ws.data_ptr(), ws.numel(), _stream(dev)), "fm_cache_append")
+        self._run(L.lib().fm_cache_append, seqs.data_ptr(), seqs.numel(), L.ptr(cu), k_new.data_ptr(), v_new.data_ptr(), k_new.shape[1],
+                  k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1))
 
     def fork(self, parents: Seqs, children: Seqs) -> None:
         """The empty sequence ``children[i]`` becomes a copy of ``parents[i]``: full pages are shared, the rows of a last page
@@ -116,24 +125,16 @@ class PagedCache:
         parents, children = _int32(parents, self.device, "parents"), self._seqs(children, "children")
         if parents.numel() != children.numel():
             raise ValueError("parents and children must pair up")
-        with _on(self.device):
-            ws = self._workspace(children.numel())
-            L.check(L.lib().fm_cache_fork(self._ref, parents.data_ptr(), children.data_ptr(), children.numel(), ws.data_ptr(), ws.numel(),
-                                          _stream(self.device)), "fm_cache_fork")
+        self._run(L.lib().fm_cache_fork, parents.data_ptr(), children.data_ptr(), children.numel())
 
     def free(self, seqs: Seqs) -> None:
         """Empty these sequences; pages that no other sequence shares become free."""
         seqs = self._seqs(seqs)
-        with _on(self.device):
-            ws = self._workspace(seqs.numel())
-            L.check(L.lib().fm_cache_free(self._ref, seqs.data_ptr(), seqs.numel(), ws.data_ptr(), ws.numel(), _stream(self.device)),
-                    "fm_cache_free")
+        self._run(L.lib().fm_cache_free, seqs.data_ptr(), seqs.numel())
 
     def compact(self) -> None:
         """Move the used pages to the low end of the pool (the fewest moves that do it); tables follow."""
-        with _on(self.device):
-            ws = self._workspace(0)
-            L.check(L.lib().fm_cache_compact(self._ref, ws.data_ptr(), ws.numel(), _stream(self.device)), "fm_cache_compact")
+        self._run(L.lib().fm_cache_compact)
 
     def copy_pages(self, src: Seqs, dst: Seqs) -> None:
         """Contents of pages ``src[i]`` to ``dst[i]`` (keys and values), tables untouched.  ``dst`` names no page twice and none

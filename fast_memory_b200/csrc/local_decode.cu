@@ -438,13 +438,18 @@ local_decode_kernel(const __grid_constant__ LocalParams p, const __grid_constant
     }
 }
 
-// CTA c joins the item that started in CTA c of the other kernel and went on in the `more` CTAs behind it: a warp a row.
+// CTA c joins the item that started in CTA c of the other kernel and went on in the `more` CTAs behind it.  The warps are dealt out
+// to its rows; those of one row take every n-th part and are added up in their order.
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * kRows) local_decode_join(const __grid_constant__ LocalParams p, const float *part_o, const float *part_lse, const Cut *cuts)
 {
+    __shared__ float sums[kRows][D];
+    __shared__ float totals[kRows];
     const Cut cut = cuts[blockIdx.x];
-    const int r = threadIdx.x >> 5, lane = threadIdx.x & 31, token = cut.t0 + r / p.G, head = cut.h * p.G + r % p.G;
-    if (cut.more == 0 || r >= kRows / p.G * p.G || token >= cut.t1) return;
+    if (cut.more == 0) return;
+    const int rows = (cut.t1 - cut.t0) * p.G, n = kRows / rows;                // warps a row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = warp % rows, mine = warp / rows;
+    const int token = cut.t0 + r / p.G, head = cut.h * p.G + r % p.G;
     auto slot = [&](int i) { return (int64_t(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kRows + r; };
     float m = -INFINITY;
     bool bad = false;
@@ -455,26 +460,33 @@ __global__ void __launch_bounds__(32 * kRows) local_decode_join(const __grid_con
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (__any_sync(0xffffffffu, bad)) {
-        local_row_forward<T, D>(p, cut.D, head, token);
-        return;
-    }
+    bad = __any_sync(0xffffffffu, bad);
     constexpr int N = D / 32;
     float acc[N] = {}, total = 0.f;
-    for (int i0 = 0; i0 <= cut.more && m > -INFINITY; i0 += 32) {
-        const int n = min(32, cut.more + 1 - i0);
-        const float mine = lane < n ? expf(part_lse[slot(i0 + lane)] - m) : 0.f;
-        total += mine;
+    if (mine < n && m > -INFINITY && !bad) {
 #pragma unroll 8
-        for (int i = 0; i < n; ++i) {                                          // (parts that saw nothing are zero)
-            const float w = __shfl_sync(0xffffffffu, mine, i);
-            const float *src = part_o + slot(i0 + i) * D + lane * N;
+        for (int i = mine; i <= cut.more; i += n) {                            // (parts that saw nothing are zero)
+            const float w = expf(part_lse[slot(i)] - m);
+            const float *src = part_o + slot(i) * D + lane * N;
+            total += w;
 #pragma unroll
             for (int c = 0; c < N; ++c) acc[c] = fmaf(w, src[c], acc[c]);
         }
     }
 #pragma unroll
-    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    for (int c = 0; c < N; ++c) sums[warp][lane * N + c] = acc[c];
+    if (lane == 0) totals[warp] = total;
+    __syncthreads();
+    if (mine > 0) return;
+    if (bad) {
+        local_row_forward<T, D>(p, cut.D, head, token);
+        return;
+    }
+    for (int i = 1; i < n; ++i) {
+        total += totals[r + i * rows];
+#pragma unroll
+        for (int c = 0; c < N; ++c) acc[c] += sums[r + i * rows][lane * N + c];
+    }
     const float inv = total > 0.f ? 1.f / total : 0.f;
     const int64_t row = int64_t(head) * p.S + cut.D.q0 + token;
     T *dst = static_cast<T *>(p.o) + row * D + lane * N;

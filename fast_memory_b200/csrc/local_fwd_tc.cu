@@ -522,7 +522,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
 }
 
 // Blocks of query tiles, at most, and the parts that their key tiles are cut into: only where the blocks fill less than half
-// of the SMs, with at least four key tiles a part.
+// of the SMs, with at least two key tiles a part.
 struct Shape {
     int64_t blocks;
     int parts;
@@ -537,7 +537,7 @@ Shape shape_of(const LocalParams &p)
     if (p.window && !p.prefix) keys = std::min<int64_t>(keys, int64_t(p.window) * (p.causal ? 1 : 2) + per);
     const int64_t tiles = ceil_div(keys, ltc::kTile);
     s.parts = 1;
-    if (s.blocks > 0 && s.blocks * 2 <= sm_count()) s.parts = int(std::max<int64_t>(1, std::min<int64_t>(sm_count() / s.blocks, tiles / 4)));
+    if (s.blocks > 0 && s.blocks * 2 <= sm_count()) s.parts = int(std::max<int64_t>(1, std::min<int64_t>(sm_count() / s.blocks, tiles / 2)));
     return s;
 }
 

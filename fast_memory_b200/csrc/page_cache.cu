@@ -19,6 +19,9 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kCopyThreads = 256;
+// 16-byte pieces (of K; V has as many) that the plan's CTA copies itself: 64 KB take it about 1.5 us, a launch of its own costs the
+// host 2.5 us and the device as much.
+constexpr int64_t kFewPieces = 2048;
 
 struct Cache {
     char *k, *v;
@@ -169,9 +172,54 @@ __device__ __forceinline__ void finish(const Cache &c, PlanHead *head, int count
     }
 }
 
-__global__ void __launch_bounds__(kPlanThreads) cache_append_plan(Cache c, const int32_t *seqs, const int32_t *cu, int n, int tokens, void *ws)
+// What is appended: rows of k and v, strides in bytes.
+struct NewRows {
+    const int32_t *seqs, *cu;
+    const char *k, *v;
+    int64_t k_sh, k_st, v_sh, v_st;
+    int n, tokens;
+};
+
+// 32 tokens from t0 on and head h: their places are looked up once, then 16-byte pieces go side by side.  By a whole CTA.
+__device__ __forceinline__ void append_rows(const Cache &c, const PlanWs &w, const NewRows &a, int t0, int h, int64_t *to)
+{
+    if (threadIdx.x < 32) {
+        const int t = t0 + threadIdx.x;
+        int64_t row = -1;
+        if (t < (a.cu ? min(a.tokens, a.cu[a.n]) : a.tokens)) {
+            const int i = a.cu ? find_item(a.cu, a.n, t) : t;
+            const int at = w.start[i] + t - (a.cu ? a.cu[i] : i);
+            const int page = c.table[int64_t(a.seqs[i]) * c.width + (at >> c.shift)];
+            if (page >= 0 && page < c.n_pages) row = ((int64_t(page) * c.heads + h) << c.shift) + (at & ((1 << c.shift) - 1));
+        }
+        to[threadIdx.x] = row;
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < 32 * c.row16; x += blockDim.x) {
+        const int t = x / c.row16, o = x % c.row16;
+        const int64_t row = to[t];
+        if (row < 0) continue;
+        const uint4 k = *reinterpret_cast<const uint4 *>(a.k + h * a.k_sh + (t0 + t) * a.k_st + o * 16);
+        const uint4 v = *reinterpret_cast<const uint4 *>(a.v + h * a.v_sh + (t0 + t) * a.v_st + o * 16);
+        *reinterpret_cast<uint4 *>(c.k + (row * c.row16 + o) * 16) = k;
+        *reinterpret_cast<uint4 *>(c.v + (row * c.row16 + o) * 16) = v;
+    }
+}
+
+__global__ void __launch_bounds__(kCopyThreads) cache_append_rows(Cache c, NewRows a, void *ws)
+{
+    __shared__ int64_t to[32];
+    const PlanWs w = plan_ws(ws, c.n_seqs, a.n);
+    if (w.head->go) append_rows(c, w, a, blockIdx.x * 32, blockIdx.y, to);
+}
+
+// copy: the rows as well, where they are so few that another launch would take longer
+__global__ void __launch_bounds__(kPlanThreads) cache_append_plan(Cache c, NewRows a, void *ws, bool copy)
 {
     __shared__ int warp_sums[32], err;
+    __shared__ int64_t to[32];
+    const int32_t *seqs = a.seqs, *cu = a.cu;
+    const int n = a.n, tokens = a.tokens;
     const PlanWs w = plan_ws(ws, c.n_seqs, n);
     clear_marks(c, w, &err);
     const int total = scan_needs(n, w.off, warp_sums, [&](int i) {
@@ -190,42 +238,40 @@ __global__ void __launch_bounds__(kPlanThreads) cache_append_plan(Cache c, const
             c.refs[page] = 1;
         }
         for (int i = threadIdx.x; i < n; i += kPlanThreads) c.lengths[seqs[i]] = w.start[i] + (cu ? cu[i + 1] - cu[i] : 1);
+        if (copy) {
+            __syncthreads();
+            for (int t = 0; t < tokens; t += 32)
+                for (int h = 0; h < c.heads; ++h) {
+                    append_rows(c, w, a, t, h, to);
+                    __syncthreads();
+                }
+        }
     }
     finish(c, w.head, n, &err);
 }
 
-// 32 tokens a CTA and one head (blockIdx.y): their places are looked up once, then 16-byte pieces go side by side.
-__global__ void __launch_bounds__(kCopyThreads) cache_append_rows(Cache c, const int32_t *seqs, const int32_t *cu, int n, int tokens, const char *k_new,
-                                                                  const char *v_new, int64_t k_sh, int64_t k_st, int64_t v_sh, int64_t v_st, void *ws)
+// The rows of item i's partial page, head h, K or V: one contiguous run.  By the threads `first`, `first` + `step` ...
+__device__ __forceinline__ void fork_rows(const Cache &c, const PlanWs &w, int i, int h, bool v, int first, int step)
 {
-    __shared__ int64_t to[32];
-    const PlanWs w = plan_ws(ws, c.n_seqs, n);
-    if (!w.head->go) return;
-    const int t0 = blockIdx.x * 32, h = blockIdx.y;
-    if (threadIdx.x < 32) {
-        const int t = t0 + threadIdx.x;
-        int64_t row = -1;
-        if (t < (cu ? min(tokens, cu[n]) : tokens)) {
-            const int i = cu ? find_item(cu, n, t) : t;
-            const int at = w.start[i] + t - (cu ? cu[i] : i);
-            const int page = c.table[int64_t(seqs[i]) * c.width + (at >> c.shift)];
-            if (page >= 0 && page < c.n_pages) row = ((int64_t(page) * c.heads + h) << c.shift) + (at & ((1 << c.shift) - 1));
-        }
-        to[threadIdx.x] = row;
-    }
-    __syncthreads();
-    for (int x = threadIdx.x; x < 32 * c.row16; x += kCopyThreads) {
-        const int t = x / c.row16, o = x % c.row16;
-        const int64_t row = to[t];
-        if (row < 0) continue;
-        const uint4 a = *reinterpret_cast<const uint4 *>(k_new + h * k_sh + (t0 + t) * k_st + o * 16);
-        const uint4 b = *reinterpret_cast<const uint4 *>(v_new + h * v_sh + (t0 + t) * v_st + o * 16);
-        *reinterpret_cast<uint4 *>(c.k + (row * c.row16 + o) * 16) = a;
-        *reinterpret_cast<uint4 *>(c.v + (row * c.row16 + o) * 16) = b;
-    }
+    const int rows = w.start[i] & ((1 << c.shift) - 1);
+    if (rows == 0) return;
+    const int src = w.src[i], dst = w.alloc[w.off[i]];
+    if (src < 0 || src >= c.n_pages) return;
+    uint4 *pool = reinterpret_cast<uint4 *>(v ? c.v : c.k);
+    const uint4 *from = pool + ((int64_t(src) * c.heads + h) << c.shift) * c.row16;
+    uint4 *to = pool + ((int64_t(dst) * c.heads + h) << c.shift) * c.row16;
+#pragma unroll 4
+    for (int x = first; x < rows * c.row16; x += step) to[x] = from[x];
 }
 
-__global__ void __launch_bounds__(kPlanThreads) cache_fork_plan(Cache c, const int32_t *parents, const int32_t *children, int n, void *ws)
+__global__ void __launch_bounds__(kCopyThreads) cache_fork_rows(Cache c, int n, void *ws)
+{
+    const PlanWs w = plan_ws(ws, c.n_seqs, n);
+    if (w.head->go) fork_rows(c, w, blockIdx.x, blockIdx.y, blockIdx.z, threadIdx.x, kCopyThreads);
+}
+
+// copy: the rows as well, a warp a run, where they are so few that another launch would take longer
+__global__ void __launch_bounds__(kPlanThreads) cache_fork_plan(Cache c, const int32_t *parents, const int32_t *children, int n, void *ws, bool copy)
 {
     __shared__ int warp_sums[32], err;
     const PlanWs w = plan_ws(ws, c.n_seqs, n);
@@ -259,24 +305,12 @@ __global__ void __launch_bounds__(kPlanThreads) cache_fork_plan(Cache c, const i
             }
             if ((threadIdx.x & 31) == 0) c.lengths[children[i]] = len;
         }
+        if (copy) {
+            __syncthreads();
+            for (int x = threadIdx.x >> 5; x < 2 * n * c.heads; x += kPlanWarps) fork_rows(c, w, x / (2 * c.heads), x / 2 % c.heads, x & 1, threadIdx.x & 31, 32);
+        }
     }
     finish(c, w.head, n, &err);
-}
-
-// The rows of the partial pages: CTA (item, head, K or V) copies one contiguous run.
-__global__ void __launch_bounds__(kCopyThreads) cache_fork_rows(Cache c, int n, void *ws)
-{
-    const PlanWs w = plan_ws(ws, c.n_seqs, n);
-    if (!w.head->go) return;
-    const int i = blockIdx.x, h = blockIdx.y;
-    const int rows = w.start[i] & ((1 << c.shift) - 1);
-    if (rows == 0) return;
-    const int src = w.src[i], dst = w.alloc[w.off[i]];
-    if (src < 0 || src >= c.n_pages) return;
-    char *pool = blockIdx.z ? c.v : c.k;
-    const uint4 *from = reinterpret_cast<const uint4 *>(pool) + ((int64_t(src) * c.heads + h) << c.shift) * c.row16;
-    uint4 *to = reinterpret_cast<uint4 *>(pool) + ((int64_t(dst) * c.heads + h) << c.shift) * c.row16;
-    for (int x = threadIdx.x; x < rows * c.row16; x += kCopyThreads) to[x] = from[x];
 }
 
 __global__ void __launch_bounds__(kPlanThreads) cache_free_plan(Cache c, const int32_t *seqs, int n, void *ws)
@@ -468,13 +502,13 @@ int fm_cache_append(const fm_page_cache *a, const int32_t *seqs, int64_t n, cons
                ((k_stride_head | k_stride_row | v_stride_head | v_stride_row) * e) % 16 == 0, "fm_cache_append: rows must start on 16-byte boundaries");
     if (int rc = check_ws(a, n, workspace, workspace_bytes, "fm_cache_append")) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cache_append_plan<<<1, kPlanThreads, 0, st>>>(c, seqs, cu_new, int(n), int(n_tokens), workspace);
+    const NewRows rows{seqs, cu_new, static_cast<const char *>(k_new), static_cast<const char *>(v_new), k_stride_head * e, k_stride_row * e,
+                       v_stride_head * e, v_stride_row * e, int(n), int(n_tokens)};
+    const bool copy = n_tokens * c.heads * c.row16 <= kFewPieces;
+    cache_append_plan<<<1, kPlanThreads, 0, st>>>(c, rows, workspace, copy);
     FM_LAUNCHED("cache_append_plan");
-    if (n_tokens > 0) {
-        const dim3 grid(unsigned(ceil_div(n_tokens, 32)), unsigned(c.heads));
-        cache_append_rows<<<grid, kCopyThreads, 0, st>>>(c, seqs, cu_new, int(n), int(n_tokens), static_cast<const char *>(k_new),
-                                                         static_cast<const char *>(v_new), k_stride_head * e, k_stride_row * e, v_stride_head * e,
-                                                         v_stride_row * e, workspace);
+    if (n_tokens > 0 && !copy) {
+        cache_append_rows<<<dim3(unsigned(ceil_div(n_tokens, 32)), unsigned(c.heads)), kCopyThreads, 0, st>>>(c, rows, workspace);
         FM_LAUNCHED("cache_append_rows");
     }
     return FM_OK;
@@ -491,10 +525,13 @@ int fm_cache_fork(const fm_page_cache *a, const int32_t *parents, const int32_t 
     FM_REQUIRE(parents && children, "fm_cache_fork: null pointer");
     if (int rc = check_ws(a, n, workspace, workspace_bytes, "fm_cache_fork")) return rc;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    cache_fork_plan<<<1, kPlanThreads, 0, st>>>(c, parents, children, int(n), workspace);
+    const bool copy = ((n * c.heads) << c.shift) * c.row16 <= kFewPieces;
+    cache_fork_plan<<<1, kPlanThreads, 0, st>>>(c, parents, children, int(n), workspace, copy);
     FM_LAUNCHED("cache_fork_plan");
-    cache_fork_rows<<<dim3(unsigned(n), unsigned(c.heads), 2), kCopyThreads, 0, st>>>(c, int(n), workspace);
-    FM_LAUNCHED("cache_fork_rows");
+    if (!copy) {
+        cache_fork_rows<<<dim3(unsigned(n), unsigned(c.heads), 2), kCopyThreads, 0, st>>>(c, int(n), workspace);
+        FM_LAUNCHED("cache_fork_rows");
+    }
     return FM_OK;
 }
 

@@ -18,7 +18,6 @@ holds (NaN included).
 from __future__ import annotations
 
 import contextlib
-import ctypes
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -43,11 +42,14 @@ def _int32(values: Optional[Prefix], dev: torch.device, name: str, count: Option
     if values is None:
         return None
     if isinstance(values, torch.Tensor):
+        if values.dtype is torch.int32 and values.dim() == 1 and values.device == dev and values.is_contiguous() and \
+                (count is None or values.numel() == count):
+            return values                                     # the usual case
         if values.dim() != 1 or values.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"{name} must be a 1-d int32 or int64 tensor")
         if values.device != dev:
             raise ValueError(f"{name} is on {values.device}, the tensors are on {dev}")
-        t = values if values.dtype is torch.int32 and values.is_contiguous() else values.to(torch.int32).contiguous()
+        t = values.to(torch.int32).contiguous()
     else:
         t = torch.tensor([int(x) for x in values], dtype=torch.int32, device=dev)
     if count is not None and t.numel() != count:
@@ -106,12 +108,15 @@ def _on(dev: torch.device):
     return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
-def _doc_args(q, k, v, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, prefix):
-    return L.LocalAttnArgs(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-        q.shape[1], k.shape[1], L.dtype_id(q.dtype), q.shape[2], q.shape[0], k.shape[0], 1 if cu_q is None else cu_q.numel() - 1,
-        int(window), int(causal), float(sm_scale), float(softcap), L.ptr(cu_q), L.ptr(cu_k), L.ptr(prefix), L.ptr(slopes), None, None, None,
-        0, 0, 0, 0)
+def _doc_args(q, k, v, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, prefix) -> bytes:
+    """``fm_local_attn_args`` of a call over documents."""
+    (qh, qs, _), (kh, ks, _), (vh, vs, _) = q.stride(), k.stride(), v.stride()
+    Hq, S, d = q.shape
+    H, N, _ = k.shape
+    return L.pack_local_attn_args(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), qh, qs, kh, ks, vh, vs, S, N, L.dtype_id(q.dtype), d, Hq, H,
+        1 if cu_q is None else cu_q.numel() - 1, int(window), 1 if causal else 0, float(sm_scale), float(softcap), L.ptr(cu_q), L.ptr(cu_k),
+        L.ptr(prefix), L.ptr(slopes), 0, 0, 0, 0, 0, 0, 0)
 
 
 def _stream(dev: torch.device) -> int:
@@ -124,16 +129,17 @@ def _scratch(nbytes: int, dev: torch.device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
-def _forward(args: L.LocalAttnArgs, q: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+def _forward(args: bytes, q: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     dev = q.device
     o = q.new_empty(q.shape)
     lse = q.new_empty(q.shape[:2], dtype=torch.float32)
-    lib, ref = L.lib(), ctypes.byref(args)
+    lib = L.lib()
     with _on(dev):
-        nbytes = lib.fm_local_attn_workspace_bytes(ref)
+        nbytes = lib.fm_local_attn_workspace_bytes(args)
         ws = _scratch(nbytes, dev)
-        status = lib.fm_local_attn_fwd(ref, o.data_ptr(), lse.data_ptr(), L.ptr(ws), nbytes, _stream(dev))
-    L.check(status, "fm_local_attn_fwd")
+        status = lib.fm_local_attn_fwd(args, o.data_ptr(), lse.data_ptr(), L.ptr(ws), nbytes, _stream(dev))
+    if status:
+        L.check(status, "fm_local_attn_fwd")
     return o, lse
 
 
@@ -149,13 +155,14 @@ def _local_bwd(q, k, v, out, lse, d_out, d_lse, sm_scale, causal, window, softca
     dev = q.device
     dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
     args = _doc_args(q, k, v, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, prefix)
-    lib, ref = L.lib(), ctypes.byref(args)
+    lib = L.lib()
     with _on(dev):
-        nbytes = lib.fm_local_attn_bwd_workspace_bytes(ref)
+        nbytes = lib.fm_local_attn_bwd_workspace_bytes(args)
         ws = _scratch(nbytes, dev)
-        status = lib.fm_local_attn_bwd(ref, out.data_ptr(), lse.data_ptr(), d_out.data_ptr(), d_out.stride(0), d_out.stride(1),
+        status = lib.fm_local_attn_bwd(args, out.data_ptr(), lse.data_ptr(), d_out.data_ptr(), d_out.stride(0), d_out.stride(1),
                                        L.ptr(d_lse), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), L.ptr(ws), nbytes, _stream(dev))
-    L.check(status, "fm_local_attn_bwd")
+    if status:
+        L.check(status, "fm_local_attn_bwd")
     return dq, dk, dv
 
 
@@ -304,8 +311,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if pieces == 0:
         return torch.empty_like(q), torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
     q = _rows(q)
-    args = L.LocalAttnArgs(
+    args = L.pack_local_attn_args(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q.stride(0), q.stride(1), 0, 0, 0, 0, q.shape[1], 0, L.dtype_id(q.dtype), d,
-        q.shape[0], H, pieces, int(window), int(causal), float(sm_scale), float(softcap), L.ptr(cu_q), None, L.ptr(prefix), L.ptr(slopes),
+        q.shape[0], H, pieces, int(window), 1 if causal else 0, float(sm_scale), float(softcap), L.ptr(cu_q), 0, L.ptr(prefix), L.ptr(slopes),
         page_table.data_ptr(), lengths.data_ptr(), L.ptr(seqs), page_table.shape[1], n_pages, page, page_table.shape[0])
     return _forward(args, q)
