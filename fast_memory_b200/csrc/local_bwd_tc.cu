@@ -74,9 +74,9 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
     const int tokens = kTile / p.G, rows = tokens * p.G;
 
     if (warp == 0) {
-        const int nb = gridDim.x / p.H, h = blockIdx.x / nb;
+        const int h = blockIdx.x % p.H;
         Doc doc;
-        const int index = find_block<true>(p, kTile, blockIdx.x % nb, doc);
+        const int index = find_block<true>(p, kTile, blockIdx.x / p.H, doc);   // (the most queries first)
         if (lane == 0) {
             sh.h = h;
             sh.n_q = 0;
@@ -483,9 +483,9 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
     const int tokens = kTile / p.G, rows = tokens * p.G;
 
     if (warp == 0) {
-        const int nb = gridDim.x / p.H, h = blockIdx.x / nb;
+        const int nb = gridDim.x / p.H, h = blockIdx.x % p.H;
         Doc doc;
-        const int index = find_block<false>(p, tokens, nb - 1 - int(blockIdx.x % nb), doc);   // (the most keys first)
+        const int index = find_block<false>(p, tokens, nb - 1 - int(blockIdx.x / p.H), doc);   // (the most keys first)
         if (lane == 0) {
             sh.h = h;
             sh.t0 = sh.t1 = sh.n_pre = sh.lo = sh.n_k = 0;

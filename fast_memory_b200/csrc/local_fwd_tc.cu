@@ -224,9 +224,9 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         // the last blocks of a document have the most keys (causal): they go first
         const int nb = gridDim.x / p.H;
         Doc doc;
-        const int index = find_block<false>(p, 2 * (kTile / p.G), nb - 1 - int(blockIdx.x % nb), doc);
+        const int index = find_block<false>(p, 2 * (kTile / p.G), nb - 1 - int(blockIdx.x / p.H), doc);
         if (lane == 0) {
-            if (index >= 0) make_block(p, sh.b, doc, index, blockIdx.x / nb, blockIdx.y, gridDim.y);
+            if (index >= 0) make_block(p, sh.b, doc, index, blockIdx.x % p.H, blockIdx.y, gridDim.y);
             else sh.b = Block{};
         }
         __syncwarp();

@@ -149,7 +149,11 @@ template <typename T> __device__ __forceinline__ bool put_row(const uint32_t (&o
 __device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // Blocks of `per` rows, document by document (`KEYS`: of keys, else of queries): the document of block number `b` and which of its
-// blocks that is (-1: there is no such block).  Called by one whole warp; every lane gets the answer.
+// blocks that is (-1: there is no such block).  Called by one whole warp; every lane gets the answer.  Documents come, 32 at
+// a time, in the order of what a block of theirs costs: blocks of keys by falling number of queries, blocks of queries by rising
+// number of keys (they are handed out from the last one).  The grids have the KV head as their fastest index: then the long
+// blocks of every head run first and the short ones fill the gaps at the end.  (One head after the other, 8192 tokens with a window of
+// 4096 waited 13 % longer for the last key block, 8 % for the last query block.)
 template <bool KEYS> __device__ __forceinline__ int find_block(const LocalParams &p, int per, int b, Doc &doc)
 {
     const int lane = threadIdx.x & 31;
@@ -158,7 +162,20 @@ template <bool KEYS> __device__ __forceinline__ int find_block(const LocalParams
         const int t = t0 + lane;
         Doc D = {};
         if (t <= p.n_docs) D = local_doc<KEYS>(p, t);
-        const int n = ((KEYS ? D.nk : D.nq) + per - 1) / per;
+        int n = ((KEYS ? D.nk : D.nq) + per - 1) / per, from = lane;             // from: the lane that has this place's document
+        if (p.n_docs > 1) {
+            const int cost = KEYS ? -D.nq : D.nk;
+            int rank = 0;
+#pragma unroll
+            for (int l = 0; l < 32; ++l) {
+                const int other = __shfl_sync(0xffffffffu, cost, l);
+                rank += other < cost || (other == cost && l < lane);
+            }
+#pragma unroll
+            for (int l = 0; l < 32; ++l)
+                if (__shfl_sync(0xffffffffu, rank, l) == lane) from = l;
+            n = __shfl_sync(0xffffffffu, n, from);
+        }
         int s = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -167,14 +184,14 @@ template <bool KEYS> __device__ __forceinline__ int find_block(const LocalParams
         }
         const int total = __shfl_sync(0xffffffffu, s, 31);
         if (b < before + total) {
-            const int l = __ffs(__ballot_sync(0xffffffffu, b < before + s)) - 1;
+            const int at = __ffs(__ballot_sync(0xffffffffu, b < before + s)) - 1, l = __shfl_sync(0xffffffffu, from, at);
             doc.q0 = __shfl_sync(0xffffffffu, D.q0, l);
             doc.nq = __shfl_sync(0xffffffffu, D.nq, l);
             doc.k0 = __shfl_sync(0xffffffffu, D.k0, l);
             doc.nk = __shfl_sync(0xffffffffu, D.nk, l);
             doc.prefix = __shfl_sync(0xffffffffu, D.prefix, l);
             doc.seq = __shfl_sync(0xffffffffu, D.seq, l);
-            return b - before - __shfl_sync(0xffffffffu, s - n, l);
+            return b - before - __shfl_sync(0xffffffffu, s - n, at);
         }
         before += total;
     }
