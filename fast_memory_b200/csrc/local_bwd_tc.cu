@@ -51,7 +51,7 @@ template <int DIM> struct DkvShared {
     int abort;
     int h, j0, q_lo, n_q;                                        // head, first key, first query tile, query tiles
     Doc D;
-    alignas(16) float lse2[2][kTile], delta[2][kTile];           // both negated
+    alignas(16) float lse2[2][kTile], delta[2][kTile];           // negated; delta too if there is no cap
     alignas(16) float slope2[kTile], place[kTile];               // negated slope; token of a column, from the tile's first
     alignas(16) int token[kTile];
 };
@@ -197,7 +197,7 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                         delta = g.delta[int64_t(head) * p.S + D.q0 + token];
                     }
                     sh.lse2[buf][r] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;          // no such row, or one that sees nothing: P = 0
-                    sh.delta[buf][r] = -delta;
+                    sh.delta[buf][r] = CAP ? delta : -delta;
                     if (i == 0 && p.slopes && r < rows) sh.slope2[r] = -p.slopes[head] * kLog2e;
                 }
                 __syncwarp();
@@ -257,7 +257,7 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
             all = make_int2(local_query_run(p, D, last).x, local_query_run(p, D, max(j0, min(D.prefix, last))).y);
         }
         const f32x2 scale2 = pair(p.scale * kLog2e, p.scale * kLog2e), c2 = pair(p.cap * kLog2e, p.cap * kLog2e);
-        const f32x2 minus = pair(-1.f, -1.f), one = pair(1.f, 1.f);
+        const f32x2 minus = pair(-1.f, -1.f);
         const float kc = p.cap > 0.f ? p.scale / p.cap : 0.f;
         bool ok = true;
         for (int i = 0; i < n_q; ++i) {
@@ -268,7 +268,7 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                  tc::mbar_wait_or_abort(bar_addr(&sh.s_full), i & 1, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after_sync();
-            f32x2 pr[32];                                        // P, times the derivative of the cap
+            f32x2 pr[32];                                        // P; with a cap, P times its derivative, negated (tanh^2 - 1: one operation)
             unsigned seen[2] = {0xffffffffu, 0xffffffffu};
             if (masked) {
 #pragma unroll
@@ -306,7 +306,7 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                             w.y = (seen[x] >> (2 * c + 1) & 1u) ? w.y : 0.f;
                         }
                         pk[c] = pack2<T>(w.x, w.y);
-                        pr[x * 16 + c] = CAP ? mul2(pair(w.x, w.y), fma2(mul2(t[c], minus), t[c], one)) : pair(w.x, w.y);
+                        pr[x * 16 + c] = CAP ? mul2(pair(w.x, w.y), fma2(t[c], t[c], minus)) : pair(w.x, w.y);
                     }
                     tc::tmem_st_x16(t_s + x * 16, pk);
                 }
@@ -330,7 +330,8 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
                         const f32x2 n = (c & 1) ? delta[c >> 1].y : delta[c >> 1].x;
-                        float2 w = split(mul2(pr[x * 16 + c], add2(pair(s[2 * c], s[2 * c + 1]), n)));
+                        const f32x2 dp = pair(s[2 * c], s[2 * c + 1]);
+                        float2 w = split(mul2(pr[x * 16 + c], CAP ? fma2(dp, minus, n) : add2(dp, n)));
                         if constexpr (decltype(with_mask)::value) {          // P = 0 is not enough: dP may be NaN there
                             w.x = (seen[x] >> (2 * c) & 1u) ? w.x : 0.f;
                             w.y = (seen[x] >> (2 * c + 1) & 1u) ? w.y : 0.f;
@@ -621,8 +622,8 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
         const int pre = valid ? D.prefix : 0;
         const int safe_lo = p.window ? shift + t1 - p.window : 0, safe_hi = n_k > 0 ? local_run(p, shift + t0, D.nk).y : 0;
         const f32x2 scale2 = pair(p.scale * kLog2e, p.scale * kLog2e), c2 = pair(p.cap * kLog2e, p.cap * kLog2e);
-        const f32x2 minus = pair(-1.f, -1.f), one = pair(1.f, 1.f);
-        const f32x2 nlse = pair(-lse2, -lse2), ndelta = pair(-delta, -delta), nslope = pair(-slope2, -slope2);
+        const f32x2 minus = pair(-1.f, -1.f);
+        const f32x2 nlse = pair(-lse2, -lse2), sdelta = CAP ? pair(delta, delta) : pair(-delta, -delta), nslope = pair(-slope2, -slope2);
         const float kc = p.cap > 0.f ? p.scale / p.cap : 0.f;
         bool ok = true;
         for (int n = 0; n < n_k; ++n) {
@@ -632,7 +633,7 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
             ok = tc::mbar_wait_or_abort(bar_addr(&sh.s_full[b]), (n >> 1) & 1, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after_sync();
-            f32x2 pr[32];                                        // P, times the derivative of the cap
+            f32x2 pr[32];                                        // P; with a cap, P times its derivative, negated (tanh^2 - 1: one operation)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 uint32_t s[32];
@@ -648,7 +649,7 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
                         e = fma2(nslope, pair(fabsf(d), fabsf(d - 1.f)), e);
                     }
                     e = exp2_pair(e);
-                    pr[x * 16 + c] = CAP ? mul2(e, fma2(mul2(t[c], minus), t[c], one)) : e;
+                    pr[x * 16 + c] = CAP ? mul2(e, fma2(t[c], t[c], minus)) : e;
                 }
             }
             ok = tc::mbar_wait_or_abort(bar_addr(&sh.dp_full), n & 1, abort_flag);
@@ -663,7 +664,8 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
                     const int a = run.x - col0 - x * 32, e = run.y - col0 - x * 32, q = pre - col0 - x * 32;
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
-                        float2 w = split(mul2(pr[x * 16 + c], add2(pair(s[2 * c], s[2 * c + 1]), ndelta)));
+                        const f32x2 dp = pair(s[2 * c], s[2 * c + 1]);
+                        float2 w = split(mul2(pr[x * 16 + c], CAP ? fma2(dp, minus, sdelta) : add2(dp, sdelta)));
                         if constexpr (decltype(with_mask)::value) {
                             const int i = 2 * c;
                             if (!((i >= a && i < e) || i < q)) w.x = 0.f;

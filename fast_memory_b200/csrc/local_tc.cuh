@@ -74,24 +74,24 @@ __device__ __forceinline__ f32x2 exp2_pair(f32x2 x)
     return pair(fast_exp2(v.x), fast_exp2(v.y));
 }
 
-// tanh of a pair: x + x^3 p(x^2), p the polynomial of least relative error on |x| <= 0.35 (degree 2) or 0.7 (degree 4); 1e-7 and
-// 7e-8 in fp32.
-__device__ __forceinline__ f32x2 tanh_035(f32x2 x)
-{
-    const f32x2 u = mul2(x, x);
-    f32x2 q = fma2(u, pair(-4.91485037e-2f, -4.91485037e-2f), pair(1.32998258e-1f, 1.32998258e-1f));
-    q = fma2(q, u, pair(-3.33326638e-1f, -3.33326638e-1f));
-    return fma2(mul2(x, u), q, x);
-}
-__device__ __forceinline__ f32x2 tanh_070(f32x2 x)
-{
-    const f32x2 u = mul2(x, x);
-    f32x2 q = fma2(u, pair(-5.13866311e-3f, -5.13866311e-3f), pair(2.00919714e-2f, 2.00919714e-2f));
-    q = fma2(q, u, pair(-5.35588600e-2f, -5.35588600e-2f));
-    q = fma2(q, u, pair(1.33291110e-1f, 1.33291110e-1f));
-    q = fma2(q, u, pair(-3.33331913e-1f, -3.33331913e-1f));
-    return fma2(mul2(x, u), q, x);
-}
+// tanh(k s) for |k s| <= 0.4: s (k + k^3 s^2 p(k^2 s^2)), p the polynomial of degree 2 of least relative error, 2e-7 in fp32.  k is
+// multiplied into the coefficients: five operations a pair.
+struct ShortTanh {
+    f32x2 k, c0, c1, c2;
+    __device__ __forceinline__ ShortTanh(float x)
+    {
+        const float x2 = x * x, x3 = x * x2, x5 = x3 * x2, x7 = x5 * x2;
+        k = pair(x, x);
+        c0 = pair(-0.333318823f * x3, -0.333318823f * x3);
+        c1 = pair(0.13277629f * x5, 0.13277629f * x5);
+        c2 = pair(-0.0477942206f * x7, -0.0477942206f * x7);
+    }
+    __device__ __forceinline__ f32x2 operator()(f32x2 s) const
+    {
+        const f32x2 u = mul2(s, s);
+        return mul2(s, fma2(fma2(fma2(c2, u, c1), u, c0), u, k));
+    }
+};
 // tanh x = 1 - 2 / (1 + e^2x): e^2x = inf gives 1, 0 gives -1
 __device__ __forceinline__ float tanh_any(float x)
 {
@@ -100,20 +100,19 @@ __device__ __forceinline__ float tanh_any(float x)
     return fmaf(-2.f, r, 1.f);
 }
 
-// t = tanh(s k).  One formula for the warp: the shortest that |s k| allows in every lane that holds a row (what the others hold
-// must not choose).  Scores are usually small against their cap.
+// t = tanh(s k), k > 0.  One formula for the warp, the short one if |s k| allows it in every lane that holds a row (what the others
+// hold must not choose) and the powers of k stay in fp32's range.  Scores are usually small against their cap.  More tiers, a shorter
+// one up to 0.2 or a longer one up to 0.7, cost more in code than they save: chunked prompts 860 us, with this one alone 770.
 __device__ __forceinline__ void cap_scores(f32x2 (&t)[16], const uint32_t (&s)[32], float k, bool valid)
 {
     float big[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < 32; c += 2) big[c >> 1 & 1] = max3(big[c >> 1 & 1], fabsf(__uint_as_float(s[c])), fabsf(__uint_as_float(s[c + 1])));
-    const float top = valid ? fmaxf(big[0], big[1]) * fabsf(k) : 0.f;
-    if (__all_sync(0xffffffffu, top <= 0.35f)) {
+    const float top = valid ? fmaxf(big[0], big[1]) * ((k >= 0x1p-12f && k <= 0x1p12f) ? k : INFINITY) : 0.f;
+    if (__all_sync(0xffffffffu, top <= 0.4f)) {
+        const ShortTanh tanh_pair(k);
 #pragma unroll
-        for (int c = 0; c < 16; ++c) t[c] = tanh_035(mul2(pair(s[2 * c], s[2 * c + 1]), pair(k, k)));
-    } else if (__all_sync(0xffffffffu, top <= 0.7f)) {
-#pragma unroll
-        for (int c = 0; c < 16; ++c) t[c] = tanh_070(mul2(pair(s[2 * c], s[2 * c + 1]), pair(k, k)));
+        for (int c = 0; c < 16; ++c) t[c] = tanh_pair(pair(s[2 * c], s[2 * c + 1]));
     } else {
 #pragma unroll
         for (int c = 0; c < 16; ++c) t[c] = pair(tanh_any(__uint_as_float(s[2 * c]) * k), tanh_any(__uint_as_float(s[2 * c + 1]) * k));
