@@ -153,7 +153,7 @@ static int local_params(const fm_local_attn_args *a, LocalParams &p)
     FM_REQUIRE(a->n_kv_heads > 0 && a->n_q_heads > 0 && a->n_q_heads % a->n_kv_heads == 0,
                "local attention: %d query heads do not share %d KV heads evenly", a->n_q_heads, a->n_kv_heads);
     FM_REQUIRE(a->n_docs > 0 && a->window >= 0, "local attention: bad document count %d or window %d", a->n_docs, a->window);
-    FM_REQUIRE(a->softcap >= 0.f, "local attention: the cap must not be negative");
+    FM_REQUIRE(a->softcap >= 0.f && a->softcap < INFINITY, "local attention: the cap must be finite and not negative");
     FM_REQUIRE(int64_t(a->n_q_heads) * a->n_q_rows < (int64_t(1) << 31) && int64_t(a->n_kv_heads) * a->n_k_rows < (int64_t(1) << 31),
                "local attention: more than 2^31 rows over all heads");
     if (a->d != 16 && a->d != 32 && a->d != 64 && a->d != 128 && a->d != 256) {

