@@ -150,7 +150,9 @@ def _local_fwd(q, k, v, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, p
 
 def _local_bwd(q, k, v, out, lse, d_out, d_lse, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, prefix):
     q, k, v, d_out = _rows(q), _rows(k), _rows(v), _rows(d_out)
-    out, lse = out.contiguous(), lse.contiguous()
+    if not out.is_contiguous() or out.data_ptr() % 16:
+        out = out.clone(memory_format=torch.contiguous_format)
+    lse = lse.contiguous()
     d_lse = None if d_lse is None else d_lse.contiguous()
     dev = q.device
     dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)

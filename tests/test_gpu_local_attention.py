@@ -283,6 +283,19 @@ def test_strides_alignment_and_views(dtype):
     assert torch.equal(o, o1)
 
 
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_backward_takes_any_layout_of_out(dtype):
+    """``out`` and ``lse`` of a merge may be views: not on a 16-byte boundary, or token major."""
+    c = Case(dtype=dtype, d=64, hq=4, h=2, nq=(90, 40), window=50, seed=24)
+    o, lse = _run(c)
+    want = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    odd = torch.empty(o.numel() + 1, dtype=dtype, device="cuda")[1:].view(o.shape).copy_(o)
+    odd_lse = torch.empty(lse.numel() + 1, device="cuda")[1:].view(lse.shape).copy_(lse)
+    for a, b in ((odd, odd_lse), (o.transpose(0, 1).contiguous().transpose(0, 1), lse.t().contiguous().t())):
+        got = fm.local_attention_backward(c.q, c.k, c.v, c.scale, a, b, c.d_out, **c.kwargs())
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_gradient_of_a_broadcast_input():
     c = Case(d=64, hq=2, h=2, nq=(100,), seed=5)
     v = c.v[:1].clone().requires_grad_()
