@@ -29,6 +29,8 @@ Prefix = Union[torch.Tensor, Sequence[int]]
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` [heads, rows, d] itself if its rows are contiguous, start on 16-byte boundaries and do not overlap, else a copy."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:             # (a row is a multiple of 16 bytes)
+        return t
     sh, st, sd = t.stride()
     e = t.element_size()
     d = t.shape[2]
@@ -131,7 +133,7 @@ def _scratch(nbytes: int, dev: torch.device) -> Optional[torch.Tensor]:
 
 def _forward(args: bytes, q: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     dev = q.device
-    o = q.new_empty(q.shape)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = q.new_empty(q.shape[:2], dtype=torch.float32)
     lib = L.lib()
     with _on(dev):
@@ -155,7 +157,7 @@ def _local_bwd(q, k, v, out, lse, d_out, d_lse, sm_scale, causal, window, softca
     lse = lse.contiguous()
     d_lse = None if d_lse is None else d_lse.contiguous()
     dev = q.device
-    dq, dk, dv = q.new_empty(q.shape), q.new_empty(k.shape), q.new_empty(v.shape)
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     args = _doc_args(q, k, v, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, prefix)
     lib = L.lib()
     with _on(dev):
