@@ -464,8 +464,10 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
         const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
         bool fine = ok && l < INFINITY && l >= 0.f;
-        // a whole tile goes out through the query tile's shared memory, which no product reads any more
-        const bool whole = ok && gridDim.y == 1 && b.t1[s] - b.t0[s] == b.tokens && b.tokens > 0;
+        // a whole tile goes out through the query tile's shared memory: with a step done, the products that read it have finished, so its
+        // load has long landed.  A tile that sees no key waits for nothing, while its load (the block's other tile sees some)
+        // may still be in flight: its zeros go straight out
+        const bool whole = ok && gridDim.y == 1 && done > 0 && b.t1[s] - b.t0[s] == b.tokens;
         if (ok && b.t0[s] < b.t1[s]) {
             unsigned char *tile = smem_dyn + s * C::kTileBytes;
 #pragma unroll

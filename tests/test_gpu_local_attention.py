@@ -427,3 +427,18 @@ def test_wrong_prefix_sums_stay_inside_the_arrays():
         o, lse = fm.local_attention(c.q, c.k, c.v, c.scale, cu_seqlens_q=t, cu_seqlens_k=t, prefix=torch.tensor([-4, 1000, 3], device="cuda"))
         fm.local_attention_backward(c.q, c.k, c.v, c.scale, torch.zeros_like(o), torch.zeros_like(lse), c.d_out, cu_seqlens_q=t, cu_seqlens_k=t)
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("nq,nk,hq,d", [(256, 100, 1, 64), (256, 100, 1, 128), (300, 70, 1, 128), (200, 40, 1, 64), (128, 50, 2, 128), (64, 20, 4, 64)])
+def test_rows_without_a_key_beside_rows_with_one(nq, nk, hq, d, dtype):
+    """A block of two query tiles, the first of them whole and blind: its rows are zero, whatever the queries hold."""
+    c = Case(dtype=dtype, d=d, hq=hq, h=1, nq=(nq,) * 6, nk=(nk,) * 6, seed=30)
+    ro, rl, to, tl = c.forward()
+    blind = torch.isinf(rl)
+    assert int(blind.sum()) == 6 * hq * (nq - nk)
+    for _ in range(20):
+        o, lse = _run(c)
+        assert (o[blind] == 0).all()
+        assert_within(lse, rl, tl, "lse")
+        assert_within(o, ro, to, "o")

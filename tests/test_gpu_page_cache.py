@@ -348,3 +348,20 @@ def test_from_the_cache_into_a_memory():
     ref = torch.softmax(s, -1) @ v.double().repeat_interleave(G, 0)
     assert (o.double() - ref).abs().max() <= 3 * 2.0 ** -8 * float(v.abs().max()) / 4
     assert (lse.double() - torch.logsumexp(s, -1)).abs().max() <= 1e-3
+
+
+@pytest.mark.parametrize("nq,nk,hq,d", [(256, 100, 1, 128), (128, 50, 2, 64)])
+def test_rows_without_a_key_beside_rows_with_one_over_pages(nq, nk, hq, d):
+    """Lengths shorter than the queries, the first query tile of a block whole and blind."""
+    case = Case(hq=hq, h=1, d=d, nq=(nq,) * 3, nk=(nk,) * 3, seed=31)
+    cache, seqs = _filled(case, 16, 5, poison=True)
+    kw = case.kwargs()
+    kw.pop("cu_seqlens_k")
+    ro, rl, to, tl = case.forward()
+    blind = torch.isinf(rl)
+    assert blind.any()
+    for _ in range(20):
+        o, lse = cache.attend(case.q, case.scale, seqs=seqs, **kw)
+        assert (o[blind] == 0).all()
+        assert_within(lse, rl, tl, "lse")
+        assert_within(o, ro, to, "o")
