@@ -29,11 +29,12 @@ Prefix = Union[torch.Tensor, Sequence[int]]
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` [heads, rows, d] itself if its rows are contiguous, start on 16-byte boundaries and do not overlap, else a copy."""
-    if t.is_contiguous() and t.data_ptr() % 16 == 0:             # (a row is a multiple of 16 bytes)
-        return t
     sh, st, sd = t.stride()
+    _, n, d = t.shape
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:             # (a row is a multiple of 16 bytes)
+        # contiguous says nothing of the stride of a dim of size one, or of an empty tensor's
+        return t if st == d and sh == n * d else t.as_strided(t.shape, (n * d, d, 1))
     e = t.element_size()
-    d = t.shape[2]
     ok = sd == 1 and (st * e) % 16 == 0 and (sh * e) % 16 == 0 and t.data_ptr() % 16 == 0 and \
         (t.shape[1] == 1 or st >= d) and (t.shape[0] == 1 or sh >= d)
     return t if ok else t.clone(memory_format=torch.contiguous_format)

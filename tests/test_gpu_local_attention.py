@@ -442,3 +442,25 @@ def test_rows_without_a_key_beside_rows_with_one(nq, nk, hq, d, dtype):
         assert (o[blind] == 0).all()
         assert_within(lse, rl, tl, "lse")
         assert_within(o, ro, to, "o")
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_strides_of_dims_of_size_one(dtype):
+    """One KV head, or one new token, cut from a buffer whose rows have an odd width."""
+    c = Case(dtype=dtype, d=64, hq=1, h=1, nq=(3,), seed=33)
+    wide = lambda t: torch.zeros(2, t.shape[1] * 64 + 1, dtype=dtype, device="cuda")[:, :-1].unflatten(1, t.shape[1:])[:1].copy_(t)
+    q, k, v, g = (wide(t) for t in (c.q, c.k, c.v, c.d_out))
+    assert q.is_contiguous() and q.stride(0) % 8
+    o, lse = _run(c)
+    o1, lse1 = fm.local_attention(q, k, v, c.scale, **c.kwargs())
+    assert torch.equal(o, o1) and torch.equal(lse, lse1)
+    want = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    assert all(torch.equal(a, b) for a, b in zip(want, fm.local_attention_backward(q, k, v, c.scale, o, lse, g, **c.kwargs())))
+    cache = fm.PagedCache(1, 64, n_pages=2, n_seqs=1, max_len=16, page_size=16, dtype=dtype)
+    cache.append([0], k, v, [0, 3])
+    one = torch.zeros(3, 1, 131, dtype=dtype, device="cuda")[:, :, :64][:1].copy_(c.q[:, 2:])
+    assert one.is_contiguous()
+    cache.append([0], one, one)
+    assert torch.equal(cache.gather([0], [0, 4])[0], torch.cat([c.k, c.q[:, 2:]], 1))
+    a, b = cache.attend(one, c.scale), cache.attend(one.clone(memory_format=torch.contiguous_format), c.scale)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))

@@ -111,3 +111,22 @@ def test_cpu_tensors_are_refused():
         fm.PagedCache(1, 64, n_pages=2, n_seqs=1, max_len=10, device="cpu")
     with pytest.raises(fm.FastMemError):
         fm.paged_attention(q, q[None], q[None], torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), 1.0)
+
+
+def _one_head(dtype=torch.bfloat16, n=3):                 # one head's rows cut from a buffer of odd width: the head stride is the buffer's
+    return torch.randn(4, n * 64 + 1).to(dtype)[:, :n * 64].unflatten(1, (n, 64))[:1]
+
+
+def _one_row(dtype=torch.bfloat16):                       # the first row of one head of a buffer of odd width
+    return torch.randn(3, 1, 131).to(dtype)[:, :, :64][:1]
+
+
+@pytest.mark.parametrize("make", [_one_head, _one_row, lambda: torch.randn(5, 7, 131)[:, :0, :64], lambda: torch.randn(3, 5, 64)[:, :1],
+                                  lambda: torch.randn(2, 9, 131)[..., :64], lambda: torch.randn(4, 6, 64).transpose(0, 1), lambda: torch.randn(2, 8, 64)])
+def test_rows_have_strides_the_library_takes(make):
+    """Any view's rows, whatever the strides of its dims of size one."""
+    from fast_memory_b200.local import _rows
+    t = make()
+    r = _rows(t)
+    assert torch.equal(r, t)
+    assert all(s * r.element_size() % 16 == 0 for s in r.stride()[:2]) and r.stride(2) == 1
