@@ -19,7 +19,7 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 from . import _lib as L
-from .local import _int32, _on, _prefix_sums, _rows, _scratch, _stream, paged_attention
+from .local import _PRE, _compiling, _included, _int32, _modes, _on, _prefix_sums, _rows, _scratch, _stream, paged_attention
 
 Seqs = Union[torch.Tensor, Sequence[int]]
 
@@ -78,6 +78,8 @@ class PagedCache:
     def _run(self, call, *args) -> None:
         """One page operation on the current stream.  Operations on a cache follow one another, so they share a
         scratch buffer (one a stream); a captured one gets its own, which lives as long as its graph."""
+        if not _compiling() and (_modes() or _included(_PRE)):
+            self._refuse_tracing()
         dev, lib = self.device, L.lib()
         with _on(dev):
             stream = _stream(dev)
@@ -89,6 +91,13 @@ class PagedCache:
             status = call(self._ref, *args, ws.data_ptr(), ws.numel(), stream)
         if status:
             L.check(status, call.__name__)
+
+    @staticmethod
+    def _refuse_tracing() -> None:
+        """A traced graph would hold nothing of a call that goes straight to the library.  (Called where a mode is active at all.)"""
+        from torch.fx.experimental.proxy_tensor import get_proxy_mode
+        if get_proxy_mode() is not None:
+            raise L.FastMemError("page operations change the cache in place and cannot be traced")
 
     def _seqs(self, seqs: Seqs, name: str = "seqs") -> torch.Tensor:
         t = _int32(seqs, self.device, name)
@@ -116,8 +125,9 @@ class PagedCache:
         if (k_new.shape[1] if cu is None else cu.numel() - 1) != seqs.numel():
             raise ValueError("cu_new must have one entry per sequence plus one (left out: one token per sequence)")
         k_new, v_new = _rows(k_new), _rows(v_new)
+        (kh, kt, _), (vh, vt, _) = k_new.stride(), v_new.stride()
         self._run(L.lib().fm_cache_append, seqs.data_ptr(), seqs.numel(), L.ptr(cu), k_new.data_ptr(), v_new.data_ptr(), k_new.shape[1],
-                  k_new.stride(0), k_new.stride(1), v_new.stride(0), v_new.stride(1))
+                  kh, kt, vh, vt)
 
     def fork(self, parents: Seqs, children: Seqs) -> None:
         """The empty sequence ``children[i]`` becomes a copy of ``parents[i]``: full pages are shared, the rows of a last page
@@ -142,6 +152,8 @@ class PagedCache:
         src, dst = _int32(src, self.device, "src"), _int32(dst, self.device, "dst")
         if src.numel() != dst.numel():
             raise ValueError("src and dst must pair up")
+        if not _compiling() and (_modes() or _included(_PRE)):
+            self._refuse_tracing()
         with _on(self.device):
             L.check(L.lib().fm_cache_copy_pages(self._ref, src.data_ptr(), dst.data_ptr(), src.numel(), _stream(self.device)),
                     "fm_cache_copy_pages")
@@ -159,6 +171,8 @@ class PagedCache:
         starts = _int32(starts, self.device, "starts", seqs.numel())
         if cu.numel() != seqs.numel() + 1:
             raise ValueError("cu must have one entry per sequence plus one")
+        if not _compiling() and (_modes() or _included(_PRE)):
+            self._refuse_tracing()
         k, v = (torch.empty(self.n_heads, n_tokens, self.d, dtype=self.k_pages.dtype, device=self.device) for _ in range(2))
         with _on(self.device):
             L.check(L.lib().fm_cache_gather(self._ref, seqs.data_ptr(), cu.data_ptr(), L.ptr(starts), seqs.numel(), n_tokens, k.data_ptr(),

@@ -21,6 +21,7 @@ import contextlib
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -30,11 +31,14 @@ Prefix = Union[torch.Tensor, Sequence[int]]
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` [heads, rows, d] itself if its rows are contiguous, start on 16-byte boundaries and do not overlap, else a copy."""
     sh, st, sd = t.stride()
-    _, n, d = t.shape
     if t.is_contiguous() and t.data_ptr() % 16 == 0:             # (a row is a multiple of 16 bytes)
+        if not (sh | st) & 7:
+            return t
         # contiguous says nothing of the stride of a dim of size one, or of an empty tensor's
-        return t if st == d and sh == n * d else t.as_strided(t.shape, (n * d, d, 1))
+        _, n, d = t.shape
+        return t.as_strided(t.shape, (n * d, d, 1))
     e = t.element_size()
+    d = t.shape[2]
     ok = sd == 1 and (st * e) % 16 == 0 and (sh * e) % 16 == 0 and t.data_ptr() % 16 == 0 and \
         (t.shape[1] == 1 or st >= d) and (t.shape[0] == 1 or sh >= d)
     return t if ok else t.clone(memory_format=torch.contiguous_format)
@@ -101,6 +105,29 @@ def _check_qkv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.devic
     if q.shape[2] not in (16, 32, 64, 128, 256):
         raise L.FastMemError(f"local attention: head dim {q.shape[2]} (16, 32, 64, 128 and 256 are built)")
     return dev
+
+
+_PRE = torch._C.DispatchKey.PreDispatch
+_included, _modes = torch._C._dispatch_tls_is_dispatch_key_included, torch._C._len_torch_dispatch_stack
+_layers, _compiling = torch._C._functorch.get_dynamic_layer_stack_depth, torch.compiler.is_compiling
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _observed(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether PyTorch has to see this call as an operator: it is traced, watched by a mode or transformed (a call that goes straight to
+    the library would leave no mark there), or the tensors are not plain ones.  (0.5 us)"""
+    if _compiling() or _modes() or _layers() or _included(_PRE):
+        return True
+    for t in tensors:
+        if t is not None and type(t) not in _PLAIN:
+            return True
+    return False
+
+
+def _refuse_tangents(*tensors: torch.Tensor) -> None:
+    """No silent loss of a forward-mode derivative: a registered operator without one drops the tangent too."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise L.FastMemError("local attention has no forward-mode derivative (backward-mode gradients only)")
 
 
 _HERE = contextlib.nullcontext()
@@ -171,6 +198,17 @@ def _local_bwd(q, k, v, out, lse, d_out, d_lse, sm_scale, causal, window, softca
     return dq, dk, dv
 
 
+def _paged_fwd(q, k_pages, v_pages, page_table, lengths, sm_scale, seqs, cu_q, causal, window, softcap, slopes, prefix):
+    q = _rows(q)
+    n_pages, H, page, d = k_pages.shape
+    args = L.pack_local_attn_args(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q.stride(0), q.stride(1), 0, 0, 0, 0, q.shape[1], 0, L.dtype_id(q.dtype), d,
+        q.shape[0], H, q.shape[1] if cu_q is None else cu_q.numel() - 1, int(window), 1 if causal else 0, float(sm_scale), float(softcap),
+        L.ptr(cu_q), 0, L.ptr(prefix), L.ptr(slopes), page_table.data_ptr(), lengths.data_ptr(), L.ptr(seqs), page_table.shape[1], n_pages, page,
+        page_table.shape[0])
+    return _forward(args, q)
+
+
 def _check_call(q, k, v, causal, window, softcap, slopes, cu_seqlens_q, cu_seqlens_k, prefix):
     dev = _check_qkv(q, k, v)
     L.dtype_id(q.dtype)
@@ -235,6 +273,19 @@ def _backward(ctx, grad_o, grad_lse):
 _local_attention_op.register_autograd(_backward, setup_context=_setup_context)
 
 
+@torch.library.custom_op("fast_memory_b200::paged_attention", mutates_args=())
+def _paged_attention_op(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
+                        sm_scale: float, seqs: Optional[torch.Tensor], cu_q: Optional[torch.Tensor], causal: bool, window: int, softcap: float,
+                        slopes: Optional[torch.Tensor], prefix: Optional[torch.Tensor]) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The operator behind :func:`paged_attention` where it is traced or a gradient is wanted: it has none and says so in the backward pass."""
+    return _paged_fwd(q, k_pages, v_pages, page_table, lengths, sm_scale, seqs, cu_q, causal, window, softcap, slopes, prefix)
+
+
+@_paged_attention_op.register_fake
+def _(q, k_pages, v_pages, page_table, lengths, sm_scale, seqs, cu_q, causal, window, softcap, slopes, prefix):
+    return q.new_empty(q.shape), q.new_empty(q.shape[:2], dtype=torch.float32)
+
+
 # ---- the functions -------------------------------------------------------------------------------------------------
 def local_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale: float, *, causal: bool = True, window: int = 0,
                     softcap: float = 0.0, slopes: Optional[torch.Tensor] = None, cu_seqlens_q: Optional[Prefix] = None,
@@ -254,7 +305,8 @@ def local_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, sm_scale:
 
     Differentiable in q, k and v through both results (:func:`local_attention_backward` is the explicit form)."""
     slopes, cu_q, cu_k, prefix = _check_call(q, k, v, causal, window, softcap, slopes, cu_seqlens_q, cu_seqlens_k, prefix)
-    if torch.compiler.is_compiling() or (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+    _refuse_tangents(q, k, v)
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) or _observed(q, k, v):
         return _local_attention_op(q, k, v, float(sm_scale), bool(causal), int(window), float(softcap), slopes, cu_q, cu_k, prefix)
     return _local_fwd(q, k, v, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, prefix)
 
@@ -268,7 +320,8 @@ def local_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     ``[Hq, S, d]`` and, where the loss reads the LSE, ``d_lse`` ``[Hq, S]`` fp32.
 
     ``out`` (q's dtype) and ``lse`` (fp32) are the result the caller ended up with - of this attention alone or merged with a
-    memory's, as :meth:`Memory.query_backward` takes them (mem:332, 354-378).  The same call gives the same bits."""
+    memory's, as :meth:`Memory.query_backward` takes them (mem:332, 354-378).  The same call gives the same bits.  The results
+    are constants to autograd."""
     slopes, cu_q, cu_k, prefix = _check_call(q, k, v, causal, window, softcap, slopes, cu_seqlens_q, cu_seqlens_k, prefix)
     L.require_cuda(q, out, lse, d_out, d_lse)
     if out.dtype != q.dtype or d_out.dtype != q.dtype:
@@ -277,6 +330,10 @@ def local_attention_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
         raise TypeError("lse and d_lse must be float32 (natural log)")
     if out.shape != q.shape or d_out.shape != q.shape or lse.shape != q.shape[:2] or (d_lse is not None and d_lse.shape != lse.shape):
         raise ValueError("out and d_out must be shaped like q, lse and d_lse [Hq, S]")
+    _refuse_tangents(q, k, v, out, lse, d_out)
+    if _observed(q, k, v, out, lse, d_out, d_lse):
+        return _local_attention_bwd_op(q, k, v, out, lse, d_out, d_lse, float(sm_scale), bool(causal), int(window), float(softcap), slopes, cu_q,
+                                       cu_k, prefix)
     return _local_bwd(q, k, v, out, lse, d_out, d_lse, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, prefix)
 
 
@@ -291,7 +348,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     :param seqs: which sequence each piece of q belongs to (left out: piece i is sequence i)
     :param prefix: per piece, the first keys that all its tokens see whatever the window
 
-    The other options are those of :func:`local_attention`.  For inference: no gradient."""
+    The other options are those of :func:`local_attention`.  For inference: a backward pass through the result raises."""
     dev = L.require_cuda(q, k_pages, v_pages, page_table, lengths)
     if q.dim() != 3 or k_pages.dim() != 4 or v_pages.shape != k_pages.shape or q.shape[2] != k_pages.shape[3]:
         raise ValueError(f"q [Hq, T, d] and pages [n_pages, H, page_size, d] are needed, got {tuple(q.shape)} {tuple(k_pages.shape)} "
@@ -300,7 +357,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise TypeError("q and the pages must share a dtype")
     if page_table.dtype != torch.int32 or lengths.dtype != torch.int32 or page_table.dim() != 2 or lengths.shape != page_table.shape[:1]:
         raise TypeError("page_table [n_seqs, width] and lengths [n_seqs] must be int32")
-    n_pages, H, page, d = k_pages.shape
+    H = k_pages.shape[1]
     if H == 0 or q.shape[0] == 0 or q.shape[0] % H:
         raise ValueError(f"{q.shape[0]} query heads do not share {H} KV heads evenly")
     for t in (k_pages, v_pages, page_table, lengths):
@@ -315,9 +372,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     slopes, prefix = _slopes(slopes, q.shape[0], dev), _int32(prefix, dev, "prefix", pieces)
     if pieces == 0:
         return torch.empty_like(q), torch.empty(q.shape[:2], dtype=torch.float32, device=dev)
-    q = _rows(q)
-    args = L.pack_local_attn_args(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), q.stride(0), q.stride(1), 0, 0, 0, 0, q.shape[1], 0, L.dtype_id(q.dtype), d,
-        q.shape[0], H, pieces, int(window), 1 if causal else 0, float(sm_scale), float(softcap), L.ptr(cu_q), 0, L.ptr(prefix), L.ptr(slopes),
-        page_table.data_ptr(), lengths.data_ptr(), L.ptr(seqs), page_table.shape[1], n_pages, page, page_table.shape[0])
-    return _forward(args, q)
+    _refuse_tangents(q, k_pages, v_pages)
+    if (torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad)) or \
+            _observed(q, k_pages, v_pages, page_table, lengths):
+        return _paged_attention_op(q, k_pages, v_pages, page_table, lengths, float(sm_scale), seqs, cu_q, bool(causal), int(window),
+                                   float(softcap), slopes, prefix)
+    return _paged_fwd(q, k_pages, v_pages, page_table, lengths, sm_scale, seqs, cu_q, causal, window, softcap, slopes, prefix)

@@ -464,3 +464,31 @@ def test_strides_of_dims_of_size_one(dtype):
     assert torch.equal(cache.gather([0], [0, 4])[0], torch.cat([c.k, c.q[:, 2:]], 1))
     a, b = cache.attend(one, c.scale), cache.attend(one.clone(memory_format=torch.contiguous_format), c.scale)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_traced_and_transformed_calls():
+    """A traced graph holds the operators and computes them again; a forward-mode derivative is refused; vmap loops."""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    c, f = Case(d=64, nq=(40, 30), hq=2, h=1, seed=34), Case(d=64, nq=(40, 30), hq=2, h=1, seed=35)
+    kw = c.kwargs()
+    cu = kw["cu_seqlens_q"]
+
+    def step(q, k, v, g, cu):
+        o, lse = fm.local_attention(q, k, v, c.scale, cu_seqlens_q=cu)
+        return (o, lse, *fm.local_attention_backward(q, k, v, c.scale, o, lse, g, cu_seqlens_q=cu))
+
+    want = step(f.q, f.k, f.v, f.d_out, cu)
+    for how in ({}, {"pre_dispatch": True}, {"tracing_mode": "fake"}):
+        graph = make_fx(step, **how)(c.q, c.k, c.v, c.d_out, cu)
+        assert all(torch.equal(a, b) for a, b in zip(graph(f.q, f.k, f.v, f.d_out, cu), want)), how
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(c.q, c.q)
+        with pytest.raises(fm.FastMemError, match="forward-mode"):
+            fm.local_attention(dual, c.k, c.v, c.scale)
+        with pytest.raises(fm.FastMemError, match="forward-mode"):
+            fm.local_attention_backward(c.q, c.k, c.v, c.scale, want[0], want[1], dual)
+    o, lse = torch.func.vmap(lambda q: fm.local_attention(q, c.k, c.v, c.scale, **kw))(torch.stack([c.q, f.q]))
+    for i, q in enumerate((c.q, f.q)):
+        o1, lse1 = fm.local_attention(q, c.k, c.v, c.scale, **kw)
+        assert torch.equal(o[i], o1) and torch.equal(lse[i], lse1)

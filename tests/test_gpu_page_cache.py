@@ -365,3 +365,43 @@ def test_rows_without_a_key_beside_rows_with_one_over_pages(nq, nk, hq, d):
         assert (o[blind] == 0).all()
         assert_within(lse, rl, tl, "lse")
         assert_within(o, ro, to, "o")
+
+
+def test_traced_attention_over_pages():
+    """A traced graph holds the operator; a backward pass through its result says that there is none; page operations are not traced."""
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    case = Case(hq=4, h=2, d=64, nq=(5, 40), nk=(30, 90), seed=36)
+    cache, seqs = _filled(case, 16, 3)
+    seqs = torch.tensor(seqs, dtype=torch.int32, device="cuda")
+    kw = case.kwargs()
+    kw.pop("cu_seqlens_k")
+    f = lambda q: cache.attend(q, case.scale, seqs=seqs, **kw)
+    q2 = case.q.flip(1).contiguous()
+    want = f(q2)
+    for how in ({}, {"pre_dispatch": True}):
+        graph = make_fx(f, **how)(case.q)
+        assert all(torch.equal(a, b) for a, b in zip(graph(q2), want))
+    o, lse = torch.compile(f, backend="aot_eager")(q2)
+    assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    leaf = q2.clone().requires_grad_()
+    o, lse = f(leaf)
+    assert torch.equal(o.detach(), want[0]) and torch.equal(lse.detach(), want[1])
+    with pytest.raises(RuntimeError, match="no autograd"):
+        o.sum().backward()
+    with torch.no_grad():
+        assert not f(leaf)[0].requires_grad
+    with forward_ad.dual_level(), pytest.raises(fm.FastMemError, match="forward-mode"):
+        f(forward_ad.make_dual(q2, q2))
+    k = torch.zeros(2, 1, 64, dtype=case.dtype, device="cuda")
+    before = cache.lengths.clone()
+    for call in (lambda t: cache.append(seqs[:1], t, t) or t, lambda t: cache.free(seqs) or t, lambda t: cache.fork(seqs, seqs) or t,
+                 lambda t: cache.compact() or t, lambda t: cache.copy_pages(seqs, seqs) or t,
+                 lambda t: cache.gather(seqs[:1], torch.tensor([0, 1], device="cuda"), n_tokens=1)[0]):
+        with pytest.raises(fm.FastMemError, match="traced"):
+            make_fx(call)(k)
+    assert torch.equal(cache.lengths, before)
+    torch.compile(lambda t: cache.append(seqs[:1], t, t), backend="aot_eager")(k)
+    before[seqs[0]] += 1
+    assert torch.equal(cache.lengths, before)
+    cache.check()

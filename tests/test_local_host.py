@@ -1,4 +1,5 @@
 """Refusals of the local attention and page cache entry points that need no GPU: every argument is checked before any CUDA call."""
+import contextlib
 import ctypes
 
 import pytest
@@ -6,6 +7,7 @@ import torch
 
 import fast_memory_b200 as fm
 from fast_memory_b200 import _lib as L
+from fast_memory_b200 import cache as cache_module
 
 FAKE = 1 << 20            # an address that is only ever compared with null
 
@@ -130,3 +132,77 @@ def test_rows_have_strides_the_library_takes(make):
     r = _rows(t)
     assert torch.equal(r, t)
     assert all(s * r.element_size() % 16 == 0 for s in r.stride()[:2]) and r.stride(2) == 1
+
+
+def test_calls_that_pytorch_has_to_see_are_noticed():
+    """Under tracing, a dispatch mode or a functorch transform a call must go by way of the registered operator."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    from fast_memory_b200.local import _observed
+    x = torch.ones(2, 3)
+    saw = []
+
+    def look(t):
+        saw.append(_observed(t))
+        return t * 2
+
+    look(x)
+    look(torch.nn.Parameter(x))
+    with torch.no_grad(), torch.device("cpu"):
+        look(x)
+    assert saw == [False] * 3
+    saw.clear()
+    make_fx(look)(x)
+    make_fx(look, pre_dispatch=True)(x)
+    make_fx(look, tracing_mode="fake")(x)
+    torch.func.vmap(look)(x)
+    torch.func.grad(lambda t: look(t).sum())(x)
+    with FlopCounterMode(display=False):
+        look(x)
+    assert saw == [True] * 6
+
+    class Sub(torch.Tensor):
+        pass
+
+    assert _observed(None, x.as_subclass(Sub))
+
+
+def test_a_forward_mode_derivative_is_refused_not_dropped():
+    from torch.autograd import forward_ad
+    from fast_memory_b200.local import _refuse_tangents
+    x = torch.ones(3)
+    with forward_ad.dual_level():
+        _refuse_tangents(x, x)                             # inside a level, but no tangent
+        with pytest.raises(fm.FastMemError, match="forward-mode"):
+            _refuse_tangents(x, forward_ad.make_dual(x, x))
+
+    def f(t):
+        _refuse_tangents(t)
+        return t
+
+    with pytest.raises(fm.FastMemError, match="forward-mode"):
+        torch.func.jvp(f, (x,), (x,))
+
+
+def test_page_operations_refuse_to_be_traced(monkeypatch):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    lib = type("Lib", (), {"fm_page_cache_workspace_bytes": lambda self, *a: 16})()
+    cache = fm.PagedCache.__new__(fm.PagedCache)
+    cache.device, cache.n_seqs, cache._ws, cache._ref, calls = torch.device("cpu"), 1, {}, b"", []
+    monkeypatch.setattr(L, "lib", lambda: lib)
+    monkeypatch.setattr(cache_module, "_on", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(cache_module, "_stream", lambda dev: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+
+    def f(t):
+        cache._run(lambda *a: calls.append(a))
+        return t * 2
+
+    f(torch.ones(1))
+    with FlopCounterMode(display=False):                   # a mode that only watches
+        f(torch.ones(1))
+    for kw in ({}, {"pre_dispatch": True}):
+        with pytest.raises(fm.FastMemError, match="traced"):
+            make_fx(f, **kw)(torch.ones(1))
+    assert len(calls) == 2
