@@ -187,6 +187,7 @@ static int local_params(const fm_local_attn_args *a, LocalParams &p)
     p.cu_q = a->cu_q; p.cu_k = a->cu_k; p.prefix = a->prefix;
     p.slopes = a->slopes; p.scale = a->sm_scale; p.cap = a->softcap;
     p.window = a->window; p.causal = a->causal != 0;
+    tc_test_hooks(p.wait_ns, p.skip_tile);
     if (a->page_table) {
         FM_REQUIRE(a->lengths && a->n_seqs > 0 && a->n_pages > 0 && a->n_pages < (int64_t(1) << 31), "paged attention: lengths, n_seqs and n_pages are needed");
         int shift = 0;

@@ -28,6 +28,10 @@ struct LocalParams {
     int table_ld, page_shift, n_pages, n_seqs;
     void *o;
     float *lse;                                      // [Hq, S]
+    // how long a pipeline wait may take before the CTA gives up and, a hook for the test of that path only, the tile of every CTA whose
+    // load is left out (-1: none)
+    uint64_t wait_ns;
+    int skip_tile;
 };
 
 struct BwdParams {

@@ -151,16 +151,17 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                         tc::tma_load_3d(s_v + c * kBlock, &tm_v, c * 64, D.k0 + j0, h, bar_addr(&sh.kv_full));
                     }
                 }
-                bool ok = true;
+                bool ok = true, tail_open = false;
                 int i = 0;
                 for (; i < n_q; ++i) {
                     const int slot = i % C::kStages, t0 = (q_lo + i) * tokens;
-                    if (i >= C::kStages) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((i / C::kStages) & 1) ^ 1, abort_flag);
+                    if (i >= C::kStages) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((i / C::kStages) & 1) ^ 1, abort_flag, p.wait_ns);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     const bool cut = t0 + tokens > D.nq;                       // the document's last queries
                     const uint32_t bar = bar_addr(cut ? &sh.tail : &sh.full[slot]);
                     const uint32_t dst = s_q0 + slot * 2 * C::kTileB;
+                    if (i == p.skip_tile) continue;                            // never, but in a test
                     if (lane == 0) {
                         tc::mbar_arrive_expect_tx(bar, 2u * (DIM / 64) * 128u * rows);
                         for (int c = 0; c < DIM / 64; ++c) {
@@ -169,8 +170,9 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                         }
                     }
                     if (cut) {
-                        ok = tc::mbar_wait_or_abort(bar, 0, abort_flag);
+                        ok = tc::mbar_wait_or_abort(bar, 0, abort_flag, p.wait_ns);
                         ok = __all_sync(0xffffffffu, ok);
+                        tail_open = !ok;
                         if (!ok) break;
                         for (int x = (D.nq - t0) * p.G * 8 + lane; x < rows * 8; x += 32)
                             for (int c = 0; c < 2 * (DIM / 64); ++c)
@@ -180,17 +182,18 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                         if (lane == 0) tc::mbar_arrive(bar_addr(&sh.full[slot]));
                     }
                 }
-                if (!ok) {
-                    if (lane == 0) *abort_flag = 1;
-                    tc::mbar_wait(bar_addr(&sh.kv_full), 0);
-                    for (int x = max(i - C::kStages, 0); x < i; ++x) tc::mbar_wait(bar_addr(&sh.full[x % C::kStages]), (x / C::kStages) & 1);
-                }
+                if (!ok && lane == 0) *abort_flag = 1;
+                // whoever gave up: every copy in flight lands before the CTA's shared memory goes away
+                tc::mbar_wait(bar_addr(&sh.kv_full), 0);
+                for (int x = max(i - C::kStages, 0); x < i; ++x)
+                    if (x != p.skip_tile) tc::mbar_wait(bar_addr(&sh.full[x % C::kStages]), (x / C::kStages) & 1);
+                if (tail_open) tc::mbar_wait(bar_addr(&sh.tail), 0);
             }
         } else if (warp == kStatWarp) {
             bool ok = true;
             for (int i = 0; i < n_q; ++i) {
                 const int buf = i & 1, t0 = (q_lo + i) * tokens;
-                if (i >= 2) ok = tc::mbar_wait_or_abort(bar_addr(&sh.stat_empty[buf]), ((i >> 1) & 1) ^ 1, abort_flag);
+                if (i >= 2) ok = tc::mbar_wait_or_abort(bar_addr(&sh.stat_empty[buf]), ((i >> 1) & 1) ^ 1, abort_flag, p.wait_ns);
                 if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
@@ -214,14 +217,14 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
             const int n = uniform(n_q);
             const bool leader = tc::elect_one();
             bool ok = true;
-            auto wait = [&](uint64_t *bar, int parity) { ok = ok && tc::mbar_wait_or_abort(bar_addr(bar), parity, abort_flag); };
+            auto wait = [&](uint64_t *bar, int parity) { ok = ok && tc::mbar_wait_or_abort(bar_addr(bar), parity, abort_flag, p.wait_ns); };
             auto q_tile = [&](int i) { return s_q0 + (i % C::kStages) * 2 * C::kTileB; };
             auto wait_q = [&](int i) { wait(&sh.full[i % C::kStages], (i / C::kStages) & 1); };
             auto product = [&](uint32_t d, uint32_t a_tile, uint32_t b_tile, uint64_t *bar) {            // S^T or dP^T
                 const uint64_t a = desc_k(a_tile, 0), b = desc_k(b_tile, 0);
 #pragma unroll
                 for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16_if(leader && ok, d, a + step_k(ks), b + step_k(ks), idesc_s, ks > 0);
-                tc::umma_commit_if(leader, bar_addr(bar));
+                tc::umma_commit_if(leader && ok, bar_addr(bar));               // (nothing is announced once a wait gave up)
             };
             auto gather = [&](uint32_t d, uint32_t a, uint32_t b_tile, bool more) {                       // dV or dK
                 const uint64_t b = desc_mn(b_tile, 0);
@@ -242,7 +245,7 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 wait(&sh.ds_full, i & 1);
                 tc::fence_after_sync();
                 gather(tm + 384, tm + 128, q_tile(i), i > 0);
-                tc::umma_commit_if(leader, bar_addr(&sh.empty[i % C::kStages]));
+                tc::umma_commit_if(leader && ok, bar_addr(&sh.empty[i % C::kStages]));
                 if (i + 1 < n) product(tm + 128, s_v, q_tile(i + 1) + C::kTileB, &sh.dp_full);
             }
             if (leader && !ok) *abort_flag = 1;
@@ -269,8 +272,8 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
             const int buf = i & 1, t0 = (q_lo + i) * tokens;
             const f32x2 dist0 = pair(float(D.nk - D.nq + t0 - j), float(D.nk - D.nq + t0 - j));
             const bool masked = !(all.x <= t0 && min(t0 + tokens, D.nq) <= all.y);
-            ok = tc::mbar_wait_or_abort(bar_addr(&sh.stat_full[buf]), (i >> 1) & 1, abort_flag) &&
-                 tc::mbar_wait_or_abort(bar_addr(&sh.s_full), i & 1, abort_flag);
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.stat_full[buf]), (i >> 1) & 1, abort_flag, p.wait_ns) &&
+                 tc::mbar_wait_or_abort(bar_addr(&sh.s_full), i & 1, abort_flag, p.wait_ns);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after_sync();
             f32x2 pr[32];                                        // P; with a cap, P times its derivative, negated (tanh^2 - 1: one operation)
@@ -322,7 +325,7 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
             tc::fence_before_sync();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(bar_addr(&sh.p_full));
-            ok = tc::mbar_wait_or_abort(bar_addr(&sh.dp_full), i & 1, abort_flag);
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.dp_full), i & 1, abort_flag, p.wait_ns);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after_sync();
             auto gradients = [&](auto with_mask) {
@@ -357,7 +360,7 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
             }
         }
         if (ok && n_q > 0) {
-            ok = tc::mbar_wait_or_abort(bar_addr(&sh.drain), 0, abort_flag);
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.drain), 0, abort_flag, p.wait_ns);
             ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
         }
         ok = tc::named_barrier_and(1, 256, ok);                                // all warps go on together
@@ -544,22 +547,24 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
                     tc::tma_load_4d(s_do + c * kBlock, &tm_do, c * 64, 0, D.q0 + t0, h, bar_addr(&sh.q_full));
                 }
             }
-            bool ok = true;
+            bool ok = true, tail_open = false;
             int i = 0;
             for (; i < 2 * n_k; ++i) {
                 const int slot = i % C::kRing, kt = key_tile(i >> 1), live = D.nk - kt * kTile;
-                if (i >= C::kRing) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((i / C::kRing) & 1) ^ 1, abort_flag);
+                if (i >= C::kRing) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((i / C::kRing) & 1) ^ 1, abort_flag, p.wait_ns);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 const bool cut = !(i & 1) && live < kTile;                     // the K tile's rows behind the last key meet dS = 0
                 const uint32_t bar = bar_addr(cut ? &sh.tail : &sh.full[slot]), dst = ring0 + slot * C::kTileB;
+                if (i == p.skip_tile) continue;                                // never, but in a test
                 if (lane == 0) {
                     tc::mbar_arrive_expect_tx(bar, C::kTileB);
                     for (int c = 0; c < DIM / 64; ++c) tc::tma_load_3d(dst + c * kBlock, (i & 1) ? &tm_v : &tm_k, c * 64, D.k0 + kt * kTile, h, bar);
                 }
                 if (cut) {
-                    ok = tc::mbar_wait_or_abort(bar, 0, abort_flag);
+                    ok = tc::mbar_wait_or_abort(bar, 0, abort_flag, p.wait_ns);
                     ok = __all_sync(0xffffffffu, ok);
+                    tail_open = !ok;
                     if (!ok) break;
                     for (int x = live * 8 + lane; x < kTile * 8; x += 32)
                         for (int c = 0; c < DIM / 64; ++c)
@@ -569,25 +574,25 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
                     if (lane == 0) tc::mbar_arrive(bar_addr(&sh.full[slot]));
                 }
             }
-            if (!ok) {
-                if (lane == 0) *abort_flag = 1;
-                tc::mbar_wait(bar_addr(&sh.q_full), 0);
-                for (int x = max(i - C::kRing, 0); x < i; ++x) tc::mbar_wait(bar_addr(&sh.full[x % C::kRing]), (x / C::kRing) & 1);
-            }
+            if (!ok && lane == 0) *abort_flag = 1;
+            if (n_k > 0) tc::mbar_wait(bar_addr(&sh.q_full), 0);
+            for (int x = max(i - C::kRing, 0); x < i; ++x)
+                if (x != p.skip_tile) tc::mbar_wait(bar_addr(&sh.full[x % C::kRing]), (x / C::kRing) & 1);
+            if (tail_open) tc::mbar_wait(bar_addr(&sh.tail), 0);
         } else if (warp == kMmaWarp && n_k > 0) {
             const uint32_t tm = uniform(int(tmem));
             const int tiles = uniform(n_k);
             const bool leader = tc::elect_one();
             bool ok = true;
-            auto wait = [&](uint64_t *bar, int parity) { ok = ok && tc::mbar_wait_or_abort(bar_addr(bar), parity, abort_flag); };
+            auto wait = [&](uint64_t *bar, int parity) { ok = ok && tc::mbar_wait_or_abort(bar_addr(bar), parity, abort_flag, p.wait_ns); };
             auto tile = [&](int i) { return ring0 + (i % C::kRing) * C::kTileB; };                        // i = 2 n: K, 2 n + 1: V
             auto product = [&](uint32_t d, uint32_t a_tile, int i, uint64_t *bar) {                       // S or dP
                 wait(&sh.full[i % C::kRing], (i / C::kRing) & 1);
                 const uint64_t a = desc_k(a_tile, 0), b = desc_k(tile(i), 0);
 #pragma unroll
                 for (int ks = 0; ks < DIM / 16; ++ks) tc::umma_f16_if(leader && ok, d, a + step_k(ks), b + step_k(ks), idesc_s, ks > 0);
-                tc::umma_commit_if(leader, bar_addr(bar));
-                if (i & 1) tc::umma_commit_if(leader, bar_addr(&sh.empty[i % C::kRing]));
+                tc::umma_commit_if(leader && ok, bar_addr(bar));               // (nothing is announced once a wait gave up)
+                if (i & 1) tc::umma_commit_if(leader && ok, bar_addr(&sh.empty[i % C::kRing]));
             };
             wait(&sh.q_full, 0);
             product(tm, s_q, 0, &sh.s_full[0]);
@@ -601,7 +606,7 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
 #pragma unroll
                 for (int ks = 0; ks < kTile / 16; ++ks)
                     tc::umma_f16_ts_if(leader && ok, tm + 384, tm + (n & 1) * 128 + (ks >> 2) * 64 + (ks & 3) * 8, k + step_mn(ks), idesc_o, n > 0 || ks > 0);
-                tc::umma_commit_if(leader, bar_addr(&sh.empty[(2 * n) % C::kRing]));
+                tc::umma_commit_if(leader && ok, bar_addr(&sh.empty[(2 * n) % C::kRing]));
                 if (n + 2 < tiles) product(tm + (n & 1) * 128, s_q, 2 * n + 4, &sh.s_full[n & 1]);
             }
             if (leader && !ok) *abort_flag = 1;
@@ -635,7 +640,7 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
             const int j0 = key_tile(n) * kTile, b = n & 1, col0 = j0 + half * 64;
             const bool masked = !(j0 + kTile <= D.prefix || (j0 >= safe_lo && j0 + kTile <= safe_hi));
             const uint32_t t_s = tmem + b * 128 + half * 64 + lanes;
-            ok = tc::mbar_wait_or_abort(bar_addr(&sh.s_full[b]), (n >> 1) & 1, abort_flag);
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.s_full[b]), (n >> 1) & 1, abort_flag, p.wait_ns);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after_sync();
             f32x2 pr[32];                                        // P; with a cap, P times its derivative, negated (tanh^2 - 1: one operation)
@@ -657,7 +662,7 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
                     pr[x * 16 + c] = CAP ? mul2(e, fma2(t[c], t[c], minus)) : e;
                 }
             }
-            ok = tc::mbar_wait_or_abort(bar_addr(&sh.dp_full), n & 1, abort_flag);
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.dp_full), n & 1, abort_flag, p.wait_ns);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after_sync();
             auto gradients = [&](auto with_mask) {
@@ -689,7 +694,7 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
             if (lane == 0) tc::mbar_arrive(bar_addr(&sh.ds_full));
         }
         if (ok && n_k > 0) {
-            ok = tc::mbar_wait_or_abort(bar_addr(&sh.drain), 0, abort_flag);
+            ok = tc::mbar_wait_or_abort(bar_addr(&sh.drain), 0, abort_flag, p.wait_ns);
             ok = __all_sync(0xffffffffu, ok) && !*abort_flag;
         }
         ok = tc::named_barrier_and(1, 256, ok);                                // all warps go on together

@@ -196,8 +196,9 @@ local_decode_kernel(const __grid_constant__ LocalParams p, const __grid_constant
                 z = min(max(p.table[int64_t(q.D.seq) * p.table_ld + (j >> p.page_shift)], 0), p.n_pages - 1) * p.H + q.h;
                 y = j & (page - 1);
             }
-            if (done >= kRing) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((done / kRing) & 1) ^ 1, abort_flag);
+            if (done >= kRing) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((done / kRing) & 1) ^ 1, abort_flag, p.wait_ns);
             if (!__all_sync(0xffffffffu, ok)) break;
+            if (done == p.skip_tile) continue;                                 // never, but in a test
             if (lane == 0) {
                 sh.piece[slot] = q;
                 tc::mbar_arrive_expect_tx(bar_addr(&sh.full[slot]), 2u * uint32_t(live) * box_rows * (D * 2));
@@ -210,7 +211,8 @@ local_decode_kernel(const __grid_constant__ LocalParams p, const __grid_constant
         }
         if (!ok && lane == 0) *abort_flag = 1;
         // nothing may still be in flight when the CTA goes
-        for (int s = max(done - kRing, 0); s < done; ++s) tc::mbar_wait(bar_addr(&sh.full[s % kRing]), (s / kRing) & 1);
+        for (int s = max(done - kRing, 0); s < done; ++s)
+            if (s != p.skip_tile) tc::mbar_wait(bar_addr(&sh.full[s % kRing]), (s / kRing) & 1);
         return;
     }
 
@@ -224,7 +226,7 @@ local_decode_kernel(const __grid_constant__ LocalParams p, const __grid_constant
     bool valid[2] = {false, false}, started = false;
     for (int it = 0; it < count; ++it) {
         const int slot = it % kRing;
-        bool ok = tc::mbar_wait_or_abort(bar_addr(&sh.full[slot]), (it / kRing) & 1, abort_flag);
+        bool ok = tc::mbar_wait_or_abort(bar_addr(&sh.full[slot]), (it / kRing) & 1, abort_flag, p.wait_ns);
         ok = tc::named_barrier_and(1, 128, ok);                                // (the warps leave together, or not at all)
         if (!ok) {
             // a wait gave up: the rest of the stretch goes row by row, parts of cut items by way of local_decode_join

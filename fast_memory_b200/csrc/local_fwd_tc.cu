@@ -244,7 +244,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         if (warp == kLoadWarp) {
             // ---- loads ----------------------------------------------------------------------------------------------------
             int issued = 0;
-            bool ok = true, met = false;
+            bool ok = true, met = false, tail_open = false;
             if (n1 > n0) {
                 if (lane < 2 && b.t0[lane] < b.t1[lane]) {
                     const int s = lane;
@@ -272,21 +272,23 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                     for (int kv = 0; kv < 2; ++kv) {
                         const int slot = issued % C::kRing;
                         const bool cut = kv == 1 && rows < kTile;                  // a V tile whose last rows must be zeroed
+                        const bool skip = issued == p.skip_tile;                   // never, but in a test
                         if (!met && (issued >= C::kRing || cut)) {
                             meet();
                             met = true;
                         }
-                        if (issued >= C::kRing) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((issued / C::kRing) & 1) ^ 1, abort_flag);
+                        if (issued >= C::kRing) ok = tc::mbar_wait_or_abort(bar_addr(&sh.empty[slot]), ((issued / C::kRing) & 1) ^ 1, abort_flag, p.wait_ns);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         const uint32_t dst = ring0 + slot * C::kTileBytes;
                         const uint32_t bar = bar_addr(cut ? &sh.tail : &sh.full[slot]);
-                        if (lane == 0) tc::mbar_arrive_expect_tx(bar, uint32_t(live) * box_rows * (D * 2));
+                        if (lane == 0 && !skip) tc::mbar_arrive_expect_tx(bar, uint32_t(live) * box_rows * (D * 2));
                         __syncwarp();
-                        if (box < live) tc::tma_load_3d(dst + col * kBlock + box * box_rows * 128, kv ? &tm_v : &tm_k, col * 64, y, z, bar);
-                        if (cut) {                                                 // at most once a CTA: the document's last tile
-                            ok = tc::mbar_wait_or_abort(bar, 0, abort_flag);
+                        if (box < live && !skip) tc::tma_load_3d(dst + col * kBlock + box * box_rows * 128, kv ? &tm_v : &tm_k, col * 64, y, z, bar);
+                        if (cut && !skip) {                                        // at most once a CTA: the document's last tile
+                            ok = tc::mbar_wait_or_abort(bar, 0, abort_flag, p.wait_ns);
                             ok = __all_sync(0xffffffffu, ok);
+                            tail_open = !ok;
                             if (!ok) break;
                             for (int i = rows * 8 + lane; i < kTile * 8; i += 32)
 #pragma unroll
@@ -302,13 +304,13 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 }
             }
             if (!met) meet();
-            if (!ok) {
-                // unwind: every copy in flight lands before the CTA's shared memory goes away
-                if (lane == 0) *abort_flag = 1;
-                for (int i = max(issued - C::kRing, 0); i < issued; ++i) tc::mbar_wait(bar_addr(&sh.full[i % C::kRing]), (i / C::kRing) & 1);
-                for (int s = 0; s < 2; ++s)
-                    if (b.t0[s] < b.t1[s]) tc::mbar_wait(bar_addr(&sh.q_full[s]), 0);
-            }
+            if (!ok && lane == 0) *abort_flag = 1;
+            // whoever gave up: every copy in flight lands before the CTA's shared memory goes away
+            for (int i = max(issued - C::kRing, 0); i < issued; ++i)
+                if (i != p.skip_tile) tc::mbar_wait(bar_addr(&sh.full[i % C::kRing]), (i / C::kRing) & 1);
+            if (tail_open) tc::mbar_wait(bar_addr(&sh.tail), 0);
+            for (int s = 0; s < 2; ++s)
+                if (n1 > n0 && b.t0[s] < b.t1[s]) tc::mbar_wait(bar_addr(&sh.q_full[s]), 0);
         } else if (warp < kLoadWarp && n1 > n0) {
             // ---- products of one query tile: S runs two steps ahead of P V -----------------------------------------------------
             const int s = warp - kMmaWarp, m0 = uniform(n0), m1 = uniform(n1);
@@ -316,9 +318,9 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
             const Steps st(b, s);
             const bool leader = tc::elect_one();
             bool ok = true;                                                    // (what the leader's waits said; the others follow the same path)
-            auto wait = [&](uint64_t *bar, int parity) { ok = ok && tc::mbar_wait_or_abort(bar_addr(bar), parity, abort_flag); };
+            auto wait = [&](uint64_t *bar, int parity) { ok = ok && tc::mbar_wait_or_abort(bar_addr(bar), parity, abort_flag, p.wait_ns); };
             auto ring_wait = [&](int i) { wait(&sh.full[i % C::kRing], (i / C::kRing) & 1); };
-            auto commit = [&](uint64_t *bar) { tc::umma_commit_if(leader, bar_addr(bar)); };
+            auto commit = [&](uint64_t *bar) { tc::umma_commit_if(leader && ok, bar_addr(bar)); };          // (nothing is announced once a wait gave up)
             const uint64_t q = desc_k(base + s * C::kTileBytes, 0);
             int sn = m0, su = 0, ns = 0, done = 0;                             // the step whose S comes next; steps issued, and multiplied with V
             // S up to two steps ahead, but no further than the tile behind `n`: the ring has to turn.  A key tile that is passed is let go of.
@@ -362,7 +364,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 }
             }
             if (leader && !ok) *abort_flag = 1;
-            commit(&sh.drain[s]);
+            tc::umma_commit_if(leader, bar_addr(&sh.drain[s]));
             tc::mbar_wait(bar_addr(&sh.drain[s]), 0);
         }
     } else {

@@ -281,6 +281,13 @@ void tc_apply_test_hooks(TcParams &p)
     p.skip_tile = g_test_skip_tile.load(std::memory_order_relaxed);
 }
 
+void tc_test_hooks(uint64_t &wait_limit_ns, int &skip_tile)
+{
+    const uint64_t limit = g_test_wait_limit_ns.load(std::memory_order_relaxed);
+    wait_limit_ns = limit ? limit : tc::kWaitLimitNs;
+    skip_tile = g_test_skip_tile.load(std::memory_order_relaxed);
+}
+
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

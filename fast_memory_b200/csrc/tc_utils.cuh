@@ -74,7 +74,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint64_
 }
 
 // The same wait that also gives up as soon as `*abort` is set (another role of the CTA failed): checked every 64 polls.
-__device__ __forceinline__ bool mbar_wait_or_abort(uint32_t bar, uint32_t parity, const volatile int *abort)
+__device__ __forceinline__ bool mbar_wait_or_abort(uint32_t bar, uint32_t parity, const volatile int *abort, uint64_t limit_ns = kWaitLimitNs)
 {
     uint64_t t0 = 0;
     for (uint32_t i = 0;; ++i) {
@@ -83,7 +83,7 @@ __device__ __forceinline__ bool mbar_wait_or_abort(uint32_t bar, uint32_t parity
             if (*abort) return false;
             const uint64_t now = global_timer_ns();
             if (t0 == 0) t0 = now;
-            else if (now - t0 > kWaitLimitNs) return false;
+            else if (now - t0 > limit_ns) return false;
         }
     }
 }
@@ -329,5 +329,7 @@ int make_tensor_map_2d(CUtensorMap *map, const void *base, int dtype, uint64_t r
 // The same with up to five dims, innermost first (dims[0] = d, box[0] = 64); stride_bytes[i] belongs to dims[i + 1].
 int make_tensor_map(CUtensorMap *map, const void *base, int dtype, int rank, const uint64_t *dims, const uint64_t *stride_bytes,
                     const uint32_t *box);
+// The limit of pipeline waits and the tile whose load every CTA leaves out (-1: none), as set by fm_test_set_tc_hooks.
+void tc_test_hooks(uint64_t &wait_limit_ns, int &skip_tile);
 
 }  // namespace fm

@@ -492,3 +492,41 @@ def test_traced_and_transformed_calls():
     for i, q in enumerate((c.q, f.q)):
         o1, lse1 = fm.local_attention(q, c.k, c.v, c.scale, **kw)
         assert torch.equal(o[i], o1) and torch.equal(lse[i], lse1)
+
+
+@pytest.mark.parametrize("skip", [0, 1])
+@pytest.mark.parametrize("name,how", [
+    ("forward and gradients", dict(nq=(300, 70), nk=(300, 400), hq=2, h=1, d=128)),
+    ("cut over CTAs", dict(nq=(200,), nk=(900,), hq=2, h=1, d=64, dtype=HF, softcap=9.0)),
+    ("few queries", dict(nq=(1, 2, 1), nk=(500, 90, 300), hq=4, h=1, d=128)),
+])
+def test_waits_that_give_up(name, how, skip):
+    """With the test hook every CTA leaves out a tile; the waits for it run out after 20 ms, the CTA unwinds and computes its rows one
+    at a time.  The results are the same to rounding, and so is the next call."""
+    import time
+    from fast_memory_b200 import _lib as L
+    c = Case(**how, seed=37)
+    kw = c.kwargs()
+    ro, rl, to, tl = c.forward()
+    want_o, want_lse = _run(c)
+    grads = c.backward(want_o, want_lse)
+    lib = L.lib()
+    torch.cuda.synchronize()
+    assert lib.fm_test_set_tc_hooks(20, skip) == 0
+    try:
+        start = time.perf_counter()
+        o, lse = fm.local_attention(c.q, c.k, c.v, c.scale, **kw)
+        torch.cuda.synchronize()
+        middle = time.perf_counter()
+        got = fm.local_attention_backward(c.q, c.k, c.v, c.scale, want_o, want_lse, c.d_out, **kw)
+        torch.cuda.synchronize()
+        end = time.perf_counter()
+    finally:
+        assert lib.fm_test_set_tc_hooks(0, -1) == 0
+    assert 0.02 <= middle - start < 1.0 and (skip or 0.04 <= end - middle) and end - middle < 1.0
+    assert_within(lse, rl, tl, "lse")
+    assert_within(o, ro, to, "o")
+    for g, (want, bound), what in zip(got, grads, ("dq", "dk", "dv")):
+        assert_within(g, want, bound, what)
+    o, lse = _run(c)
+    assert torch.equal(o, want_o) and torch.equal(lse, want_lse)
