@@ -414,7 +414,7 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                         mask_scores(x[1], run.x - j0 - 32, run.y - j0 - 32, b.D.prefix - j0 - 32, hidden);
                     };
                     if constexpr (shaped) {
-                        if (masked) mask(0u);                                  // what is hidden must not choose the formula
+                        if (masked) mask(0u);                                  // (what is hidden must not cost the short formula)
                         shape_scores<CAP, SLOPES>(p, x[0], slope2, float(pos - j0), valid);
                         shape_scores<CAP, SLOPES>(p, x[1], slope2, float(pos - j0 - 32), valid);
                     }

@@ -92,32 +92,44 @@ struct ShortTanh {
         return mul2(s, fma2(fma2(fma2(c2, u, c1), u, c0), u, k));
     }
 };
-// tanh x = 1 - 2 / (1 + e^2x): e^2x = inf gives 1, 0 gives -1.  Near 0 that difference is off by 1e-7 whatever x is, which the cap
-// multiplies: there the polynomial.
-__device__ __forceinline__ float tanh_any(float x)
+// tanh x = 1 - 2 / (1 + e^2x): e^2x = inf gives 1, 0 gives -1.
+__device__ __forceinline__ float tanh_far(float x)
 {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + fast_exp2(x * (2.f * kLog2e))));
+    return fmaf(-2.f, r, 1.f);
+}
+// Near 0 that difference is off by 1e-7 whatever x is, which the cap multiplies: there the polynomial.
+__device__ __forceinline__ float tanh_any(float x)
+{
     const float u = x * x, low = x * fmaf(fmaf(fmaf(-0.0477942206f, u, 0.13277629f), u, -0.333318823f), u, 1.f);
-    return fabsf(x) <= 0.4f ? low : fmaf(-2.f, r, 1.f);
+    return fabsf(x) <= 0.4f ? low : tanh_far(x);
 }
 
-// t = tanh(s k).  One formula for the warp, the short one if |s k| allows it in every lane that holds a row (what the others hold
-// must not choose) and k is positive and its powers stay in fp32's range.  Scores are usually small against their cap.  More tiers, a shorter
-// one up to 0.2 or a longer one up to 0.7, cost more in code than they save: chunked prompts 860 us, with this one alone 770.
+// t = tanh(s k).  Which formula a score takes follows from that score alone: up to |s k| = 0.4 the short one, else tanh_any's.  A warp whose
+// rows (valid: the lane holds one) all stay below does without the other; the bits are the same either way, so that nothing of another
+// row and nothing hidden reaches a result.  Outside of [2^-18, 2^17] k's powers leave fp32's range: there the short one gets the
+// product.  Scores are usually small against their cap.  More tiers, a shorter one up to 0.2 or a longer one up to 0.7,
+// cost more in code than they save: chunked prompts 860 us, with this one alone 770.
 __device__ __forceinline__ void cap_scores(f32x2 (&t)[16], const uint32_t (&s)[32], float k, bool valid)
 {
+    const bool folds = k >= 0x1p-18f && k <= 0x1p17f;
     float big[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < 32; c += 2) big[c >> 1 & 1] = max3(big[c >> 1 & 1], fabsf(__uint_as_float(s[c])), fabsf(__uint_as_float(s[c + 1])));
-    const float top = valid ? fmaxf(big[0], big[1]) * ((k >= 0x1p-12f && k <= 0x1p12f) ? k : INFINITY) : 0.f;
+    const float top = valid ? fmaxf(big[0], big[1]) * (folds ? k : INFINITY) : 0.f;
+    const ShortTanh tanh_pair(folds ? k : 1.f);
     if (__all_sync(0xffffffffu, top <= 0.4f)) {
-        const ShortTanh tanh_pair(k);
 #pragma unroll
         for (int c = 0; c < 16; ++c) t[c] = tanh_pair(pair(s[2 * c], s[2 * c + 1]));
     } else {
+        const float first = folds ? 1.f : k;
 #pragma unroll
-        for (int c = 0; c < 16; ++c) t[c] = pair(tanh_any(__uint_as_float(s[2 * c]) * k), tanh_any(__uint_as_float(s[2 * c + 1]) * k));
+        for (int c = 0; c < 16; ++c) {
+            const float a = __uint_as_float(s[2 * c]), b = __uint_as_float(s[2 * c + 1]);
+            const float2 low = split(tanh_pair(mul2(pair(a, b), pair(first, first))));
+            t[c] = pair(fabsf(a * k) <= 0.4f ? low.x : tanh_far(a * k), fabsf(b * k) <= 0.4f ? low.y : tanh_far(b * k));
+        }
     }
 }
 

@@ -530,3 +530,30 @@ def test_waits_that_give_up(name, how, skip):
         assert_within(g, want, bound, what)
     o, lse = _run(c)
     assert torch.equal(o, want_o) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("how", [dict(nq=(300,)), dict(nq=(300,), hq=4, h=2, dtype=HF, slopes=True), dict(nq=(3,), nk=(300,), hq=2)])
+@pytest.mark.parametrize("softcap", [2.0, 30.0])
+def test_hidden_scores_choose_no_bits(how, softcap):
+    """With a cap there are two formulas of tanh.  Keys behind a position, and queries before one, leave every bit of what does not
+    see them (is not seen by them) as it was, whether their scores are small or large."""
+    c = Case(**{"d": 128, "hq": 2, "h": 1, "softcap": softcap, "seed": 38, **how})
+    S, N = c.q.shape[1], c.k.shape[1]
+    t, j = (150, 150) if S == N else (1, N - S + 1)                # query t is the first to see key j
+    o, lse = _run(c)
+    backward = lambda: fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    dq, dk, dv = backward()
+    for factor in (40.0, 0.0):
+        was = c.k.clone()
+        c.k[:, j:] *= factor
+        o1, lse1 = _run(c)
+        dq1 = backward()[0]
+        assert torch.equal(o1[:, :t], o[:, :t]) and torch.equal(lse1[:, :t], lse[:, :t]) and torch.equal(dq1[:, :t], dq[:, :t])
+        c.k.copy_(was)
+        was = c.q.clone()
+        c.q[:, :t] *= factor
+        _, dk1, dv1 = backward()
+        assert torch.equal(dk1[:, j:], dk[:, j:]) and torch.equal(dv1[:, j:], dv[:, j:])
+        o1, lse1 = _run(c)
+        assert torch.equal(o1[:, t:], o[:, t:]) and torch.equal(lse1[:, t:], lse[:, t:])
+        c.q.copy_(was)
