@@ -10,10 +10,11 @@
 Pages are shared by reference count; which page a call takes is decided on the device (the lowest free ones), so no call reads
 anything back and every call can be captured into a CUDA graph.  A call that cannot be served - too few free pages, a sequence
 named twice or out of range, a sequence that would outgrow its table, a fork into a sequence with tokens - changes nothing and
-sets a bit that :meth:`PagedCache.check` raises for.  Calls on one cache belong on one stream.
+sets a bit that :meth:`PagedCache.check` raises for.  Calls on one cache belong on one stream; host threads may share it.
 """
 from __future__ import annotations
 
+import threading
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -74,14 +75,16 @@ class PagedCache:
                                            status.data_ptr(), self.n_pages, width, L.dtype_id(k_pages.dtype), self.d, self.n_heads,
                                            self.page_size, self.n_seqs)
         self._ws = {}
+        self._lock = threading.Lock()
 
     def _run(self, call, *args) -> None:
         """One page operation on the current stream.  Operations on a cache follow one another, so they share a
-        scratch buffer (one a stream); a captured one gets its own, which lives as long as its graph."""
+        scratch buffer (one a stream); a captured one gets its own, which lives as long as its graph.  An operation is a plan and
+        a copy that reads it: two host threads enqueue theirs one after the other."""
         if not _compiling() and (_modes() or _included(_PRE)):
             self._refuse_tracing()
         dev, lib = self.device, L.lib()
-        with _on(dev):
+        with self._lock, _on(dev):
             stream = _stream(dev)
             ws = self._ws.get(stream)
             if ws is None or torch.cuda.is_current_stream_capturing():

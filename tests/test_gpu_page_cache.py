@@ -405,3 +405,27 @@ def test_traced_attention_over_pages():
     before[seqs[0]] += 1
     assert torch.equal(cache.lengths, before)
     cache.check()
+
+
+def test_two_host_threads_share_a_cache():
+    """Both enqueue on the default stream; rows that a kernel of their own copies, pages dealt out in whatever order."""
+    import threading
+    gen = torch.Generator().manual_seed(12)
+    H, d, n, rounds = 8, 128, 40, 25
+    c = fm.PagedCache(H, d, n_pages=2 * (n * rounds // 16 + 2), n_seqs=2, max_len=n * rounds, page_size=16)
+    new = [_new(c, n * rounds, gen) for _ in range(2)]
+
+    def run(s):
+        k, v = new[s]
+        for i in range(rounds):
+            c.append([s], k[:, i * n:(i + 1) * n], v[:, i * n:(i + 1) * n], [0, n])
+
+    threads = [threading.Thread(target=run, args=(s,)) for s in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    c.check()
+    for s in range(2):
+        k, v = c.gather([s], [0, n * rounds])
+        assert torch.equal(k, new[s][0]) and torch.equal(v, new[s][1])

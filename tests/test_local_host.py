@@ -1,6 +1,8 @@
 """Refusals of the local attention and page cache entry points that need no GPU: every argument is checked before any CUDA call."""
 import contextlib
 import ctypes
+import threading
+import time
 
 import pytest
 import torch
@@ -184,16 +186,40 @@ def test_a_forward_mode_derivative_is_refused_not_dropped():
         torch.func.jvp(f, (x,), (x,))
 
 
-def test_page_operations_refuse_to_be_traced(monkeypatch):
-    from torch.fx.experimental.proxy_tensor import make_fx
-    from torch.utils.flop_counter import FlopCounterMode
+def _host_cache(monkeypatch):
+    """A cache whose operations reach their native call without a device."""
     lib = type("Lib", (), {"fm_page_cache_workspace_bytes": lambda self, *a: 16})()
     cache = fm.PagedCache.__new__(fm.PagedCache)
-    cache.device, cache.n_seqs, cache._ws, cache._ref, calls = torch.device("cpu"), 1, {}, b"", []
+    cache.device, cache.n_seqs, cache._ws, cache._ref, cache._lock = torch.device("cpu"), 1, {}, b"", threading.Lock()
     monkeypatch.setattr(L, "lib", lambda: lib)
     monkeypatch.setattr(cache_module, "_on", lambda dev: contextlib.nullcontext())
     monkeypatch.setattr(cache_module, "_stream", lambda dev: 0)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return cache
+
+
+def test_page_operations_of_two_host_threads_do_not_interleave(monkeypatch):
+    """An operation enqueues a plan and a copy that share the stream's workspace."""
+    cache, marks = _host_cache(monkeypatch), []
+
+    def call(ref, who, ws, nbytes, stream):
+        marks.append((who, "plan"))
+        time.sleep(0.002)                                  # (a native call lets other threads run)
+        marks.append((who, "copy"))
+
+    threads = [threading.Thread(target=lambda who=who: [cache._run(call, who) for _ in range(20)]) for who in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(marks) == 120
+    assert all(a[0] == b[0] and (a[1], b[1]) == ("plan", "copy") for a, b in zip(marks[::2], marks[1::2]))
+
+
+def test_page_operations_refuse_to_be_traced(monkeypatch):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils.flop_counter import FlopCounterMode
+    cache, calls = _host_cache(monkeypatch), []
 
     def f(t):
         cache._run(lambda *a: calls.append(a))
