@@ -23,6 +23,7 @@ from . import _lib as L
 from .local import _PRE, _compiling, _included, _int32, _modes, _on, _prefix_sums, _rows, _scratch, _stream, paged_attention
 
 Seqs = Union[torch.Tensor, Sequence[int]]
+_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 _STATUS = {1: "a sequence is out of range or named twice, or prefix sums do not rise", 2: "too few free pages",
            4: "a sequence would outgrow its row of the page table", 8: "a fork into a sequence that holds tokens"}
@@ -87,9 +88,9 @@ class PagedCache:
         with self._lock, _on(dev):
             stream = _stream(dev)
             ws = self._ws.get(stream)
-            if ws is None or torch.cuda.is_current_stream_capturing():
+            if ws is None or _capturing():
                 ws = _scratch(lib.fm_page_cache_workspace_bytes(self._ref, self.n_seqs), dev)
-                if not torch.cuda.is_current_stream_capturing():
+                if not _capturing():
                     self._ws[stream] = ws
             status = call(self._ref, *args, ws.data_ptr(), ws.numel(), stream)
         if status:

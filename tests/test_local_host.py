@@ -194,7 +194,7 @@ def _host_cache(monkeypatch):
     monkeypatch.setattr(L, "lib", lambda: lib)
     monkeypatch.setattr(cache_module, "_on", lambda dev: contextlib.nullcontext())
     monkeypatch.setattr(cache_module, "_stream", lambda dev: 0)
-    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(cache_module, "_capturing", lambda: False)
     return cache
 
 
