@@ -257,6 +257,7 @@ def _(q, k, v, out, lse, d_out, d_lse, sm_scale, causal, window, softcap, slopes
 
 def _setup_context(ctx, inputs, output):
     q, k, v, sm_scale, causal, window, softcap, slopes, cu_q, cu_k, prefix = inputs
+    ctx.set_materialize_grads(False)                             # a loss that does not read the LSE makes no gradient of it
     ctx.save_for_backward(q, k, v, *output, slopes, cu_q, cu_k, prefix)
     ctx.how = (sm_scale, causal, window, softcap)
 

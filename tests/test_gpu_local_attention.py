@@ -557,3 +557,18 @@ def test_hidden_scores_choose_no_bits(how, softcap):
         o1, lse1 = _run(c)
         assert torch.equal(o1[:, t:], o[:, t:]) and torch.equal(lse1[:, t:], lse[:, t:])
         c.q.copy_(was)
+
+
+def test_a_result_that_no_loss_reads_costs_nothing(monkeypatch):
+    """A loss over o alone hands the backward pass no LSE gradient (not a tensor of zeros)."""
+    from fast_memory_b200 import local
+    c = Case(d=64, nq=(90,), seed=39)
+    leaves = [t.detach().clone().requires_grad_() for t in (c.q, c.k, c.v)]
+    calls = []
+    inner = local._local_bwd
+    monkeypatch.setattr(local, "_local_bwd", lambda *a: calls.append((a[5] is None, a[6] is None)) or inner(*a))
+    o, lse = fm.local_attention(*leaves, c.scale)
+    (o * c.d_out).sum().backward(retain_graph=True)
+    lse.sum().backward(retain_graph=True)
+    (o.sum() + lse.sum()).backward()
+    assert calls == [(False, True), (False, False), (False, False)]
