@@ -5,8 +5,6 @@
 // reduction a pair: no tiles, no masks, fp32 throughout.
 #include "local_tc.cuh"
 
-#include <type_traits>
-
 namespace fm {
 
 namespace {
@@ -110,29 +108,11 @@ template <typename T, int D> __global__ void __launch_bounds__(kRowThreads) loca
 
 inline unsigned row_grid(int64_t rows) { return unsigned(ceil_div(rows * 32, kRowThreads)); }
 
-// f(T{}, std::integral_constant<int, D>{}) for the call's element type and head dim
-template <typename T, typename F> int with_dim(int d, F &&f)
-{
-    switch (d) {
-    case 16: return f(T{}, std::integral_constant<int, 16>{});
-    case 32: return f(T{}, std::integral_constant<int, 32>{});
-    case 64: return f(T{}, std::integral_constant<int, 64>{});
-    case 128: return f(T{}, std::integral_constant<int, 128>{});
-    default: return f(T{}, std::integral_constant<int, 256>{});
-    }
-}
-template <typename F> int with_type(int dtype, int d, F &&f)
-{
-    if (dtype == FM_F32) return with_dim<float>(d, f);
-    if (dtype == FM_BF16) return with_dim<__nv_bfloat16>(d, f);
-    return with_dim<__half>(d, f);
-}
-
 }  // namespace
 
 int local_combine(const LocalParams &p, int dtype, const float *part_o, const float *part_lse, int parts, cudaStream_t st)
 {
-    return with_type(dtype, p.d, [&](auto t, auto dim) -> int {
+    return with_type_and_dim(dtype, p.d, [&](auto t, auto dim) -> int {
         local_combine_kernel<decltype(t), decltype(dim)::value><<<row_grid(int64_t(p.Hq) * p.S), kRowThreads, 0, st>>>(p, part_o, part_lse, parts);
         FM_LAUNCHED("local_combine_kernel");
         return FM_OK;
@@ -141,9 +121,9 @@ int local_combine(const LocalParams &p, int dtype, const float *part_o, const fl
 
 int local_rows_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st)
 {
-    return with_type(dtype, p.d, [&](auto t, auto dim) -> int {
+    constexpr int D = 256;
+    return with_type(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        constexpr int D = decltype(dim)::value;
         if (p.S > 0) {
             local_rows_dq_kernel<T, D><<<row_grid(int64_t(p.Hq) * p.S), kRowThreads, 0, st>>>(p, g);
             FM_LAUNCHED("local_rows_dq_kernel");
@@ -281,7 +261,7 @@ int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *l
     float *delta = static_cast<float *>(workspace);
     BwdParams g{d_o, do_stride_head, do_stride_row, lse, delta, dq, dk, dv};
     if (p.S > 0) {
-        const int rc = with_type(a->dtype, p.d, [&](auto t, auto dim) -> int {
+        const int rc = with_type_and_dim(a->dtype, p.d, [&](auto t, auto dim) -> int {
             using T = decltype(t);
             constexpr int lanes = decltype(dim)::value * sizeof(T) / 16;
             local_delta_kernel<T, decltype(dim)::value><<<unsigned(ceil_div(ceil_div(int64_t(p.Hq) * p.S, kDeltaRows) * std::min(lanes, 32), kRowThreads)), kRowThreads, 0, st>>>(p, g, static_cast<const T *>(o), d_lse, delta);

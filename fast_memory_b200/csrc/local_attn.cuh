@@ -9,6 +9,8 @@
 // a key are one run: loops walk runs and never touch a hidden key or query.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "mma_utils.cuh"
 
@@ -265,7 +267,27 @@ template <typename T, int DIM> __device__ __forceinline__ void local_row_dkv(con
     dv.store(static_cast<T *>(g.dv) + row * DIM, 1.f);
 }
 
-// ---- backward a row a warp ------------------------------------------------------------------------------------------------------
+// f(T{}) for an element type, f(T{}, std::integral_constant<int, D>{}) for an element type and a head dim
+template <typename F> int with_type(int dtype, F &&f)
+{
+    if (dtype == FM_F32) return f(float{});
+    if (dtype == FM_BF16) return f(__nv_bfloat16{});
+    return f(__half{});
+}
+template <typename F> int with_type_and_dim(int dtype, int d, F &&f)
+{
+    return with_type(dtype, [&](auto t) -> int {
+        switch (d) {
+        case 16: return f(t, std::integral_constant<int, 16>{});
+        case 32: return f(t, std::integral_constant<int, 32>{});
+        case 64: return f(t, std::integral_constant<int, 64>{});
+        case 128: return f(t, std::integral_constant<int, 128>{});
+        default: return f(t, std::integral_constant<int, 256>{});
+        }
+    });
+}
+
+// ---- backward a row a warp, head dim 256 ------------------------------------------------------------------------------------------
 int local_rows_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st);
 
 }  // namespace fm

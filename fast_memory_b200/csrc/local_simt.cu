@@ -474,25 +474,6 @@ template <typename T, int D> int bwd(const LocalParams &p, const BwdParams &g, c
     return FM_OK;
 }
 
-// f(T{}, integral_constant<D>) for what the CUDA cores serve: every head dim in fp32, 16, 32 and 256 in 16 bits (64 and 128 too, where a
-// group does not fit a tensor-core tile)
-template <typename T, typename F> int with_dim(int d, F &&f)
-{
-    switch (d) {
-    case 16: return f(T{}, std::integral_constant<int, 16>{});
-    case 32: return f(T{}, std::integral_constant<int, 32>{});
-    case 64: return f(T{}, std::integral_constant<int, 64>{});
-    case 128: return f(T{}, std::integral_constant<int, 128>{});
-    default: return f(T{}, std::integral_constant<int, 256>{});
-    }
-}
-template <typename F> int with_type(int dtype, int d, F &&f)
-{
-    if (dtype == FM_F32) return with_dim<float>(d, f);
-    if (dtype == FM_BF16) return with_dim<__nv_bfloat16>(d, f);
-    return with_dim<__half>(d, f);
-}
-
 }  // namespace
 
 size_t local_simt_fwd_workspace(const LocalParams &p)
@@ -503,12 +484,12 @@ size_t local_simt_fwd_workspace(const LocalParams &p)
 
 int local_simt_fwd(const LocalParams &p, int dtype, void *ws, cudaStream_t st)
 {
-    return with_type(dtype, p.d, [&](auto t, auto dim) { return fwd<decltype(t), decltype(dim)::value>(p, ws, st); });
+    return with_type_and_dim(dtype, p.d, [&](auto t, auto dim) { return fwd<decltype(t), decltype(dim)::value>(p, ws, st); });
 }
 
 int local_simt_bwd(const LocalParams &p, const BwdParams &g, int dtype, cudaStream_t st)
 {
-    return with_type(dtype, p.d, [&](auto t, auto dim) -> int {
+    return with_type_and_dim(dtype, p.d, [&](auto t, auto dim) -> int {
         using T = decltype(t);
         constexpr int D = decltype(dim)::value;
         if constexpr (D <= 128) return bwd<T, D>(p, g, st);
