@@ -53,11 +53,12 @@ __global__ void __launch_bounds__(kRowThreads) local_combine_kernel(const __grid
     if (lane == 0) p.lse[row] = total > 0.f ? m + logf(total) : -INFINITY;
 }
 
-// delta[row] = dO . O - d_lse.  16 bytes a lane, as many lanes a row as that takes; bound by HBM, so that a lane has the loads of
+// delta[row] = dO . O - d_lse.  range (fp16 on the tensor cores): the larger of 8 max |dO| and |delta| of a row that sees a key, else 0.
+// 16 bytes a lane, as many lanes a row as that takes; bound by HBM, so that a lane has the loads of
 // several rows in flight (32 heads of 8192 rows, d = 128, bf16: 22.8 us, 90 % of the measured copy rate; a row at a time 26.5).
 constexpr int kDeltaRows = 4;
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowThreads) local_delta_kernel(LocalParams p, BwdParams g, const T *o, const float *d_lse, float *delta)
+__global__ void __launch_bounds__(kRowThreads) local_delta_kernel(LocalParams p, BwdParams g, const T *o, const float *d_lse, float *delta, float *range)
 {
     constexpr int E = 16 / sizeof(T), L = D / E < 32 ? D / E : 32, M = D / (E * L);      // elements a load, lanes a row, loads a lane and row
     const int64_t rows = int64_t(p.Hq) * p.S, w0 = (int64_t(blockIdx.x) * kRowThreads + threadIdx.x) / L * kDeltaRows;
@@ -84,7 +85,27 @@ __global__ void __launch_bounds__(kRowThreads) local_delta_kernel(LocalParams p,
         }
 #pragma unroll
         for (int i = L / 2; i; i >>= 1) x += __shfl_xor_sync(0xffffffffu, x, i);
-        if (lane == 0 && w0 + r < rows) delta[w0 + r] = x - (d_lse ? d_lse[w0 + r] : 0.f);
+        if (lane == 0 && w0 + r < rows) {
+            if (d_lse) x -= d_lse[w0 + r];
+            delta[w0 + r] = x;
+        }
+        if constexpr (std::is_same<T, __half>::value) {
+            if (range) {
+                float top = 0.f;
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    const T *t = reinterpret_cast<const T *>(&v[r][m]);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) top = fmaxf(top, fabsf(Elem<T>::to_f32(t[i])));
+                }
+#pragma unroll
+                for (int i = L / 2; i; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+                if (lane == 0 && w0 + r < rows) {
+                    top = fmaxf(8.f * top, fabsf(x));
+                    range[w0 + r] = g.lse[w0 + r] > -INFINITY && top < INFINITY ? top : 0.f;
+                }
+            }
+        }
     }
 }
 
@@ -186,8 +207,12 @@ static int local_params(const fm_local_attn_args *a, LocalParams &p)
     return FM_OK;
 }
 
-// Workspace of the backward pass: delta, then the parts of dV and dK.
+// Workspace of the backward pass: delta, the ranges, then the parts of dV and dK.
 static size_t delta_bytes(const LocalParams &p) { return align_up(size_t(p.Hq) * size_t(p.S) * sizeof(float), 256); }
+static size_t range_bytes(const LocalParams &p, int dtype)
+{
+    return dtype == FM_F16 && p.S > 0 && local_tc_fits(p, dtype) ? 2 * delta_bytes(p) : 0;
+}
 static size_t parts_bytes(const LocalParams &p, int dtype) { return p.S > 0 && local_tc_fits(p, dtype) ? local_tc_bwd_workspace(p) : 0; }
 
 static size_t forward_workspace(const LocalParams &p, int dtype)
@@ -231,7 +256,7 @@ int fm_local_attn_fwd(const fm_local_attn_args *a, void *o, float *lse, void *wo
 size_t fm_local_attn_bwd_workspace_bytes(const fm_local_attn_args *a)
 {
     fm::LocalParams p;
-    return fm::local_params(a, p) ? 0 : fm::delta_bytes(p) + fm::parts_bytes(p, a->dtype);
+    return fm::local_params(a, p) ? 0 : fm::delta_bytes(p) + fm::range_bytes(p, a->dtype) + fm::parts_bytes(p, a->dtype);
 }
 
 int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *lse, const void *d_o, int64_t do_stride_head,
@@ -248,7 +273,7 @@ int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *l
     if (p.S == 0 && p.N == 0) return FM_OK;
     FM_REQUIRE(p.S == 0 || (p.q && o && lse && d_o && dq), "fm_local_attn_bwd: null pointer");
     FM_REQUIRE(p.N == 0 || (p.k && p.v && dk && dv), "fm_local_attn_bwd: null pointer");
-    const size_t need = delta_bytes(p) + parts_bytes(p, a->dtype);
+    const size_t ranges = range_bytes(p, a->dtype), need = delta_bytes(p) + ranges + parts_bytes(p, a->dtype);
     if (need && (workspace_bytes < need || !workspace)) {
         set_error("fm_local_attn_bwd: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
         return FM_ERR_WORKSPACE;
@@ -259,18 +284,19 @@ int fm_local_attn_bwd(const fm_local_attn_args *a, const void *o, const float *l
                "fm_local_attn_bwd: rows must start on 16-byte boundaries");
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     float *delta = static_cast<float *>(workspace);
-    BwdParams g{d_o, do_stride_head, do_stride_row, lse, delta, dq, dk, dv};
+    float *range = ranges ? reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(p)) : nullptr;
+    BwdParams g{d_o, do_stride_head, do_stride_row, lse, delta, range, range ? range + delta_bytes(p) / sizeof(float) : nullptr, dq, dk, dv};
     if (p.S > 0) {
         const int rc = with_type_and_dim(a->dtype, p.d, [&](auto t, auto dim) -> int {
             using T = decltype(t);
             constexpr int lanes = decltype(dim)::value * sizeof(T) / 16;
-            local_delta_kernel<T, decltype(dim)::value><<<unsigned(ceil_div(ceil_div(int64_t(p.Hq) * p.S, kDeltaRows) * std::min(lanes, 32), kRowThreads)), kRowThreads, 0, st>>>(p, g, static_cast<const T *>(o), d_lse, delta);
+            local_delta_kernel<T, decltype(dim)::value><<<unsigned(ceil_div(ceil_div(int64_t(p.Hq) * p.S, kDeltaRows) * std::min(lanes, 32), kRowThreads)), kRowThreads, 0, st>>>(p, g, static_cast<const T *>(o), d_lse, delta, range);
             FM_LAUNCHED("local_delta_kernel");
             return FM_OK;
         });
         if (rc) return rc;
     }
-    if (p.S > 0 && local_tc_fits(p, a->dtype)) return local_tc_bwd(p, g, a->dtype, reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(p)), st);
+    if (p.S > 0 && local_tc_fits(p, a->dtype)) return local_tc_bwd(p, g, a->dtype, reinterpret_cast<float *>(static_cast<char *>(workspace) + delta_bytes(p) + ranges), st);
     return local_simt_bwd(p, g, a->dtype, st);
 }
 

@@ -40,6 +40,8 @@ struct BwdParams {
     const void *dout;
     int64_t do_sh, do_st;
     const float *lse, *delta;                        // delta = rowsum(dO * O) - d_lse
+    const float *range;                              // fp16 on the tensor cores: [Hq, S], how large a row's dP - delta gets; else null
+    float *tops;                                     // and [Hq, S] for the largest of 32 rows of a query tile, at the first of them
     void *dq, *dk, *dv;                              // [Hq, S, d], [H, N, d] twice
 };
 

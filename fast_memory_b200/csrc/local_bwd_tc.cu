@@ -21,9 +21,13 @@
 // the warpgroups run apart, took 767 us: a product with N = 64 costs 48 cycles, not 32 (shared-memory reads).
 //
 // P and dS are rounded to the element type because the products take 16-bit operands; sums are fp32 (TMEM) and rounded once.
-// scale is applied to the sums.  Rows of a tile that are not the document's are zero where a contraction runs over them; a
-// hidden NaN inside the document shows as a result that is not finite, and such rows are computed again one pair at a time, as
-// are all rows of a CTA whose pipeline wait gave up.
+// scale is applied to the sums.  fp16 has no room below 2^-14 and above 2^16: there P is held as 2^12 P, and dS times the power of two
+// that brings the largest of 8 |dO| and |delta| - of a row for dQ, of the query tiles that a CTA walks for dK - to [2^6, 2^7); the sums
+// are divided by them.  Weights keep all their bits down to 2^-26, dS down to 2^-20 of that largest, whatever size a loss gives its
+// gradient.  dQ goes first and leaves the largest of each 32 rows for dK, dV.  (16 packed documents, 16384 tokens: 8 us more than without.)
+// Rows of a tile that are not the document's are zero where a contraction runs over them; a hidden NaN inside the document shows as a
+// result that is not finite, and such rows are computed again one pair at a time, as are all rows of a CTA whose pipeline wait
+// gave up.
 #include "local_tc.cuh"
 
 #include <type_traits>
@@ -40,6 +44,15 @@ constexpr int kMmaWarp = 8, kLoadWarp = 9, kStatWarp = 10;
 template <int D> struct Bytes {
     static constexpr uint32_t kTileB = uint32_t(D / 64) * kBlock;
 };
+
+// Powers of two by which fp16 operands are held larger than they are.
+constexpr float kLogP = 12.f, kPUp = 4096.f;
+template <typename T> constexpr bool kNarrow = std::is_same<T, __half>::value;
+__device__ __forceinline__ float scale_up(float range)
+{
+    const int e = 6 - (int(__float_as_uint(range) >> 23) - 127);
+    return range < 0x1p-126f ? 1.f : __int_as_float((min(max(e, -100), 100) + 127) << 23);
+}
 
 // ======================================================= dK, dV ============================================================
 template <int D> struct DkvCfg {
@@ -59,6 +72,7 @@ template <int DIM> struct DkvShared {
     alignas(16) float lse2[2][kTile], delta[2][kTile];           // negated; delta too if there is no cap
     alignas(16) float slope2[kTile], place[kTile];               // negated slope; token of a column, from the tile's first
     alignas(16) int token[kTile];
+    float up;                                                    // dS is held times this (fp16)
 };
 
 template <typename T, int DIM, bool CAP, bool SLOPES>
@@ -191,25 +205,54 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
             }
         } else if (warp == kStatWarp) {
             bool ok = true;
+            float lse[4], delta[4], up = 1.f;
+            auto fetch = [&](int i) {                            // a tile's numbers, a tile ahead
+                const int t0 = (q_lo + i) * tokens;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int r = lane + 32 * x, token = t0 + r / p.G;
+                    lse[x] = -INFINITY;
+                    delta[x] = 0.f;
+                    if (i < n_q && r < rows && token < D.nq) {
+                        const int64_t at = int64_t(h * p.G + r % p.G) * p.S + D.q0 + token;
+                        lse[x] = g.lse[at];
+                        delta[x] = g.delta[at];
+                    }
+                }
+            };
+            fetch(0);
+            if constexpr (kNarrow<T>) {
+                float top = 0.f;
+                for (int x = lane; x < 4 * n_q; x += 32) {
+                    const int r = (x & 3) * 32, token = (q_lo + (x >> 2)) * tokens + r / p.G;
+                    if (r < rows && token < D.nq) top = fmaxf(top, g.tops[int64_t(h * p.G + r % p.G) * p.S + D.q0 + token]);
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                up = scale_up(top);
+                if (lane == 0) sh.up = up;                       // (there with the first tile's numbers)
+                up /= kPUp;
+            }
+            if (n_q > 0 && p.slopes)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int r = lane + 32 * x;
+                    if (r < rows) sh.slope2[r] = -p.slopes[h * p.G + r % p.G] * kLog2e;
+                }
             for (int i = 0; i < n_q; ++i) {
-                const int buf = i & 1, t0 = (q_lo + i) * tokens;
+                const int buf = i & 1;
                 if (i >= 2) ok = tc::mbar_wait_or_abort(bar_addr(&sh.stat_empty[buf]), ((i >> 1) & 1) ^ 1, abort_flag, p.wait_ns);
                 if (!__all_sync(0xffffffffu, ok)) break;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    const int r = lane + 32 * x, token = t0 + r / p.G, head = h * p.G + r % p.G;
-                    const bool valid = r < rows && token < D.nq;
-                    float lse = -INFINITY, delta = 0.f;
-                    if (valid) {
-                        lse = g.lse[int64_t(head) * p.S + D.q0 + token];
-                        delta = g.delta[int64_t(head) * p.S + D.q0 + token];
-                    }
-                    sh.lse2[buf][r] = lse == -INFINITY ? -INFINITY : -lse * kLog2e;          // no such row, or one that sees nothing: P = 0
-                    sh.delta[buf][r] = CAP ? delta : -delta;
-                    if (i == 0 && p.slopes && r < rows) sh.slope2[r] = -p.slopes[head] * kLog2e;
+                    const int r = lane + 32 * x;
+                    // no such row, or one that sees nothing: P = 0
+                    sh.lse2[buf][r] = lse[x] == -INFINITY ? -INFINITY : kNarrow<T> ? fmaf(-lse[x], kLog2e, kLogP) : -lse[x] * kLog2e;
+                    sh.delta[buf][r] = (CAP ? delta[x] : -delta[x]) * up;
                 }
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(bar_addr(&sh.stat_full[buf]));
+                fetch(i + 1);
             }
             if (!ok && lane == 0) *abort_flag = 1;
         } else if (warp == kMmaWarp && n_q > 0) {
@@ -328,6 +371,8 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
             ok = tc::mbar_wait_or_abort(bar_addr(&sh.dp_full), i & 1, abort_flag, p.wait_ns);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::fence_after_sync();
+            const float up = kNarrow<T> ? sh.up * ((CAP ? -1.f : 1.f) / kPUp) : 1.f;
+            const f32x2 up2 = pair(up, up);                      // of dP (fp16)
             auto gradients = [&](auto with_mask) {
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
@@ -339,7 +384,7 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                     for (int c = 0; c < 16; ++c) {
                         const f32x2 n = (c & 1) ? delta[c >> 1].y : delta[c >> 1].x;
                         const f32x2 dp = pair(s[2 * c], s[2 * c + 1]);
-                        float2 w = split(mul2(pr[x * 16 + c], CAP ? fma2(dp, minus, n) : add2(dp, n)));
+                        float2 w = split(mul2(pr[x * 16 + c], kNarrow<T> ? fma2(dp, up2, n) : CAP ? fma2(dp, minus, n) : add2(dp, n)));
                         if constexpr (decltype(with_mask)::value) {          // P = 0 is not enough: dP may be NaN there
                             w.x = (seen[x] >> (2 * c) & 1u) ? w.x : 0.f;
                             w.y = (seen[x] >> (2 * c + 1) & 1u) ? w.y : 0.f;
@@ -368,7 +413,7 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
         tc::fence_after_sync();
         // first warpgroup: dV, second: dK; a whole tile goes out through the shared memory of K or V, which no product reads any more
         bool fine = ok;
-        const float f = half ? p.scale : 1.f;
+        const float down = !kNarrow<T> || n_q == 0 ? 1.f : half ? 1.f / sh.up : 1.f / kPUp, f = (half ? p.scale : 1.f) * down;
         const bool whole = ok && j0 >= 0 && j0 + kTile <= D.nk && gridDim.y == 1;
         if (gridDim.y > 1) {
             // parts stay fp32, and local_dkv_join looks for what is not finite
@@ -382,6 +427,10 @@ local_dkv_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = ok ? 0u : 0x7fc00000u;
+                }
+                if constexpr (kNarrow<T>) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * down);
                 }
                 if (valid) {
 #pragma unroll
@@ -633,6 +682,16 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
         const int safe_lo = p.window ? shift + t1 - p.window : 0, safe_hi = n_k > 0 ? local_run(p, shift + t0, D.nk).y : 0;
         const f32x2 scale2 = pair(p.scale * kLog2e, p.scale * kLog2e), c2 = pair(p.cap * kLog2e, p.cap * kLog2e);
         const f32x2 minus = pair(-1.f, -1.f);
+        float up = 1.f;
+        if constexpr (kNarrow<T>) {
+            float top = valid ? g.range[out_row] : 0.f;
+            up = scale_up(top);
+            delta *= up;
+#pragma unroll
+            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (lane == 0 && half == 0 && valid) g.tops[out_row] = top;
+        }
+        const f32x2 up2 = CAP ? pair(-up, -up) : pair(up, up);                 // of dP (fp16)
         const f32x2 nlse = pair(-lse2, -lse2), sdelta = CAP ? pair(delta, delta) : pair(-delta, -delta), nslope = pair(-slope2, -slope2);
         const float kc = p.cap > 0.f ? p.scale / p.cap : 0.f;
         bool ok = true;
@@ -675,7 +734,7 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
                         const f32x2 dp = pair(s[2 * c], s[2 * c + 1]);
-                        float2 w = split(mul2(pr[x * 16 + c], CAP ? fma2(dp, minus, sdelta) : add2(dp, sdelta)));
+                        float2 w = split(mul2(pr[x * 16 + c], kNarrow<T> ? fma2(dp, up2, sdelta) : CAP ? fma2(dp, minus, sdelta) : add2(dp, sdelta)));
                         if constexpr (decltype(with_mask)::value) {
                             const int i = 2 * c;
                             if (!((i >= a && i < e) || i < q)) w.x = 0.f;
@@ -716,7 +775,7 @@ local_dq_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ B
 #pragma unroll
                     for (int i = 0; i < 32; ++i) o[i] = 0;
                 }
-                const bool good = put_row<T>(o, p.scale, whole ? base_ptr : nullptr, out, row, col);
+                const bool good = put_row<T>(o, kNarrow<T> ? p.scale / up : p.scale, whole ? base_ptr : nullptr, out, row, col);
                 fine = fine && good;
             }
         }
@@ -781,14 +840,14 @@ template <typename T, int DIM> int launch(const LocalParams &p, const BwdParams 
         auto *dq = local_dq_kernel<T, DIM, decltype(cap)::value, decltype(slopes)::value>;
         FM_CUDA_OK(func_attr_cached((const void *)dkv, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DkvCfg<DIM>::kSmem));
         FM_CUDA_OK(func_attr_cached((const void *)dq, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)DqCfg<DIM>::kSmem));
+        dq<<<unsigned(q_blocks), kThreads, DqCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, tm_dq, idesc_s, idesc_o);
+        FM_LAUNCHED("local_dq_kernel");
         dkv<<<dim3(unsigned(ks.blocks), unsigned(ks.parts)), kThreads, DkvCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, tm_dk, tm_dv, idesc_s, idesc_o, parts);
         FM_LAUNCHED("local_dkv_kernel");
         if (ks.parts > 1) {
             local_dkv_join<T, DIM><<<unsigned(ceil_div(int64_t(p.H) * p.N * 32, 256)), 256, 0, st>>>(p, g, parts, ks.parts);
             FM_LAUNCHED("local_dkv_join");
         }
-        dq<<<unsigned(q_blocks), kThreads, DqCfg<DIM>::kSmem, st>>>(p, g, tm_q, tm_do, tm_k, tm_v, tm_dq, idesc_s, idesc_o);
-        FM_LAUNCHED("local_dq_kernel");
         return FM_OK;
     };
     if (p.cap > 0.f) return p.slopes ? launch_mode(std::true_type{}, std::true_type{}) : launch_mode(std::true_type{}, std::false_type{});

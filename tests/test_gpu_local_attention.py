@@ -572,3 +572,33 @@ def test_a_result_that_no_loss_reads_costs_nothing(monkeypatch):
     lse.sum().backward(retain_graph=True)
     (o.sum() + lse.sum()).backward()
     assert calls == [(False, True), (False, False), (False, False)]
+
+
+@pytest.mark.parametrize("softcap", [0.0, 6.0])
+@pytest.mark.parametrize("nq,nk", [((2048,), (2048,)), ((40, 200), (1500, 900))])
+@pytest.mark.parametrize("size", [2.0 ** -18, 2.0 ** -12, 1.0, 2.0 ** 10])
+def test_fp16_gradients_of_every_size(size, nq, nk, softcap):
+    """Output gradients as losses of any scale give them.  With B = max(8 |dO|, |delta|) dS is held times more than 2^5 / B, so that a
+    subnormal one is off by up to 2^-25 / 2^5 B = 2^-30 B; P is held times 2^12: 2^-37.  The results' own last place: 2^-25."""
+    c = Case(dtype=HF, d=64, hq=2, h=1, nq=nq, nk=nk, causal=False, softcap=softcap, scale=1.0, seed=40)
+    c.q *= 0.125
+    c.d_out *= size
+    o, lse = _run(c)
+    B = max(8 * float(c.d_out.abs().max()), float((c.d_out.double() * o.double()).sum(-1).abs().max()))
+    c.tiny = lambda n: n * 2.0 ** -30 * B * c.scale
+    grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    for got, (want, bound), what in zip(grads, c.backward(o, lse), ("dq", "dk", "dv")):
+        assert_within(got, want, bound + 2.0 ** -25, what)
+
+
+def test_fp16_gradients_of_a_document_stand_alone():
+    """How large a neighbour's output gradients are changes no bit; nor do those of rows that see no key."""
+    c = Case(dtype=HF, d=128, hq=4, h=2, nq=(200, 300, 50), nk=(200, 300, 20), seed=41)
+    o, lse = _run(c)
+    backward = lambda: fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    want = backward()
+    c.d_out[:, 200:500] *= 2.0 ** 9
+    c.d_out[:, 500:530] = 60000.0                          # of the third document: blind
+    got = backward()
+    for a, b in zip(got, want):
+        assert torch.equal(a[:, :200], b[:, :200]) and torch.equal(a[:, 500:], b[:, 500:])
