@@ -47,7 +47,6 @@ template <int D> struct Bytes {
 
 // Powers of two by which fp16 operands are held larger than they are.
 constexpr float kLogP = 12.f, kPUp = 4096.f;
-template <typename T> constexpr bool kNarrow = std::is_same<T, __half>::value;
 __device__ __forceinline__ float scale_up(float range)
 {
     const int e = 6 - (int(__float_as_uint(range) >> 23) - 127);

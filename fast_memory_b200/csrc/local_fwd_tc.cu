@@ -12,8 +12,9 @@
 // both busy.  With steps of 128 keys TMEM holds one buffer of S, and a tile's softmax (2000 cycles) and products (1500 with their
 // hand-over) take turns.
 // The reference m is the maximum of the row's first step and is renewed only when a step's sum of p exceeds 2^12: the sums are
-// fp32 and P is a floating-point number (fp16 reaches 2^16), so a reference that is too small costs no accuracy.  Most steps then
-// need no maximum at all, and O is rescaled in TMEM next to never.
+// fp32 and P is a floating-point number, so a reference that is too small costs no accuracy.  Most steps then
+// need no maximum at all, and O is rescaled in TMEM next to never.  fp16, with bits down to 2^-24 and a top of 2^16, takes 1/8 of
+// the maximum and 2^15: a weight is off by 2^-28 of the largest at most, over 2^17 keys half a step of the result.
 // l sums the unrounded p; P is rounded to the element type because the second product takes 16-bit operands.
 // 32 heads of 8192 tokens, window 4096, d = 128: 400 us, 1030 TFLOP/s (63 % of cuBLAS's measured bf16 rate).  A step of both tiles takes
 // 1300 to 1600 cycles.  What is between that and the whole time: about 3000 cycles at the start and 4000 at the end of a block.
@@ -43,7 +44,8 @@ using namespace ltc;
 constexpr int kThreads = 384;
 constexpr int kMmaWarp = 8, kLoadWarp = 10;         // warp 11 completes the third warpgroup: registers are split by warpgroup
 constexpr int kStep = 64;                           // keys of a step: half a key tile
-constexpr float kMostSum = 4096.f;                  // sum of a step's p from which a row's reference is renewed
+template <typename T> constexpr float kBelow = kNarrow<T> ? 3.f : 0.f;                    // what a reference lies below the maximum
+template <typename T> constexpr float kMostSum = kNarrow<T> ? 32768.f : 4096.f;          // sum of a step's p from which it is renewed
 
 template <int D> struct Cfg {
     static constexpr uint32_t kTileBytes = uint32_t(D / 64) * kBlock;
@@ -419,16 +421,16 @@ local_fwd_kernel(const __grid_constant__ LocalParams p, const __grid_constant__ 
                         shape_scores<CAP, SLOPES>(p, x[1], slope2, float(pos - j0 - 32), valid);
                     }
                     if (masked) mask(0xff800000u);
-                    if (fresh && m == -INFINITY) m = fmaxf(row_max(x[0]), row_max(x[1])) * mul;
+                    if (fresh && m == -INFINITY) m = fmaxf(row_max(x[0]), row_max(x[1])) * mul - kBelow<T>;
                     fresh = __any_sync(0xffffffffu, m == -INFINITY);
                     const float sub = m == -INFINITY ? 0.f : m;
                     exp_scores<T>(x[0], mul, sub, t_p, sums);
                     exp_scores<T>(x[1], mul, sub, t_p + 16, sums);
                 }
                 float sum = total(sums);
-                const bool grow = sum > kMostSum;
+                const bool grow = sum > kMostSum<T>;
                 if (__any_sync(0xffffffffu, grow)) {                           // rows that have outgrown their reference get a new one
-                    const float top = fmaxf(row_max(x[0]), row_max(x[1])) * mul, f = grow ? fast_exp2(m - top) : 1.f;
+                    const float top = fmaxf(row_max(x[0]), row_max(x[1])) * mul - kBelow<T>, f = grow ? fast_exp2(m - top) : 1.f;
                     if (done > 0) {
                         // every product into O has finished: the next one waits for this step's P
                         ok = tc::mbar_wait_or_abort(bar_addr(&sh.o_done[s][buf ^ 1]), ((done - 1) >> 1) & 1, abort_flag);
