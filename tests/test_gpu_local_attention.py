@@ -604,13 +604,13 @@ def test_fp16_gradients_of_a_document_stand_alone():
         assert torch.equal(a[:, :200], b[:, :200]) and torch.equal(a[:, 500:], b[:, 500:])
 
 
-@pytest.mark.parametrize("nq,floor", [(1, 2.0 ** -40), (200, 2.0 ** -28)])
+@pytest.mark.parametrize("nq,n,heads,floor", [(1, 4096, 300, 2.0 ** -40), (200, 8192, 80, 2.0 ** -28)])
 @pytest.mark.parametrize("below", [18.3, 23.4, 26.5])
-def test_fp16_weights_far_below_the_largest(nq, floor, below):
-    """One key of weight 1 and no value, 16383 of weight 2^-below that make up the result.  A weight is off by its rounding or by
-    2^-25 of what the kernel holds 1 as: 2^15 where rows are few, 2^3 elsewhere; the result's own last place is 2^-25."""
-    n = 16384
-    c = Case(dtype=HF, d=64, hq=1, h=1, nq=(nq,), nk=(n,), causal=False, scale=1.0, seed=42)
+def test_fp16_weights_far_below_the_largest(nq, n, heads, floor, below):
+    """One key of weight 1 and no value, the others of weight 2^-below that make up the result.  A weight is off by its rounding or by
+    2^-25 of what the kernel holds 1 as: 2^15 where rows are few, 2^3 elsewhere; the result's own last place is 2^-25.  As many
+    heads as keep the kernels from cutting a row's keys into parts, which have references of their own."""
+    c = Case(dtype=HF, d=64, hq=heads, h=heads, nq=(nq,), nk=(n,), causal=False, scale=1.0, seed=42)
     c.q.zero_(), c.k.zero_()
     c.q[..., 0], c.k[:, 0, 0] = 4.0, below * 0.6931471805599453 / 4
     c.v[:, 0], c.v[:, 1:] = 0.0, c.v[:, 1:].abs() + 0.5
