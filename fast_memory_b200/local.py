@@ -56,6 +56,8 @@ def _int32(values: Optional[Prefix], dev: torch.device, name: str, count: Option
             raise TypeError(f"{name} must be a 1-d int32 or int64 tensor")
         if values.device != dev:
             raise ValueError(f"{name} is on {values.device}, the tensors are on {dev}")
+        if values.dtype is torch.int64:                           # a number out of range stays one
+            values = values.clamp(-2 ** 31, 2 ** 31 - 1)
         t = values.to(torch.int32).contiguous()
     else:
         t = torch.tensor([int(x) for x in values], dtype=torch.int32, device=dev)

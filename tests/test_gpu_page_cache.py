@@ -429,3 +429,15 @@ def test_two_host_threads_share_a_cache():
     for s in range(2):
         k, v = c.gather([s], [0, n * rounds])
         assert torch.equal(k, new[s][0]) and torch.equal(v, new[s][1])
+
+
+def test_sequence_numbers_of_64_bits():
+    gen = torch.Generator().manual_seed(13)
+    c = fm.PagedCache(1, 64, n_pages=4, n_seqs=2, max_len=32, page_size=16)
+    k, v = _new(c, 5, gen)
+    c.append(torch.tensor([1], device="cuda"), k, v, torch.tensor([0, 5], device="cuda"))
+    c.check()
+    c.free(torch.tensor([2 ** 32 + 1], device="cuda"))
+    with pytest.raises(fm.FastMemError, match="out of range"):
+        c.check()
+    assert c.lengths.tolist() == [0, 5]

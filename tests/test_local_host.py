@@ -232,3 +232,10 @@ def test_page_operations_refuse_to_be_traced(monkeypatch):
         with pytest.raises(fm.FastMemError, match="traced"):
             make_fx(f, **kw)(torch.ones(1))
     assert len(calls) == 2
+
+
+def test_wide_numbers_do_not_wrap():
+    """2^32 + 1 is no name of sequence 1."""
+    from fast_memory_b200.local import _int32
+    t = _int32(torch.tensor([2 ** 32 + 1, -2 ** 40, 7, -1, 2 ** 31]), torch.device("cpu"), "seqs")
+    assert t.dtype is torch.int32 and t.tolist() == [2 ** 31 - 1, -2 ** 31, 7, -1, 2 ** 31 - 1]
