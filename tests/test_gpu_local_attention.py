@@ -619,3 +619,60 @@ def test_fp16_weights_far_below_the_largest(nq, n, heads, floor, below):
     ro, rl, to, tl = c.forward()
     assert_within(lse, rl, tl, "lse")
     assert_within(o, ro, to + 2.0 ** -25, "o")
+
+
+@pytest.mark.parametrize("name,how", [
+    ("group of 12", dict(hq=24, h=2, nq=(50, 3), nk=(130, 90), d=128)),
+    ("group of 16, few rows", dict(hq=16, h=1, nq=(1, 1, 1), nk=(200, 70, 900), d=64, dtype=HF, window=150)),
+    ("group of 17, few rows", dict(hq=34, h=2, nq=(1, 1, 2), nk=(200, 70, 500), d=128, softcap=12.0)),
+    ("group of 40", dict(hq=40, h=1, nq=(33, 70), d=64, dtype=HF, slopes=True)),
+    ("group of 100", dict(hq=100, h=1, nq=(30,), nk=(300,), d=128, prefix=(20,), window=90)),
+    ("group of 128", dict(hq=128, h=1, nq=(9, 21), d=128, causal=False)),
+    ("group of 130", dict(hq=130, h=1, nq=(20, 5), nk=(90, 5), d=64)),
+    ("group of 40, fp32", dict(hq=40, h=1, nq=(33,), d=64, dtype=F)),
+])
+def test_many_query_heads_a_key_head(name, how):
+    """Up to 16 the kernel of few rows takes them, up to 128 a query tile, beyond that the CUDA cores."""
+    c = Case(**how, seed=43)
+    o, lse = _run(c)
+    ro, rl, to, tl = c.forward()
+    assert_within(lse, rl, tl, "lse")
+    assert_within(o, ro, to, "o")
+    grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, d_lse=c.d_lse, **c.kwargs())
+    for got, (want, bound), what in zip(grads, c.backward(o, lse, c.d_lse), ("dq", "dk", "dv")):
+        assert_within(got, want, bound, what)
+
+
+@pytest.mark.parametrize("how", [
+    dict(nq=tuple(1 + (i * 37) % 23 for i in range(700)), hq=2, h=1, d=64, prefix=tuple(i % 5 for i in range(700)), softcap=9.0, tail=11),
+    dict(nq=tuple((i * 29) % 7 if i % 90 else 400 for i in range(600)), nk=tuple((i * 31) % 9 if i % 90 else 500 for i in range(600)), hq=2, h=2, d=128,
+         dtype=HF, window=100),
+    dict(nq=tuple(1 + i % 3 for i in range(500)), nk=tuple(1 + i % 3 + i % 70 for i in range(500)), hq=4, h=1, d=128),
+])
+def test_hundreds_of_documents(how):
+    c = Case(**how, seed=44)
+    o, lse = _run(c)
+    ro, rl, to, tl = c.forward()
+    assert_within(lse, rl, tl, "lse")
+    assert_within(o, ro, to, "o")
+    grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    for got, (want, bound), what in zip(grads, c.backward(o, lse), ("dq", "dk", "dv")):
+        assert_within(got, want, bound, what)
+
+
+@pytest.mark.parametrize("how", [
+    dict(nq=(4500,), hq=2, h=1, d=128, window=2000, prefix=(300,)),
+    dict(nq=(5000,), hq=1, h=1, d=64, dtype=HF, softcap=20.0),
+    dict(nq=(700,), nk=(9000,), hq=4, h=1, d=128, slopes=True),
+    dict(nq=(3000,), hq=1, h=1, d=32, causal=False),
+    dict(nq=(1500,), nk=(2500,), hq=1, h=1, d=256, window=700),
+])
+def test_long_rows(how):
+    c = Case(**how, seed=45)
+    o, lse = _run(c)
+    ro, rl, to, tl = c.forward()
+    assert_within(lse, rl, tl, "lse")
+    assert_within(o, ro, to, "o")
+    grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    for got, (want, bound), what in zip(grads, c.backward(o, lse), ("dq", "dk", "dv")):
+        assert_within(got, want, bound, what)

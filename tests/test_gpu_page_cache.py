@@ -441,3 +441,18 @@ def test_sequence_numbers_of_64_bits():
     with pytest.raises(fm.FastMemError, match="out of range"):
         c.check()
     assert c.lengths.tolist() == [0, 5]
+
+
+@pytest.mark.parametrize("how", [
+    dict(hq=4, h=1, nq=(1,) * 31 + (400,), nk=tuple(40 + 9 * i for i in range(31)) + (900,)),            # many rows a sequence on average
+    dict(hq=2, h=2, nq=(1,) * 60 + (500,), nk=tuple(30 + 7 * i for i in range(60)) + (800,), window=120),  # few
+])
+def test_single_tokens_and_a_chunk_in_one_call(how):
+    case = Case(d=128, **how, seed=46)
+    cache, seqs = _filled(case, 32, len(case.nk), poison=True)
+    kw = case.kwargs()
+    kw.pop("cu_seqlens_k")
+    o, lse = cache.attend(case.q, case.scale, seqs=seqs, **kw)
+    ro, rl, to, tl = case.forward()
+    assert_within(lse, rl, tl, "lse")
+    assert_within(o, ro, to, "o")
