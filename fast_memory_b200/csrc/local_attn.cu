@@ -187,6 +187,9 @@ static int local_params(const fm_local_attn_args *a, LocalParams &p)
     p.n_docs = a->n_docs;
     p.cu_q = a->cu_q; p.cu_k = a->cu_k; p.prefix = a->prefix;
     p.slopes = a->slopes; p.scale = a->sm_scale; p.cap = a->softcap;
+    // A cap out of reach: what it changes of a score is less than half a bit for products up to 2^88, while scale / cap has few bits left
+    // (below 2^-126) or none.
+    if (fabsf(p.scale) <= p.cap * 0x1p-100f) p.cap = 0.f;
     p.window = a->window; p.causal = a->causal != 0;
     tc_test_hooks(p.wait_ns, p.skip_tile);
     if (a->page_table) {

@@ -676,3 +676,19 @@ def test_long_rows(how):
     grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
     for got, (want, bound), what in zip(grads, c.backward(o, lse), ("dq", "dk", "dv")):
         assert_within(got, want, bound, what)
+
+
+@pytest.mark.parametrize("dtype,nq", [(HF, 2), (BF, 300), (F, 100)])
+@pytest.mark.parametrize("cap", [1e30, 1e37, 3e38])
+def test_a_cap_out_of_reach_changes_nothing(dtype, nq, cap):
+    """(s / cap)^2 / 3 of a score is nothing in 32 bits; scale / cap, which does not fit a normal number, must not stand in its way."""
+    c = Case(dtype=dtype, d=64, hq=2, h=1, nq=(nq,), nk=(nq + 50,), scale=1e-4, seed=47)
+    c.q *= 300.0
+    c.k *= 100.0
+    o, lse = _run(c)
+    kw = dict(c.kwargs(), softcap=cap)
+    o1, lse1 = fm.local_attention(c.q, c.k, c.v, c.scale, **kw)
+    assert torch.equal(o, o1) and torch.equal(lse, lse1)
+    want = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    got = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
