@@ -175,7 +175,8 @@ __device__ __forceinline__ float local_score(const LocalParams &p, float qk, flo
 }
 
 // ---- one row by a warp: right for every type, size, stride and value ---------------------------------------------------
-// Rows whose tensor-core result is not finite come here too: 0 * NaN of a hidden key is not theirs.
+// Rows whose tensor-core result is not finite come here too: 0 * NaN of a hidden key is not theirs.  A row that turns out to be NaN as a
+// whole ends there: after a diverged step every row comes here.
 template <typename T, int DIM> __device__ __forceinline__ void local_row_forward(const LocalParams &p, const Doc &D, int head, int i)
 {
     const int h = head / p.G, pos = D.nk - D.nq + i;
@@ -202,6 +203,7 @@ template <typename T, int DIM> __device__ __forceinline__ void local_row_forward
             const float e = b == -INFINITY ? 0.f : expf(b - m);
             l += e;
             acc.axpy(e, k);
+            if (l != l) part = 2, j = hi;                      // the row is NaN, whatever comes
         }
     }
     const int64_t row = int64_t(head) * p.S + D.q0 + i;
@@ -236,7 +238,9 @@ template <typename T, int DIM> __device__ __forceinline__ void local_row_dq(cons
             for (int j = lo; j < hi; ++j) {
                 k.load(static_cast<const T *>(p.k) + local_key_row(p, D, h, j, p.k_sh, p.k_st));
                 v.load(static_cast<const T *>(p.v) + local_key_row(p, D, h, j, p.v_sh, p.v_st));
-                acc.axpy(local_pair(p, q, k, dout, v, slope, pos - j, lse, delta).y, k);
+                const float ds = local_pair(p, q, k, dout, v, slope, pos - j, lse, delta).y;
+                acc.axpy(ds, k);
+                if (ds != ds) part = 2, j = hi;
             }
         }
     }
@@ -262,6 +266,7 @@ template <typename T, int DIM> __device__ __forceinline__ void local_row_dkv(con
             const float2 pd = local_pair(p, q, k, dout, v, slope, D.nk - D.nq + i - j, lse, g.delta[row]);
             dv.axpy(pd.x, dout);
             dk.axpy(pd.y, q);
+            if (pd.x != pd.x) head = (h + 1) * p.G, i = run.y;  // (then pd.y is NaN too)
         }
     }
     const int64_t row = int64_t(h) * p.N + D.k0 + j;

@@ -692,3 +692,21 @@ def test_a_cap_out_of_reach_changes_nothing(dtype, nq, cap):
     want = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
     got = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **kw)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_diverged_step_ends_soon():
+    """Queries that are all NaN make every row NaN, and each ends with its first key (all keys a row one at a time: 35 and 110 ms)."""
+    c = Case(d=128, hq=8, h=8, nq=(4096,), window=2048, seed=48)
+    o, lse = _run(c)
+    fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    c.q.fill_(float("nan"))
+    kw = c.kwargs()
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    torch.cuda.synchronize()
+    a.record()
+    o, lse = fm.local_attention(c.q, c.k, c.v, c.scale, **kw)
+    grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **kw)
+    b.record()
+    torch.cuda.synchronize()
+    assert all(torch.isnan(t).all() for t in (o, lse, *grads))
+    assert a.elapsed_time(b) < 20.0
