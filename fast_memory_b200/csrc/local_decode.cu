@@ -1,7 +1,7 @@
 // Local attention of few queries a document over many keys - single new tokens, short drafts -, 16-bit types, head dim 64 or 128.
 //
-// Bound by HBM: every visible key and value is read once for all heads of its group, and a block has at most 16 rows (token x
-// head of the group), one m16n8k16 tile.  What matters is that every SM always has loads in flight and that all end together:
+// Bound by HBM: a block has at most 16 rows (token x head of the group), one m16n8k16 tile, and every key and value that a block sees
+// is read once for all heads of its group; a document of more rows has several blocks, which read its keys each.  What matters is that every SM always has loads in flight and that all end together:
 //   * the key tiles (64 keys) of all (document, KV head, row block) items form ONE list that is cut into equal stretches, one a CTA
 //     and two CTAs an SM, wherever that falls; an item that is cut leaves normalised partial rows, which local_decode_join adds up
 //     in a fixed order (no atomics)
@@ -542,7 +542,10 @@ template <typename T, int D> int launch(const LocalParams &p, int dtype, void *w
 
 }  // namespace
 
-// Up to 16 rows a document on average: a row block of the other kernel would be seven eighths empty.
+// Up to 16 rows a document on average, which is all that the host knows: a row block of the other kernel would be seven eighths empty.  64
+// documents of one token over 8192 keys, 32 over 8 heads: 374 us, the other 429; of 4 tokens 374 and 433; of 8 tokens (two blocks) 668
+// and 434.  The mean misses unequal documents: 300 single tokens over 2048 keys beside a prompt of 3500 over 8192, 8 heads,
+// take 1393 us here and would take 690 there; 63 single tokens beside a chunk of 1024 go there, 549 us (here 1425).
 bool local_decode_fits(const LocalParams &p, int dtype)
 {
     return local_tc_fits(p, dtype) && p.G <= kRows && int64_t(p.S) * p.G <= int64_t(kRows) * p.n_docs;

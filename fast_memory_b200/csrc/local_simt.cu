@@ -1,6 +1,7 @@
 // Local attention on the CUDA cores, fp32 arithmetic throughout: fp32 inputs, and the head dims the tensor-core kernels are not
-// built for.  64 x 64 tiles in shared memory, 256 threads, 4 x 4 products a thread (4 x d/16 in the second products): bound by
-// fp32 FMA issue and, close behind, shared-memory bandwidth (8 16-byte loads for 64 FMAs).
+// built for.  64 x 64 tiles in shared memory, 256 threads, 4 x 4 products a thread (4 x d/16 in the second products).  Bound by latency:
+// two CTAs fit an SM (registers), 14 warps of them are there on average, and a tile's four barriers separate its loads from its
+// products; the FMA pipe is at 34 % of its issue rate, with shared memory (8 16-byte loads for 64 FMAs) the next most waited for.
 //
 //   forward   block = 64 tokens of one head; a key tile: S = Q K^T, running maximum over 16 threads by shuffles, P through shared
 //             memory, O += P V.  K and V take turns in one buffer, so that two or three CTAs of an SM cover each other's loads.
@@ -10,7 +11,7 @@
 //   dQ        block = 64 tokens of one head over the key tiles;  dK, dV: block = 64 keys of one KV head over the query tiles of
 //             every head of its group.  No atomics.
 // Rows that are not the document's are zero in the tiles; results that are not finite are computed again a pair at a time.
-// One head, fp32, d = 64, the last 512 of 4096 positions: 37 us with the join (a warp a row and no tiles: 1880 us).
+// One head, fp32, d = 64, the last 512 of 4096 positions: 37 us a call, 28 of them here and 6 in the join (a warp a row and no tiles: 1880 us).
 #include "local_attn.cuh"
 #include "local_tc.cuh"
 

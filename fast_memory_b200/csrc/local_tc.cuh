@@ -130,6 +130,7 @@ __device__ __forceinline__ void cap_scores(f32x2 (&t)[16], const uint32_t (&s)[3
         const float first = folds ? 1.f : k;
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
+            asm volatile("" ::: "memory");                                     // a pair at a time: interleaved, this branch costs the usual one registers
             const float a = __uint_as_float(s[2 * c]), b = __uint_as_float(s[2 * c + 1]);
             const float2 low = split(tanh_pair(mul2(pair(a, b), pair(first, first))));
             t[c] = pair(fabsf(a * k) <= 0.4f ? low.x : tanh_far(a * k), fabsf(b * k) <= 0.4f ? low.y : tanh_far(b * k));
