@@ -274,6 +274,16 @@ template <typename T, int DIM> __device__ __forceinline__ void local_row_dkv(con
     dv.store(static_cast<T *>(g.dv) + row * DIM, 1.f);
 }
 
+// The same as calls: what a kernel of few microseconds next to never does must not fill its instruction cache.
+template <typename T, int DIM> __device__ __noinline__ void local_row_forward_call(const LocalParams &p, const Doc &D, int head, int i)
+{
+    local_row_forward<T, DIM>(p, D, head, i);
+}
+template <typename T, int DIM> __device__ __noinline__ void local_row_dkv_call(const LocalParams &p, const BwdParams &g, const Doc &D, int h, int j)
+{
+    local_row_dkv<T, DIM>(p, g, D, h, j);
+}
+
 // f(T{}) for an element type, f(T{}, std::integral_constant<int, D>{}) for an element type and a head dim
 template <typename F> int with_type(int dtype, F &&f)
 {

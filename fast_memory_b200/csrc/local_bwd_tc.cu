@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(256) local_dkv_join(const __grid_constant__ Lo
     if (__any_sync(0xffffffffu, worst != 0.f)) {
         const int r = int(row % p.N);
         const Doc doc = local_doc<true>(p, p.cu_k ? local_find(p.cu_k, p.n_docs, r) : 0);
-        local_row_dkv<T, DIM>(p, g, doc, int(row / p.N), r - doc.k0);
+        local_row_dkv_call<T, DIM>(p, g, doc, int(row / p.N), r - doc.k0);
     }
 }
 

@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(32 * kRows) local_decode_join(const __grid_con
     __syncthreads();
     if (mine > 0) return;
     if (bad) {
-        local_row_forward<T, D>(p, cut.D, head, token);
+        local_row_forward_call<T, D>(p, cut.D, head, token);
         return;
     }
     for (int i = 1; i < n; ++i) {
