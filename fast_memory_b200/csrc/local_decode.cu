@@ -14,7 +14,7 @@
 // P is rounded to the element type as the operand of the second product; sums are fp32.  In fp16 the reference of a row is 2^-15 of its
 // running maximum, so that P fills the type's range: a weight is off by 2^-40 of the largest at most, or by its rounding.
 // 64 sequences of up to 16384 tokens, 32 over 8 heads, d = 128: 366 us, 98 % of the measured copy rate; one of 131072: 91 us (90 %) and
-// 7 us for the join.  The tcgen05 forward, its key tiles cut over CTAs, took 534 and 135 us.
+// 6.5 us for the join.  The tcgen05 forward, its key tiles cut over CTAs, took 534 and 135 us.
 #include "local_tc.cuh"
 
 #include <type_traits>

@@ -16,7 +16,7 @@
 // need no maximum at all, and O is rescaled in TMEM next to never.  fp16, with bits down to 2^-24 and a top of 2^16, takes 1/8 of
 // the maximum and 2^15: a weight is off by 2^-28 of the largest at most, over 2^17 keys half a step of the result.
 // l sums the unrounded p; P is rounded to the element type because the second product takes 16-bit operands.
-// 32 heads of 8192 tokens, window 4096, d = 128: 400 us, 1030 TFLOP/s (63 % of cuBLAS's measured bf16 rate).  A step of both tiles takes
+// 32 heads of 8192 tokens, window 4096, d = 128: 385 to 400 us, 1030 TFLOP/s and more (63 % of cuBLAS's measured bf16 rate).  A step of both tiles takes
 // 1300 to 1600 cycles.  What is between that and the whole time: about 3000 cycles at the start and 4000 at the end of a block.
 //
 //   warps 0-3, 4-7   softmax and epilogue of tile 0, 1 (a warp reaches its own quarter of the TMEM lanes).  Two threads a row

@@ -10,8 +10,9 @@
 // tables) and, where rows move, a copy kernel over the whole chip that reads the plan.  A plan that fails a check sets its
 // bit in the status word and changes nothing, and its copy kernel finds `go` = 0.  The plan is bound by latency: two sweeps
 // over the refcounts, 32 warps side by side, one ballot for 32 pages.  The copies are bound by HBM: 16 bytes a thread.
-// 64 sequences of 4096 tokens, 8 heads, d = 128: evicting half, compacting and admitting new ones, twice over, 442 us (83 % of the
-// measured copy rate with the plans between); one token for each of 64 forks, 36 us for three calls, most of it the host's.
+// 64 sequences of 4096 tokens, 8 heads, d = 128: evicting half, compacting and admitting new ones, twice over, 440-448 us (83 % of the
+// measured copy rate with the plans between); one token for each of 64 forks, 37-39 us for three calls, most of it the host's;
+// gathering 64 sequences 339 us (97 %).
 #include "common.cuh"
 
 namespace fm {
