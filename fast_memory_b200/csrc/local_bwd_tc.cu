@@ -22,9 +22,9 @@
 //
 // P and dS are rounded to the element type because the products take 16-bit operands; sums are fp32 (TMEM) and rounded once.
 // scale is applied to the sums.  fp16 has no room below 2^-14 and above 2^16: there P is held as 2^12 P, and dS times the power of two
-// that brings the largest of 8 |dO| and |delta| - of a row for dQ, of the query tiles that a CTA walks for dK - to [2^6, 2^7); the sums
-// are divided by them.  Weights keep all their bits down to 2^-26, dS down to 2^-20 of that largest, whatever size a loss gives its
-// gradient.  dQ goes first and leaves the largest of each 32 rows for dK, dV.  (16 packed documents, 16384 tokens: 8 us more than without.)
+// that brings the largest of 8 |dO| and |delta| - of a row for dQ, of the query tiles that a CTA walks for dK - into [2^6, 2^13); the
+// sums are divided by them.  Weights keep all their bits down to 2^-26, dS down to 2^-20 of that largest or further, whatever size a
+// loss gives its gradient; dP - delta may be 2^3 times that largest before a dS overflows (values of 20 and more).  dQ goes first and leaves the largest of each 32 rows for dK, dV.  (16 packed documents, 16384 tokens: 8 us more than without.)
 // Rows of a tile that are not the document's are zero where a contraction runs over them; a hidden NaN inside the document shows as a
 // result that is not finite, and such rows are computed again one pair at a time, as are all rows of a CTA whose pipeline wait
 // gave up.
@@ -49,8 +49,9 @@ template <int D> struct Bytes {
 constexpr float kLogP = 12.f, kPUp = 4096.f;
 __device__ __forceinline__ float scale_up(float range)
 {
-    const int e = 6 - (int(__float_as_uint(range) >> 23) - 127);
-    return range < 0x1p-126f ? 1.f : __int_as_float((min(max(e, -100), 100) + 127) << 23);
+    const int e = int(__float_as_uint(range) >> 23) - 127;                     // range lies in [2^e, 2^(e + 1))
+    const int up = e < 6 ? min(6 - e, 100) : e > 12 ? max(12 - e, -100) : 0;
+    return range < 0x1p-126f ? 1.f : __int_as_float((up + 127) << 23);
 }
 
 // ======================================================= dK, dV ============================================================

@@ -710,3 +710,15 @@ def test_a_diverged_step_ends_soon():
     torch.cuda.synchronize()
     assert all(torch.isnan(t).all() for t in (o, lse, *grads))
     assert a.elapsed_time(b) < 20.0
+
+
+@pytest.mark.parametrize("nq,nk", [((1,), (268,)), ((3, 40), (200, 90))])
+@pytest.mark.parametrize("size", [1.0, 64.0])
+def test_fp16_gradients_of_keys_that_weigh_little(size, nq, nk):
+    """Output gradients of usual size leave dS as it is: what is subnormal is off by 2^-25 and no more, however large others are."""
+    c = Case(dtype=HF, d=128, hq=4, h=2, nq=nq, nk=nk, scale=1.0, seed=49)
+    c.d_out *= size
+    o, lse = _run(c)
+    grads = fm.local_attention_backward(c.q, c.k, c.v, c.scale, o, lse, c.d_out, **c.kwargs())
+    for got, (want, bound), what in zip(grads, c.backward(o, lse), ("dq", "dk", "dv")):
+        assert_within(got, want, bound + 2.0 ** -25, what)
