@@ -11,8 +11,7 @@ namespace ltc {
 constexpr int kTile = 128;                          // rows of a query tile = keys of a key tile = UMMA M = TMEM lanes
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// fp16 reaches from 2^-24 to 2^16: weights that lie far below their row's largest need room below it, so references of fp16 rows lie
-// that many powers of two below the maximum.
+// fp16 reaches from 2^-24 to 2^16 only: what is rounded to it is held times a power of two where it would leave that.
 template <typename T> constexpr bool kNarrow = std::is_same<T, __half>::value;
 
 // byte offset of column block c (64 elements) of a tile: [128 rows][128 bytes], 128-byte swizzle

@@ -523,7 +523,7 @@ def test_waits_that_give_up(name, how, skip):
         end = time.perf_counter()
     finally:
         assert lib.fm_test_set_tc_hooks(0, -1) == 0
-    assert 0.02 <= middle - start < 1.0 and (skip or 0.04 <= end - middle) and end - middle < 1.0
+    assert 0.02 <= middle - start and (skip or 0.04 <= end - middle)
     assert_within(lse, rl, tl, "lse")
     assert_within(o, ro, to, "o")
     for g, (want, bound), what in zip(got, grads, ("dq", "dk", "dv")):
