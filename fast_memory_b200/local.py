@@ -164,7 +164,7 @@ def _scratch(nbytes: int, dev: torch.device) -> Optional[torch.Tensor]:
 def _forward(args: bytes, q: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     dev = q.device
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = q.new_empty(q.shape[:2], dtype=torch.float32)
+    lse = torch.empty(o.size(0), o.size(1), dtype=torch.float32, device=dev)
     lib = L.lib()
     with _on(dev):
         nbytes = lib.fm_local_attn_workspace_bytes(args)
