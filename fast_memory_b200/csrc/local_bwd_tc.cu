@@ -24,7 +24,8 @@
 // scale is applied to the sums.  fp16 has no room below 2^-14 and above 2^16: there P is held as 2^12 P, and dS times the power of two
 // that brings the largest of 8 |dO| and |delta| - of a row for dQ, of the query tiles that a CTA walks for dK - into [2^6, 2^13); the
 // sums are divided by them.  Weights keep all their bits down to 2^-26, dS down to 2^-20 of that largest or further, whatever size a
-// loss gives its gradient; dP - delta may be 2^3 times that largest before a dS overflows (values of 20 and more).  dQ goes first and leaves the largest of each 32 rows for dK, dV.  (16 packed documents, 16384 tokens: 8 us more than without.)
+// loss gives its gradient; dP - delta may be 2^3 times that largest before a dS overflows (values of 20 and more).  dQ goes first and
+// leaves the largest of each 32 rows for dK, dV.  (16 packed documents, 16384 tokens: 8 us more than without.)
 // Rows of a tile that are not the document's are zero where a contraction runs over them; a hidden NaN inside the document shows as a
 // result that is not finite, and such rows are computed again one pair at a time, as are all rows of a CTA whose pipeline wait
 // gave up.
